@@ -413,6 +413,58 @@ int msb_softmax_grad3d_f32(float *dst, const float *src, const float *label, int
                            int64_t ld_label, int mode, float ignore_label, float alpha,
                            msb_stream_t stream);
 
+/* ---- the vocabulary table's two ends (language models) ------------------------------- */
+
+/* Element types of the entries below, as `dtype`: mshadow's type tags (mshadow/base.h), here
+   MSB_FLOAT32 = 0, MSB_FLOAT16 = 2 and MSB_BFLOAT16 = 12.
+
+   `workspace` of the entries below: device memory of at least the size that the matching
+   ..._workspace() call reports, used by the call until it completes on its stream; NULL takes the
+   stream's scratch memory (see the conventions above).  A call that is captured into a graph must
+   bring its own workspace (MSB_ERR_ARGUMENT otherwise), and graphs whose replays may overlap must
+   not share one. */
+enum { MSB_FLOAT32 = 0, MSB_FLOAT16 = 2, MSB_BFLOAT16 = 12 };
+
+/* dst[i] = scale * table[index[i]], a row of zeros where index[i] is outside [0, rows): the
+   look-up of take() (mshadow/extension/take.h) for three element types, with a scale, and with
+   indices that name no row (padding; rows held by another GPU) instead of clipped ones. */
+int msb_embed_take(void *dst, const void *table, const int32_t *index, int64_t n, int64_t rows,
+                   int64_t width, int64_t ld_dst, int64_t ld_table, int dtype, float scale,
+                   msb_stream_t stream);
+/* Its gradient, dst[r] = or += scale * sum of src[i] over index[i] == r (saver 0: every row of dst is
+   written, saver 1: rows that are not named stay as they are).  Sums in binary32 over the
+   sorted indices, rounded once; AddTakeGrad (mshadow/tensor_gpu-inl.h:216-221) for three types, without
+   clipping.  Equal calls give equal bits. */
+int msb_embed_take_grad_workspace(int64_t n, int64_t width, int64_t *bytes);
+int msb_embed_take_grad(void *dst, const void *src, const int32_t *index, int64_t n, int64_t rows,
+                        int64_t width, int64_t ld_dst, int64_t ld_src, int dtype, float scale,
+                        int saver, void *workspace, int64_t workspace_bytes, msb_stream_t stream);
+
+/* Softmax cross entropy of a linear layer without its logits: z = data . weight^T (n x v),
+   lse = log sum exp z,
+   loss = lse - (1 - smooth) z[label] - smooth / (v - 1) * (sum over the other classes of z).
+   data (n x h) and weight (v x h) are MSB_FLOAT16 or MSB_BFLOAT16 (`dtype`), loss and lse
+   binary32.  A token whose label equals ignore_label or lies outside [0, v) contributes nothing:
+   loss and lse 0.  The reference composes this from a matrix product, Softmax and a loss layer
+   (mshadow/tensor_gpu-inl.h:157-161). */
+int msb_linear_softmax_loss_workspace(int64_t n, int64_t v, int64_t h, int gradient, int64_t *bytes);
+int msb_linear_softmax_loss(float *loss, float *lse, const void *data, const void *weight,
+                            const int32_t *label, int64_t n, int64_t v, int64_t h, int64_t ld_data,
+                            int64_t ld_weight, int dtype, int32_t ignore_label, float smooth,
+                            void *workspace, int64_t workspace_bytes, msb_stream_t stream);
+/* The gradients of sum_i scale * gloss[i] * loss[i] (gloss NULL: all ones), from the lse that the
+   call above returned: gdata (n x h, `dtype`; assigned) and gweight (v x h, `gweight_dtype` = `dtype` or
+   MSB_FLOAT32; saver 0 assigns, 1 adds).  Either may be NULL: not computed.  Tokens that contribute
+   nothing have zero rows in gdata, and whatever their data rows hold reaches no result.
+   SoftmaxGrad / SmoothSoftmaxGrad with ignore_label (mshadow/tensor_gpu-inl.h:169-214) between the two
+   products of a linear layer's backward pass.  Equal calls give equal bits. */
+int msb_linear_softmax_loss_grad(void *gdata, void *gweight, const void *data, const void *weight,
+                                 const int32_t *label, const float *lse, const float *gloss,
+                                 float scale, int64_t n, int64_t v, int64_t h, int64_t ld_gdata,
+                                 int64_t ld_gweight, int64_t ld_data, int64_t ld_weight, int dtype,
+                                 int gweight_dtype, int saver, int32_t ignore_label, float smooth,
+                                 void *workspace, int64_t workspace_bytes, msb_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

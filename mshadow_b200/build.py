@@ -20,7 +20,8 @@ NVCC_FLAGS = [
 
 TARGETS = [
     (os.path.join(HERE, "libmshadow_b200.so"),
-     [os.path.join(HERE, "csrc", "capi.cu"), os.path.join(HERE, "csrc", "noalloc.cu")], []),
+     [os.path.join(HERE, "csrc", "capi.cu"), os.path.join(HERE, "csrc", "noalloc.cu"),
+      os.path.join(HERE, "csrc", "vocab_capi.cu")], []),
     (os.path.join(ROOT, "tests", "cxx", "libmsb_api_suite.so"),
      [os.path.join(ROOT, "tests", "cxx", "api_suite.cu")], []),
     # the checked build of the engine (tensor leaves refuse and record accesses outside their storage)

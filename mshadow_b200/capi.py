@@ -19,6 +19,7 @@ STATUS_NAMES = {0: "MSB_OK", 1: "MSB_ERR_ARGUMENT", 2: "MSB_ERR_SHAPE", 3: "MSB_
 
 SAVETO, PLUSTO, MINUSTO, MULTO, DIVTO = range(5)
 RED_SUM, RED_MAX, RED_MIN = range(3)
+FLOAT32, FLOAT16, BFLOAT16 = 0, 2, 12
 H2D, D2H, D2D = 1, 2, 3
 
 
@@ -91,11 +92,62 @@ _SIGNATURES = {
     "msb_pack_col2patch_f32": [vp, vp, i64, i64, i64, i64, cint, cint, cint, cint, cint, cint, vp],
     "msb_softmax3d_f32": [vp, vp, i64, i64, i64, i64, i64, vp],
     "msb_softmax_grad3d_f32": [vp, vp, vp, i64, i64, i64, i64, i64, i64, cint, f32, f32, vp],
+    "msb_embed_take": [vp, vp, vp, i64, i64, i64, i64, i64, cint, f32, vp],
+    "msb_embed_take_grad_workspace": [i64, i64, C.POINTER(i64)],
+    "msb_embed_take_grad": [vp, vp, vp, i64, i64, i64, i64, i64, cint, f32, cint, vp, i64, vp],
+    "msb_linear_softmax_loss_workspace": [i64, i64, i64, cint, C.POINTER(i64)],
+    "msb_linear_softmax_loss": [vp, vp, vp, vp, vp, i64, i64, i64, i64, i64, cint, C.c_int32, f32, vp, i64, vp],
+    "msb_linear_softmax_loss_grad": [vp, vp, vp, vp, vp, vp, vp, f32, i64, i64, i64, i64, i64, i64, i64, cint, cint, cint,
+                                     C.c_int32, f32, vp, i64, vp],
 }
 
 
 def _ptr(t):
     return vp(t.data_ptr() if hasattr(t, "data_ptr") else int(t))
+
+
+_DTYPE_FLAGS = {"float32": FLOAT32, "float16": FLOAT16, "bfloat16": BFLOAT16}
+
+
+def _dtype(d):
+    """Type tag of a torch / numpy dtype (or of its name)."""
+    name = str(d).rsplit(".", 1)[-1]
+    if name not in _DTYPE_FLAGS:
+        raise MsbError(1, "element type %s is not one of %s" % (d, sorted(_DTYPE_FLAGS)))
+    return _DTYPE_FLAGS[name]
+
+
+def _same(what, expected, *tensors):
+    for t in tensors:
+        if t is not None and tuple(t.shape) != tuple(expected):
+            raise MsbError(2, "%s: shape %s where %s is expected" % (what, tuple(t.shape), tuple(expected)))
+
+
+def _kind(what, dtype, *tensors):
+    for t in tensors:
+        if t is not None and str(t.dtype) != str(dtype):
+            raise MsbError(1, "%s: %s where %s is expected" % (what, t.dtype, dtype))
+
+
+def _dense(what, *tensors):
+    for t in tensors:
+        if t is not None and t.shape[0] > 1 and t.stride(0) != 1:
+            raise MsbError(3, "%s: vectors must be dense" % what)
+
+
+def _row_ld(what, t):
+    """Leading dimension of a matrix whose rows are dense and do not overlap."""
+    if t.shape[1] > 1 and t.stride(1) != 1:
+        raise MsbError(3, "%s: the last axis must be dense" % what)
+    ld = t.stride(0) if t.shape[0] > 1 else max(t.shape[1], t.stride(0))
+    if ld < t.shape[1]:
+        raise MsbError(3, "%s: rows overlap" % what)
+    return ld
+
+
+def _workspace(t):
+    """(address, bytes) of an optional one-dimensional workspace tensor."""
+    return (None, 0) if t is None else (vp(t.data_ptr()), t.numel() * t.element_size())
 
 
 def _ld(t):
@@ -398,6 +450,85 @@ class Library:
         self.call("msb_softmax_grad3d_f32", _ptr(dst), _ptr(src), _ptr(label), batch, classes, npos, _ld(dst),
                   _ld(src), _ld(label), mode, ignore_label, alpha, stream)
         return dst
+
+
+    # ---- the vocabulary table's two ends ---------------------------------------------------
+    def embed_take(self, dst, table, index, scale=1.0, stream=None):
+        """dst[i] = scale * table[index[i]]; an index outside the table gives a row of zeros."""
+        n, width = dst.shape
+        _same("embed_take", (n,), index)
+        _same("embed_take", (table.shape[0], width), table)
+        _kind("embed_take", dst.dtype, table)
+        _kind("embed_take", "torch.int32", index)
+        _dense("embed_take", index)
+        self.call("msb_embed_take", _ptr(dst), _ptr(table), _ptr(index), n, table.shape[0], width,
+                  _row_ld("embed_take", dst), _row_ld("embed_take", table), _dtype(dst.dtype), scale, stream)
+        return dst
+
+    def embed_take_grad_workspace(self, n, rows, width, dtype=None):
+        """Bytes of workspace of embed_take_grad for n indices (the table's rows and type do not matter)."""
+        out = i64()
+        self.call("msb_embed_take_grad_workspace", n, width, C.byref(out))
+        return out.value
+
+    def embed_take_grad(self, dst, src, index, scale=1.0, saver=SAVETO, workspace=None, stream=None):
+        """dst[r] = (saver PLUSTO: +=) scale * sum of the rows of src whose index is r."""
+        n, width = src.shape
+        _same("embed_take_grad", (n,), index)
+        _same("embed_take_grad", (dst.shape[0], width), dst)
+        _kind("embed_take_grad", dst.dtype, src)
+        _kind("embed_take_grad", "torch.int32", index)
+        _dense("embed_take_grad", index)
+        ws, size = _workspace(workspace)
+        self.call("msb_embed_take_grad", _ptr(dst), _ptr(src), _ptr(index), n, dst.shape[0], width,
+                  _row_ld("embed_take_grad", dst), _row_ld("embed_take_grad", src), _dtype(dst.dtype), scale, saver, ws, size,
+                  stream)
+        return dst
+
+    def linear_softmax_loss_workspace(self, n, v, h, dtype=None, gradient=False):
+        """Bytes of workspace of linear_softmax_loss (gradient=True: of linear_softmax_loss_grad, enough for both)."""
+        out, loss = i64(), i64()
+        self.call("msb_linear_softmax_loss_workspace", n, v, h, 0, C.byref(loss))
+        if not gradient:
+            return loss.value
+        self.call("msb_linear_softmax_loss_workspace", n, v, h, 1, C.byref(out))
+        return max(loss.value, out.value)
+
+    def linear_softmax_loss(self, loss, lse, data, weight, label, ignore_label=-1, smooth=0.0, workspace=None, stream=None):
+        """Cross entropy of softmax(data . weight^T) and the log of its normaliser, per token."""
+        (n, h), v = data.shape, weight.shape[0]
+        what = "linear_softmax_loss"
+        _same(what, (n,), loss, lse, label)
+        _same(what, (v, h), weight)
+        _kind(what, data.dtype, weight)
+        _kind(what, "torch.int32", label)
+        _kind(what, "torch.float32", loss, lse)
+        _dense(what, loss, lse, label)
+        ws, size = _workspace(workspace)
+        self.call("msb_linear_softmax_loss", _ptr(loss), _ptr(lse), _ptr(data), _ptr(weight), _ptr(label), n, v, h,
+                  _row_ld(what, data), _row_ld(what, weight), _dtype(data.dtype), ignore_label, smooth, ws, size, stream)
+        return loss, lse
+
+    def linear_softmax_loss_grad(self, gdata, gweight, data, weight, label, lse, gloss=None, scale=1.0, ignore_label=-1,
+                                 smooth=0.0, saver=SAVETO, workspace=None, stream=None):
+        """Gradients of sum(scale * gloss * loss); gdata or gweight may be None.  saver PLUSTO adds to gweight."""
+        (n, h), v = data.shape, weight.shape[0]
+        what = "linear_softmax_loss_grad"
+        _same(what, (n,), lse, label, gloss)
+        _same(what, (v, h), weight, gweight)
+        _same(what, (n, h), gdata)
+        _kind(what, data.dtype, weight, gdata)
+        _kind(what, "torch.int32", label)
+        _kind(what, "torch.float32", lse, gloss)
+        _dense(what, lse, label, gloss)
+        ws, size = _workspace(workspace)
+        self.call("msb_linear_softmax_loss_grad", None if gdata is None else _ptr(gdata),
+                  None if gweight is None else _ptr(gweight), _ptr(data), _ptr(weight), _ptr(label), _ptr(lse),
+                  None if gloss is None else _ptr(gloss), scale, n, v, h, h if gdata is None else _row_ld(what, gdata),
+                  h if gweight is None else _row_ld(what, gweight), _row_ld(what, data), _row_ld(what, weight),
+                  _dtype(data.dtype), _dtype(data.dtype if gweight is None else gweight.dtype), saver, ignore_label, smooth,
+                  ws, size, stream)
+        return gdata, gweight
 
 
 _lib = None

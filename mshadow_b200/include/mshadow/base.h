@@ -119,6 +119,7 @@ enum TypeFlag {
   kInt32 = 4,
   kInt8 = 5,
   kInt64 = 6,
+  kBfloat16 = 12,
 };
 
 template <typename DType>

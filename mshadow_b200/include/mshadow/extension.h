@@ -14,4 +14,6 @@
 #include "./extension/axis.h"
 #include "./extension/complex.h"
 #include "./extension/lrn.h"
+#include "./extension/embed_take.h"
+#include "./extension/linear_softmax_loss.h"
 #endif  // MSHADOW_EXTENSION_H_

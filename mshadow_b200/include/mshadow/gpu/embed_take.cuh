@@ -1,0 +1,536 @@
+/*
+ * Embedding look-up with scaling and its gradient, for binary32, binary16 and bfloat16 tables.
+ *
+ *   EmbedTake       out[i] = scale * table[index[i]]                (0 where index[i] is outside the table)
+ *   EmbedTakeGrad   grad[r] (=|+=) scale * sum of g[i], index[i] == r  (an index outside names no row)
+ *
+ * Products with scale and sums are binary32, in ascending order of i up to the grouping below, and
+ * rounded once to the element type.  No atomics on values: results do not depend on timing.
+ *
+ * The look-up moves 16-byte groups, four in flight per thread, and is bound by memory.
+ *
+ * The gradient sorts (index, position) stably (radix_sort.cuh) and sums segments of the sorted list:
+ *   - the list is cut into chunks of kChunk entries; a chunk's CTA owns the runs that begin in it
+ *     and follows the last one past the chunk's end;
+ *   - only a run of more than kChunk entries (a frequent token) is split: each chunk leaves its
+ *     part as a binary32 row in scratch memory, and a second kernel adds the parts, in order;
+ *   - when the gradient is assigned rather than added to, further CTAs of the same launch write
+ *     zeros to the rows that no index names, so that every row of the table is written exactly
+ *     once.
+ * A short list (up to kFewTokens) is not sorted: the CTA of an entry that is the first of its index
+ * finds the later ones by scanning the list.
+ */
+#ifndef MSHADOW_GPU_EMBED_TAKE_CUH_
+#define MSHADOW_GPU_EMBED_TAKE_CUH_
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+
+#include "../bfloat.h"
+#include "./radix_sort.cuh"
+
+namespace mshadow {
+namespace cuda {
+namespace embtake {
+
+const int kChunk = 64;        // sorted entries per CTA; also the longest run that is not split
+const int kFewTokens = 512;   // lists up to this are not sorted
+const int kDepth = 8;         // source rows in flight per thread
+const int kZeroRows = 128;    // table rows per CTA that writes zeros
+
+// ---- element types: groups of 16 bytes (or single elements) as binary32 ----------------------------
+
+template <typename T, bool kVec>
+struct Group {
+  static const int kLanes = kVec ? 16 / static_cast<int>(sizeof(T)) : 1;
+};
+
+__device__ __forceinline__ float ToFloat(float v) { return v; }
+__device__ __forceinline__ float ToFloat(half::half_t v) { return __half2float(__ushort_as_half(v.half_)); }
+__device__ __forceinline__ float ToFloat(bfloat::bf16_t v) { return __uint_as_float(static_cast<uint32_t>(v.bits_) << 16); }
+__device__ __forceinline__ void FromFloat(float v, float *out) { *out = v; }
+__device__ __forceinline__ void FromFloat(float v, half::half_t *out) { out->half_ = __half_as_ushort(__float2half_rn(v)); }
+__device__ __forceinline__ void FromFloat(float v, bfloat::bf16_t *out) {
+  out->bits_ = __bfloat16_as_ushort(__float2bfloat16_rn(v));
+}
+
+/*! \brief raw bits of one group */
+template <typename T, bool kVec>
+struct Bits {
+  uint4 raw;
+};
+template <typename T>
+struct Bits<T, false> {
+  T raw;
+};
+
+template <typename T>
+__device__ __forceinline__ void LoadStream(const T *p, Bits<T, true> *b) {
+  b->raw = __ldcs(reinterpret_cast<const uint4 *>(p));
+}
+template <typename T>
+__device__ __forceinline__ void LoadStream(const T *p, Bits<T, false> *b) {
+  b->raw = *p;
+}
+template <typename T>
+__device__ __forceinline__ void Load(const T *p, Bits<T, true> *b) {
+  b->raw = *reinterpret_cast<const uint4 *>(p);
+}
+template <typename T>
+__device__ __forceinline__ void Load(const T *p, Bits<T, false> *b) {
+  b->raw = *p;
+}
+template <typename T>
+__device__ __forceinline__ void Store(T *p, const Bits<T, true> &b) {
+  *reinterpret_cast<uint4 *>(p) = b.raw;
+}
+template <typename T>
+__device__ __forceinline__ void Store(T *p, const Bits<T, false> &b) {
+  *p = b.raw;
+}
+template <typename T, bool kVec>
+__device__ __forceinline__ void Unpack(const Bits<T, kVec> &b, float (&v)[Group<T, kVec>::kLanes]) {
+  T e[Group<T, kVec>::kLanes];
+  memcpy(e, &b.raw, sizeof(e));
+#pragma unroll
+  for (int l = 0; l < Group<T, kVec>::kLanes; ++l) v[l] = ToFloat(e[l]);
+}
+template <typename T, bool kVec>
+__device__ __forceinline__ void Pack(const float (&v)[Group<T, kVec>::kLanes], Bits<T, kVec> *b) {
+  T e[Group<T, kVec>::kLanes];
+#pragma unroll
+  for (int l = 0; l < Group<T, kVec>::kLanes; ++l) FromFloat(v[l], &e[l]);
+  memcpy(&b->raw, e, sizeof(e));
+}
+
+// ---- look-up -------------------------------------------------------------------------------------------
+
+/*! \brief grid-stride over (token, group) pairs, four per thread and sweep */
+template <typename T, bool kVec>
+__global__ void __launch_bounds__(256)
+EmbedTakeKernel(T *out, int64_t ld_out, const int32_t *index, const T *table, int64_t ld_table, uint64_t total,
+                uint32_t n_groups, int32_t rows, float scale) {
+  gpu_rt::GridDependencySync();
+  typedef Group<T, kVec> G;
+  const uint64_t step = static_cast<uint64_t>(gridDim.x) * 256;
+  for (uint64_t e0 = static_cast<uint64_t>(blockIdx.x) * 256 + threadIdx.x; e0 < total; e0 += 4 * step) {
+    Bits<T, kVec> b[4];
+    uint32_t token[4], col[4];
+    int32_t r[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const uint64_t e = e0 + u * step;
+      r[u] = -1;
+      if (e < total) {
+        token[u] = static_cast<uint32_t>(e / n_groups);
+        col[u] = static_cast<uint32_t>(e - static_cast<uint64_t>(token[u]) * n_groups) * G::kLanes;
+        r[u] = index[token[u]];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      memset(&b[u], 0, sizeof(b[u]));
+      if (r[u] >= 0 && r[u] < rows) Load(table + r[u] * ld_table + col[u], &b[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (e0 + u * step >= total) continue;
+      float v[G::kLanes];
+      Unpack<T, kVec>(b[u], v);
+      const bool named = r[u] >= 0 && r[u] < rows;
+#pragma unroll
+      for (int l = 0; l < G::kLanes; ++l) v[l] = named ? v[l] * scale : 0.0f;
+      Pack<T, kVec>(v, &b[u]);
+      Store(out + token[u] * ld_out + col[u], b[u]);
+    }
+  }
+}
+
+// ---- gradient -------------------------------------------------------------------------------------------
+
+template <typename T>
+struct GradArgs {
+  T *grad;
+  int64_t ld_grad;
+  const T *g;
+  int64_t ld_g;
+  const int32_t *keys, *rows;  // sorted indices, their positions (-1: names no row)
+  const int32_t *index;        // short lists: the indices as given
+  uint32_t n, width, table_rows;
+  float scale;
+  int add;
+  uint32_t chunks, slabs;      // CTAs that sum; the ones after them write zeros
+  float *parts;                // [2 * chunks][width_pad]: parts of split runs
+  int64_t ld_parts;
+  int32_t *spans;              // [0] = number of split runs, then the chunk each begins in
+};
+
+template <typename T, bool kVec>
+__device__ __forceinline__ void WriteRow(const GradArgs<T> &a, int32_t row, uint32_t col,
+                                         const float (&acc)[Group<T, kVec>::kLanes]) {
+  T *p = a.grad + row * a.ld_grad + col;
+  Bits<T, kVec> b;
+  float v[Group<T, kVec>::kLanes];
+  if (a.add) {
+    Load(p, &b);
+    Unpack<T, kVec>(b, v);
+#pragma unroll
+    for (int l = 0; l < Group<T, kVec>::kLanes; ++l) v[l] = __fadd_rn(v[l], __fmul_rn(a.scale, acc[l]));
+  } else {
+#pragma unroll
+    for (int l = 0; l < Group<T, kVec>::kLanes; ++l) v[l] = __fadd_rn(__fmul_rn(a.scale, acc[l]), 0.0f);
+  }
+  Pack<T, kVec>(v, &b);
+  Store(p, b);
+}
+
+/*! \brief zeros for the rows [first, last) whose flag is not set */
+template <typename T, bool kVec>
+__device__ __forceinline__ void WriteZeros(const GradArgs<T> &a, uint32_t first, uint32_t last, const uint8_t *named) {
+  Bits<T, kVec> zero;
+  memset(&zero, 0, sizeof(zero));
+  const uint32_t warp = threadIdx.x >> 5, warps = blockDim.x >> 5, lane = threadIdx.x & 31;
+  for (uint32_t r = first + warp; r < last; r += warps) {
+    if (named[r - first]) continue;
+    for (uint32_t c = lane * Group<T, kVec>::kLanes; c < a.width; c += 32 * Group<T, kVec>::kLanes) {
+      Store(a.grad + r * a.ld_grad + c, zero);
+    }
+  }
+}
+
+/*! \brief first position of keys[0, n) that is not below k */
+__device__ __forceinline__ uint32_t LowerBound(const int32_t *keys, uint32_t n, int32_t k) {
+  uint32_t lo = 0, hi = n;
+  while (lo < hi) {
+    const uint32_t mid = (lo + hi) / 2;
+    if (keys[mid] < k) lo = mid + 1;
+    else hi = mid;
+  }
+  return lo;
+}
+
+/*! \brief adds the source rows of window entries [from, to) to acc, kDepth of them in flight */
+template <typename T, bool kVec>
+__device__ __forceinline__ void AddRows(const GradArgs<T> &a, const int32_t *rows, uint32_t from, uint32_t to, uint32_t col,
+                                        float (&acc)[Group<T, kVec>::kLanes]) {
+  for (uint32_t i = from; i < to; i += kDepth) {
+    Bits<T, kVec> b[kDepth];
+    int32_t r[kDepth];
+#pragma unroll
+    for (int u = 0; u < kDepth; ++u) {
+      r[u] = i + u < to ? rows[i + u] : -1;
+      if (r[u] >= 0) LoadStream(a.g + r[u] * a.ld_g + col, &b[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < kDepth; ++u) {
+      if (r[u] >= 0) {
+        float v[Group<T, kVec>::kLanes];
+        Unpack<T, kVec>(b[u], v);
+#pragma unroll
+        for (int l = 0; l < Group<T, kVec>::kLanes; ++l) acc[l] = __fadd_rn(acc[l], v[l]);
+      }
+    }
+  }
+}
+
+/*!
+ * \brief sums of the runs of a sorted list, and zeros for the rows that are not in it.
+ *  grid: chunks * slabs CTAs that sum, then (when assigning) CTAs that write zeros.
+ */
+template <typename T, bool kVec>
+__global__ void __launch_bounds__(256) EmbedSumKernel(const GradArgs<T> a) {
+  gpu_rt::GridDependencySync();
+  typedef Group<T, kVec> G;
+  __shared__ int32_t s_keys[3 * kChunk], s_rows[3 * kChunk];
+  if (blockIdx.x >= a.chunks * a.slabs) {
+    __shared__ uint8_t named[kZeroRows];
+    const uint32_t first = (blockIdx.x - a.chunks * a.slabs) * kZeroRows;
+    const uint32_t last = min(a.table_rows, first + kZeroRows);
+    for (uint32_t r = first + threadIdx.x; r < last; r += blockDim.x) {
+      const uint32_t at = LowerBound(a.keys, a.n, static_cast<int32_t>(r));
+      named[r - first] = at < a.n && a.keys[at] == static_cast<int32_t>(r);
+    }
+    __syncthreads();
+    WriteZeros<T, kVec>(a, first, last, named);
+    return;
+  }
+  const uint32_t chunk = blockIdx.x / a.slabs, slab = blockIdx.x - chunk * a.slabs;
+  const int64_t begin = static_cast<int64_t>(chunk) * kChunk;
+  // entries [begin - kChunk, begin + 2 kChunk); keys outside the list differ from all others
+  for (uint32_t i = threadIdx.x; i < 3 * kChunk; i += blockDim.x) {
+    const int64_t e = begin - kChunk + i;
+    const bool in = e >= 0 && e < a.n;
+    s_keys[i] = in ? a.keys[e] : -1;
+    s_rows[i] = in ? a.rows[e] : -1;
+  }
+  __syncthreads();
+  const uint32_t col = (slab * blockDim.x + threadIdx.x) * G::kLanes;
+  const bool active = col < a.width;
+  const bool lead = slab == 0 && threadIdx.x == 0;
+  const uint32_t lo = kChunk;
+  const uint32_t hi = kChunk + static_cast<uint32_t>(min(static_cast<int64_t>(kChunk), a.n - begin));
+  uint32_t at = lo;
+  const int32_t before = s_keys[lo - 1];
+  if (before == s_keys[lo]) {
+    // the first run began in an earlier chunk
+    uint32_t start = lo, stop = lo;
+    while (start > 0 && s_keys[start - 1] == before) --start;
+    while (stop < hi && s_keys[stop] == before) ++stop;
+    const bool split = start == 0 || s_keys[start + kChunk] == before;
+    if (split && active) {
+      float acc[G::kLanes];
+#pragma unroll
+      for (int l = 0; l < G::kLanes; ++l) acc[l] = -0.0f;
+      AddRows<T, kVec>(a, s_rows, lo, stop, col, acc);
+#pragma unroll
+      for (int l = 0; l < G::kLanes; ++l) a.parts[2 * chunk * a.ld_parts + col + l] = acc[l];
+    }
+    at = stop;
+  }
+  while (at < hi) {
+    const int32_t key = s_keys[at];
+    uint32_t stop = at + 1;
+    while (stop < 3 * kChunk && s_keys[stop] == key) ++stop;
+    const bool split = stop - at > kChunk;
+    if (split) stop = hi;  // a longer run leaves this chunk's part only
+    if (active) {
+      float acc[G::kLanes];
+#pragma unroll
+      for (int l = 0; l < G::kLanes; ++l) acc[l] = -0.0f;  // the sum of nothing: adding it changes no value
+      AddRows<T, kVec>(a, s_rows, at, stop, col, acc);
+      if (split) {
+#pragma unroll
+        for (int l = 0; l < G::kLanes; ++l) a.parts[(2 * chunk + 1) * a.ld_parts + col + l] = acc[l];
+      } else {
+        WriteRow<T, kVec>(a, key, col, acc);
+      }
+    }
+    if (split && lead) a.spans[1 + atomicAdd(a.spans, 1)] = static_cast<int32_t>(chunk);
+    at = stop;
+  }
+}
+
+/*!
+ * \brief adds the parts of the split runs.  A CTA takes one run and 128 columns at a time; its eight warps take
+ *  every eighth part each and are joined in warp order.
+ */
+template <typename T, bool kVec>
+__global__ void __launch_bounds__(256) EmbedSpanKernel(const GradArgs<T> a) {
+  gpu_rt::GridDependencySync();
+  __shared__ float s_sum[8][128];
+  const uint32_t count = static_cast<uint32_t>(a.spans[0]);
+  const uint32_t slabs = (a.width + 127) / 128;
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (uint32_t w = blockIdx.x; w < count * slabs; w += gridDim.x) {
+    const uint32_t chunk = static_cast<uint32_t>(a.spans[1 + w / slabs]);
+    const uint32_t col = (w % slabs) * 128 + lane * 4;
+    const uint32_t end = min(a.n, (chunk + 1) * kChunk);
+    const int32_t key = a.keys[end - 1];
+    const uint32_t stop = key == 0x7fffffff ? a.n : LowerBound(a.keys, a.n, key + 1);
+    const uint32_t last = (stop - 1) / kChunk;
+    float acc[4] = {-0.0f, -0.0f, -0.0f, -0.0f};
+    for (uint32_t c = chunk + warp; c <= last; c += 8 * 4) {
+      float4 p[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const uint32_t q = c + 8 * u;
+        p[u] = make_float4(-0.0f, -0.0f, -0.0f, -0.0f);
+        if (q <= last) {
+          const int64_t row = q == chunk ? 2 * static_cast<int64_t>(q) + 1 : 2 * static_cast<int64_t>(q);
+          p[u] = *reinterpret_cast<const float4 *>(a.parts + row * a.ld_parts + col);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        acc[0] = __fadd_rn(acc[0], p[u].x);
+        acc[1] = __fadd_rn(acc[1], p[u].y);
+        acc[2] = __fadd_rn(acc[2], p[u].z);
+        acc[3] = __fadd_rn(acc[3], p[u].w);
+      }
+    }
+    *reinterpret_cast<float4 *>(&s_sum[warp][lane * 4]) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+    __syncthreads();
+    const uint32_t c = (w % slabs) * 128 + threadIdx.x;
+    if (threadIdx.x < 128 && c < a.width) {
+      float sum[1] = {s_sum[0][threadIdx.x]};
+      for (int q = 1; q < 8; ++q) sum[0] = __fadd_rn(sum[0], s_sum[q][threadIdx.x]);
+      WriteRow<T, false>(a, key, c, sum);
+    }
+    __syncthreads();
+  }
+}
+
+/*!
+ * \brief short lists, in one launch and without a sort.  grid: n * slabs CTAs, then (when assigning) CTAs that
+ *  write zeros.  The CTA of an entry whose index occurred before does nothing.
+ */
+template <typename T, bool kVec>
+__global__ void __launch_bounds__(256) EmbedFewKernel(const GradArgs<T> a) {
+  gpu_rt::GridDependencySync();
+  typedef Group<T, kVec> G;
+  __shared__ int32_t s_rows[kFewTokens];
+  __shared__ uint32_t s_votes[kFewTokens / 32];
+  __shared__ uint8_t named[kZeroRows];
+  __shared__ int s_earlier;
+  if (blockIdx.x >= a.n * a.slabs) {
+    const uint32_t first = (blockIdx.x - a.n * a.slabs) * kZeroRows;
+    const uint32_t last = min(a.table_rows, first + kZeroRows);
+    for (uint32_t r = threadIdx.x; r < kZeroRows; r += blockDim.x) named[r] = 0;
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < a.n; i += blockDim.x) {
+      const int32_t k = a.index[i];
+      if (k >= static_cast<int64_t>(first) && k < static_cast<int64_t>(last)) named[k - first] = 1;
+    }
+    __syncthreads();
+    WriteZeros<T, kVec>(a, first, last, named);
+    return;
+  }
+  const uint32_t entry = blockIdx.x / a.slabs, slab = blockIdx.x - entry * a.slabs;
+  const int32_t key = a.index[entry];
+  if (key < 0 || key >= static_cast<int64_t>(a.table_rows)) return;
+  if (threadIdx.x == 0) s_earlier = 0;
+  __syncthreads();
+  for (uint32_t i0 = 0; i0 < a.n; i0 += blockDim.x) {
+    const uint32_t i = i0 + threadIdx.x;
+    const bool same = i < a.n && a.index[i] == key;
+    const uint32_t votes = __ballot_sync(0xffffffffu, same);
+    if ((threadIdx.x & 31) == 0 && i < kFewTokens) s_votes[i / 32] = votes;
+    if (same && i < entry) s_earlier = 1;
+  }
+  __syncthreads();
+  if (s_earlier) return;
+  const uint32_t words = (a.n + 31) / 32;
+  uint32_t count = 0;
+  for (uint32_t w = 0; w < words; ++w) {
+    uint32_t bits = s_votes[w];
+    if (threadIdx.x == 0) {
+      uint32_t at = count, left = bits;
+      while (left != 0) {
+        s_rows[at++] = static_cast<int32_t>(w * 32 + __ffs(left) - 1);
+        left &= left - 1;
+      }
+    }
+    count += __popc(bits);
+  }
+  __syncthreads();
+  const uint32_t col = (slab * blockDim.x + threadIdx.x) * G::kLanes;
+  if (col >= a.width) return;
+  float acc[G::kLanes];
+#pragma unroll
+  for (int l = 0; l < G::kLanes; ++l) acc[l] = -0.0f;
+  AddRows<T, kVec>(a, s_rows, 0, count, col, acc);
+  WriteRow<T, kVec>(a, key, col, acc);
+}
+
+// ---- host side ------------------------------------------------------------------------------------------
+
+template <typename T>
+inline bool Aligned(const T *p, int64_t ld, int64_t width) {
+  const int64_t lanes = 16 / sizeof(T);
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % lanes == 0 && width % lanes == 0;
+}
+
+template <typename T, bool kVec>
+inline void TakeGo(T *out, int64_t ld_out, const int32_t *index, const T *table, int64_t ld_table, int64_t n, int64_t rows,
+                   int64_t width, float scale, cudaStream_t stream) {
+  const int64_t groups = width / Group<T, kVec>::kLanes;
+  const int64_t total = n * groups;
+  const int64_t cap = static_cast<int64_t>(gpu_rt::CurrentDevice().sm_count) * 8;
+  const int64_t grid = std::min((total + 255) / 256, cap);
+  gpu_rt::LaunchAfterDrain(EmbedTakeKernel<T, kVec>, dim3(static_cast<unsigned>(grid)), dim3(256), 0, stream, out, ld_out,
+                           index, table, ld_table, static_cast<uint64_t>(total),
+                           static_cast<uint32_t>(groups),
+                           static_cast<int32_t>(rows), scale);
+  MSHADOW_CUDA_POST_KERNEL_CHECK(EmbedTakeKernel);
+}
+
+/*! \brief out[i] = scale * table[index[i]]; rows and columns of the tensors as given by n, rows, width */
+template <typename T>
+inline void TakeLaunch(T *out, int64_t ld_out, const int32_t *index, const T *table, int64_t ld_table, int64_t n,
+                       int64_t rows, int64_t width, float scale, cudaStream_t stream) {
+  if (n == 0 || width == 0) return;
+  if (Aligned(out, ld_out, width) && Aligned(table, ld_table, width)) {
+    TakeGo<T, true>(out, ld_out, index, table, ld_table, n, rows, width, scale, stream);
+  } else {
+    TakeGo<T, false>(out, ld_out, index, table, ld_table, n, rows, width, scale, stream);
+  }
+}
+
+struct GradPlan {
+  bool few;
+  uint32_t chunks;
+  int64_t ld_parts;
+  int64_t keys, rows, sort, parts, spans, bytes;  // offsets
+};
+
+inline GradPlan MakeGradPlan(int64_t n, int64_t width) {
+  GradPlan p = {};
+  p.few = n <= kFewTokens;
+  if (p.few) return p;
+  p.chunks = static_cast<uint32_t>((n + kChunk - 1) / kChunk);
+  p.ld_parts = (width + 127) / 128 * 128;
+  int64_t at = 0;
+  auto take = [&at](int64_t bytes) {
+    const int64_t was = at;
+    at += (bytes + 255) / 256 * 256;
+    return was;
+  };
+  p.keys = take(n * 4);
+  p.rows = take(n * 4);
+  p.sort = take(static_cast<int64_t>(sortdetail::ScratchBytes(n)));
+  p.parts = take(2ll * p.chunks * p.ld_parts * 4);
+  p.spans = take((1ll + p.chunks) * 4);
+  p.bytes = at;
+  return p;
+}
+
+template <typename T, bool kVec>
+inline void GradGo(GradArgs<T> a, const GradPlan &p, char *ws, cudaStream_t stream) {
+  const uint32_t items = a.width / Group<T, kVec>::kLanes;
+  const uint32_t threads = std::min(256u, (items + 31) / 32 * 32);
+  a.slabs = (items + threads - 1) / threads;
+  const uint32_t zero = a.add ? 0 : (a.table_rows + kZeroRows - 1) / kZeroRows;
+  if (p.few) {
+    const uint32_t grid = a.n * a.slabs + zero;
+    if (grid == 0) return;
+    gpu_rt::LaunchAfterDrain(EmbedFewKernel<T, kVec>, dim3(grid), dim3(threads), 0, stream, a);
+    MSHADOW_CUDA_POST_KERNEL_CHECK(EmbedFewKernel);
+    return;
+  }
+  int32_t *keys = reinterpret_cast<int32_t *>(ws + p.keys), *rows = reinterpret_cast<int32_t *>(ws + p.rows);
+  int bits = 1;
+  while (bits < 31 && (int64_t(1) << bits) < a.table_rows) ++bits;
+  a.spans = reinterpret_cast<int32_t *>(ws + p.spans);
+  MSHADOW_CUDA_CALL(cudaMemsetAsync(a.spans, 0, 4, stream));
+  const sortdetail::Source named = {static_cast<int>(a.table_rows), 1};
+  sortdetail::SortPairs<int32_t, int32_t>(keys, rows, a.index, a.n, bits, true, named, ws + p.sort, stream);
+  a.keys = keys, a.rows = rows;
+  a.chunks = p.chunks;
+  a.parts = reinterpret_cast<float *>(ws + p.parts), a.ld_parts = p.ld_parts;
+  gpu_rt::LaunchAfterDrain(EmbedSumKernel<T, kVec>, dim3(a.chunks * a.slabs + zero), dim3(threads), 0, stream, a);
+  MSHADOW_CUDA_POST_KERNEL_CHECK(EmbedSumKernel);
+  const int64_t most = static_cast<int64_t>(p.chunks) * ((a.width + 127) / 128);
+  const int64_t cap = static_cast<int64_t>(gpu_rt::CurrentDevice().sm_count) * 8;
+  gpu_rt::LaunchAfterDrain(EmbedSpanKernel<T, kVec>, dim3(static_cast<unsigned>(std::min(most, cap))), dim3(256), 0, stream, a);
+  MSHADOW_CUDA_POST_KERNEL_CHECK(EmbedSpanKernel);
+}
+
+/*! \brief grad[r] (=|+=) scale * sum of the rows of g whose index is r */
+template <typename T>
+inline void GradLaunch(T *grad, int64_t ld_grad, const T *g, int64_t ld_g, const int32_t *index, int64_t n, int64_t rows,
+                       int64_t width, float scale, bool add, const GradPlan &p, char *ws, cudaStream_t stream) {
+  if (rows == 0 || width == 0 || (n == 0 && add)) return;
+  GradArgs<T> a = {};
+  a.grad = grad, a.ld_grad = ld_grad, a.g = g, a.ld_g = ld_g, a.index = index;
+  a.n = static_cast<uint32_t>(n), a.width = static_cast<uint32_t>(width), a.table_rows = static_cast<uint32_t>(rows);
+  a.scale = scale, a.add = add;
+  if (Aligned(grad, ld_grad, width) && (n == 0 || Aligned(g, ld_g, width))) GradGo<T, true>(a, p, ws, stream);
+  else GradGo<T, false>(a, p, ws, stream);
+}
+
+}  // namespace embtake
+}  // namespace cuda
+}  // namespace mshadow
+#endif  // MSHADOW_GPU_EMBED_TAKE_CUH_

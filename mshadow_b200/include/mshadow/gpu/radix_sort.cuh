@@ -41,7 +41,8 @@ const int kMaxDigitBits = 9;
 
 /*! \brief how the first pass obtains its input */
 struct Source {
-  int clip_rows;  // > 0: keys are raw indices to be clipped to [0, clip_rows), values are 0, 1, 2, ...
+  int clip_rows;    // > 0: keys are raw indices to be clipped to [0, clip_rows), values are 0, 1, 2, ...
+  int drop_clipped;  // != 0: the value of an index that had to be clipped is -1 (an entry that names no row)
 };
 
 /*! \brief 32 bits whose unsigned order is the key order (ascending), or its reverse */
@@ -180,7 +181,9 @@ RadixScatterKernel(const K *keys_in, const V *vals_in, K *keys_out, V *vals_out,
     if (valid) {
       key[r] = LoadKey(keys_in, i, src);
       if (src.clip_rows > 0) {
-        const uint32_t iota = i;
+        int32_t named = 0;
+        if (src.drop_clipped) memcpy(&named, &keys_in[i], 4);
+        const uint32_t iota = named < 0 || named >= src.clip_rows ? 0xffffffffu : i;
         memcpy(&val[r], &iota, 4);
       } else {
         val[r] = vals_in[i];

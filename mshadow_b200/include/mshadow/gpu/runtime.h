@@ -241,6 +241,31 @@ inline bool TakeBoundsViolation(long long *offset, int *width, long long *limit)
 }
 #endif
 
+/*! \brief true while work issued to the stream is recorded into a graph instead of run */
+inline bool IsCapturing(cudaStream_t stream) {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  MSHADOW_CUDA_CALL(cudaStreamIsCapturing(stream, &status));
+  return status != cudaStreamCaptureStatusNone;
+}
+
+/*!
+ * \brief scratch memory of an operator that takes an optional workspace: the caller's (checked for size;
+ *  256-byte alignment is made inside it, WorkspaceBytes() counts for that), or the stream's own.
+ *  The stream's scratch may be released or grown by later calls and is shared by everything on the
+ *  stream, so a call that is recorded into a graph must bring its own.
+ */
+inline size_t WorkspaceBytes(size_t need) { return need == 0 ? 0 : need + 256; }
+inline char *Workspace(void *given, size_t given_bytes, size_t need, cudaStream_t stream, const char *name) {
+  if (need == 0) return nullptr;
+  if (given == nullptr) {
+    CHECK(!IsCapturing(stream)) << name << ": a call captured into a graph needs a workspace of the caller's";
+    return static_cast<char *>(Scratch::Get(stream, need));
+  }
+  CHECK(given_bytes >= WorkspaceBytes(need)) << name << ": the workspace holds " << given_bytes << " bytes, "
+                                             << WorkspaceBytes(need) << " are needed";
+  return reinterpret_cast<char *>((reinterpret_cast<uintptr_t>(given) + 255) / 256 * 256);
+}
+
 /*!
  * \brief one int per device in which a kernel records that a bounded wait gave up
  *  (see gpu/tma.cuh); allocated on first use, lives as long as the process
