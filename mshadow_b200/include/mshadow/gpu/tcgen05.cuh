@@ -68,18 +68,22 @@ inline EncodeTiledFn EncodeTiled() {
 }
 
 /*!
- * \brief map of a row-major matrix of 16-bit elements whose copies move boxes of 64 columns by
- *  `box_rows` rows; elements outside the matrix read as zero.  base and row pitch 16-byte aligned.
+ * \brief map of a row-major matrix (`type`: kFloat32, kFloat16 or kBfloat16) whose copies move boxes of 128 bytes by
+ *  `box_rows` rows; elements outside the matrix read as zero and are not written.  base and row pitch
+ *  16-byte aligned.
  */
-inline CUtensorMap MatrixMap(const void *base, bool bf16, int64_t rows, int64_t cols, int64_t ld, int box_rows) {
+inline CUtensorMap MatrixMap(const void *base, int type, int64_t rows, int64_t cols, int64_t ld, int box_rows) {
   CUtensorMap map;
+  const int elem = type == kFloat32 ? 4 : 2;
   const cuuint64_t extent[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
-  const cuuint64_t pitch[1] = {static_cast<cuuint64_t>(ld) * 2};
-  const cuuint32_t box[2] = {64, static_cast<cuuint32_t>(box_rows)};
+  const cuuint64_t pitch[1] = {static_cast<cuuint64_t>(ld) * elem};
+  const cuuint32_t box[2] = {static_cast<cuuint32_t>(128 / elem), static_cast<cuuint32_t>(box_rows)};
   const cuuint32_t step[2] = {1, 1};
   const CUresult rc =
-      EncodeTiled()(&map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
-                    const_cast<void *>(base), extent, pitch, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+      EncodeTiled()(&map, type == kFloat32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                          : type == kBfloat16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                              : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                    2, const_cast<void *>(base), extent, pitch, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
                     CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   CHECK_EQ(static_cast<int>(rc), 0) << "CUDA: cuTensorMapEncodeTiled refused a matrix";
   return map;
@@ -130,6 +134,39 @@ __device__ __forceinline__ void LoadBox(uint32_t dst, const CUtensorMap *map, in
   }
 }
 
+/*! \brief box of shared memory to column x, row y of a matrix (parts outside it are left out); kAdd: added to what is there */
+template <bool kAdd>
+__device__ __forceinline__ void StoreBox(const CUtensorMap *map, int x, int y, uint32_t src) {
+  if (kAdd) {
+    asm volatile("cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map),
+                 "r"(x), "r"(y), "r"(src)
+                 : "memory");
+  } else {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(x),
+                 "r"(y), "r"(src)
+                 : "memory");
+  }
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+/*! \brief this thread's stores have read their shared memory */
+__device__ __forceinline__ void WaitStoresRead() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+/*! \brief this thread's stores have been written */
+__device__ __forceinline__ void WaitStores() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
+/*! \brief barrier of `threads` threads (whole warps), number `id` of 1 .. 15 */
+__device__ __forceinline__ void NamedBarrier(int id, int threads) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+/*! \brief the same, true if `ok` holds for all of them */
+__device__ __forceinline__ bool NamedBarrierAnd(int id, int threads, bool ok) {
+  uint32_t r;
+  asm volatile(
+      "{\n.reg .pred p, q;\nsetp.ne.u32 p, %3, 0;\nbar.red.and.pred q, %1, %2, p;\nselp.u32 %0, 1, 0, q;\n}\n"
+      : "=r"(r)
+      : "r"(id), "r"(threads), "r"(ok ? 1u : 0u)
+      : "memory");
+  return r != 0;
+}
 // ---- tensor memory and products ---------------------------------------------------------------
 
 /*! \brief all 512 columns; executed by one whole warp (of both CTAs of a pair) */
@@ -197,6 +234,15 @@ __device__ __forceinline__ void LoadColumns(uint32_t addr, uint32_t (&r)[32]) {
         "=r"(r[30]), "=r"(r[31])
       : "r"(addr));
 }
+/*! \brief the same, 16 columns */
+__device__ __forceinline__ void LoadColumns(uint32_t addr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(addr));
+}
 /*! \brief the loads above have arrived; `r` passes through so that no use of it moves above the wait */
 __device__ __forceinline__ void WaitColumns(uint32_t (&r)[32]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"
@@ -205,6 +251,14 @@ __device__ __forceinline__ void WaitColumns(uint32_t (&r)[32]) {
                  "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]),
                  "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
                  "+r"(r[30]), "+r"(r[31])
+               :
+               : "memory");
+}
+
+__device__ __forceinline__ void WaitColumns(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
                :
                : "memory");
 }

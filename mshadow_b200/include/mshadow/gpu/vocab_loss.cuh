@@ -22,9 +22,13 @@
  * and d^T x is the piece's gradient of W.  The rounding of d is the one rounding between inputs and
  * outputs besides the final one: it is what lets the second and third product run on 16-bit
  * operands, and it is relative to each d (half a unit of its last place), so the gradients come
- * out about as exact as their own final rounding leaves them.  Before it d is multiplied by a power
- * of two that brings the largest row scale to 2^14 .. 2^15 -- a mean over thousands of tokens puts most
- * of d below the smallest binary16 number otherwise -- and the results are divided by it again, exactly.
+ * out about as exact as their own final rounding leaves them.  What is stored is not d itself but
+ *     d' = (p - q) / (1 - a) * gloss * 2^k,     d = d' * scale * (1 - a) * 2^-k
+ * with 2^k bringing the largest of gloss / (1 - a) to 2^14 .. 2^15, and the factor on the right applied to the
+ * finished sums: a mean over thousands of tokens would put most of d below the smallest binary16 number, and the
+ * label's term, which carries most of the gradient while p is small, would be rounded by the same fraction in every
+ * row -- as stored it is a power of two.  (With scale and 1 - a inside: gradients of 0.31 % instead of 0.17 %
+ * relative error, bf16, smoothing 0.1; 0.21 instead of 0.17 % without smoothing.)
  *
  * Live tokens are packed together first (PackRowsKernel): tiles of padding cost nothing, whatever
  * their hidden states hold -- an infinity in a padded row does not meet a zero of d -- and the
@@ -46,7 +50,10 @@ namespace vloss {
 
 const int kTileN = 256;       // columns of a tile
 const int kStepK = 64;        // contraction elements per stage (one 128-byte swizzle row)
-const int kThreads = 256;     // warp 0: copies, warp 1: products, warp 2: tensor memory, warps 4-7: epilogue
+const int kThreads = 384;     // warp 0: copies, warp 1: products, warp 2: tensor memory, warps 4-11: epilogue
+const int kHalfN = kTileN / 2;  // columns of a tile that one epilogue group (four warps, a thread per row) takes
+const int kChunkSteps = 16;   // kStat: stages per run of accumulation in tensor memory (1024 contraction elements)
+const uint32_t kBoxOut = 128 * 128;  // a box of 128 rows by 128 bytes, on its way out through shared memory
 const int kPadRows = 256;     // token rows of the scratch matrices are padded to this
 const float kLog2e = 1.4426950408889634f;
 
@@ -71,7 +78,8 @@ struct StageShape {
   static const uint32_t kBytesB = kRowsN * kStepK * 2;
   static const uint32_t kStage = kBytesA + kBytesB;
   static const int kStages = kCtas == 2 ? 6 : 4;
-  static const size_t kSmem = kStage * kStages + 1024;               // + alignment to the swizzle's 1024 bytes
+  static const uint32_t kOut = kStage * kStages;                     // a box per epilogue group
+  static const size_t kSmem = kOut + 2 * kBoxOut + 1024;  // + alignment to the swizzle's 1024 bytes
 };
 
 struct GemmArgs {
@@ -88,30 +96,28 @@ struct GemmArgs {
   // kStat, kDelta
   int32_t cols;          // columns of the piece that exist
   int32_t col0;          // class of the piece's first column
+  int32_t tile_n;        // kStat: columns of a tile, a multiple of 16 * CTAs and at most kTileN
   int32_t tile0;         // kStat: tiles of the pieces before this one
   int64_t pad_rows;
   const int32_t *label;
-  float2 *part;          // [tile][row]: maximum and sum of exp(z - maximum)
-  float *part_sum;       // [tile][row]: sum of z, or null
+  float2 *part;          // [tile][half][row]: maximum and sum of exp(z - maximum)
+  float *part_sum;       // [tile][half][row]: sum of z, or null
   float *label_logit;    // [row]
   const float *lse2;     // [row]: lse in base 2
   const float *row_scale;
   float q_label, q_other;
   int bf16;
-  uint16_t *delta;       // [row][ld_delta]
-  int64_t ld_delta;
   // kDataGrad
-  float *acc;            // [slice][row][ld_acc]
-  int64_t ld_acc, acc_slice;
   int accumulate;
   // kWeightGrad
-  const float *inv_scale;  // device word: what undoes the power of two in row_scale
+  const float *inv_scale;  // device word: what takes sums of d' to the gradient
   void *out;
   int64_t ld_out;
   int32_t out_rows, out_cols;
   int out_type;          // kFloat32, kFloat16, kBfloat16
   int out_add;
   int out_vec;           // rows of `out` start on 16-byte boundaries
+  int out_tiled;         // written by tiled copies (map_out)
   int *status;
 };
 
@@ -154,99 +160,162 @@ __device__ __forceinline__ Unit UnitOf(int u, int m_tiles, int n_tiles, int grou
   return t;
 }
 
-// ---- epilogues: one thread per row of the tile, 32 columns at a time ----------------------------
+// ---- epilogues: one thread per row of the tile and half of its columns ----------------------------
 
-/*!
- * \brief running maximum and sum of exponentials of one row.  The difference to the maximum is taken before the
- *  change of base (a product with log2 e folded into one multiply-add would save an addition, but it
- *  rounds at the size of the logit): the largest term is then exactly 1, and the loss of a token whose
- *  label has the largest logit is log(sum) with nothing cancelled, never negative.
- */
-struct RowStat {
-  float ref, sum, total;
-  int label;  // column of the label within the tile, or outside [0, kTileN)
+/*! \brief what an epilogue group (four warps) knows about its half of a tile */
+struct Half {
+  uint32_t acc;      // tensor memory of this thread's row, first column of the half
+  int64_t row;       // row of the matrix
+  int col;           // first column of the half, within the piece
+  uint32_t box;      // shared memory of the group's outgoing box
+  int group, thread; // 0 / 1; thread of the group: 0 .. 127
 };
 
-template <bool kTotal>
-__device__ __forceinline__ void StatColumns(const uint32_t (&r)[32], int c0, int limit, RowStat *st, float *label_logit) {
-  float v[32];
-#pragma unroll
-  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
-  if (kTotal) {
-    float t = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 32; ++i) t += c0 + i < limit ? v[i] : 0.0f;
-    st->total += t;
-  }
-  if (c0 + 32 > limit) {  // columns past the vocabulary weigh nothing
-#pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      if (c0 + i >= limit) v[i] = -INFINITY;
-    }
-  }
-  float m[4] = {v[0], v[1], v[2], v[3]};
-#pragma unroll
-  for (int i = 4; i < 32; ++i) m[i & 3] = fmaxf(m[i & 3], v[i]);
-  const float top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
-  const float ref = fmaxf(st->ref, top);
-  const float from = ref == -INFINITY ? 0.0f : ref;  // nothing but -infinity so far: any finite reference serves
-  float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-  for (int i = 0; i < 32; ++i) s[i & 3] += Exp2((v[i] - from) * kLog2e);
-  st->sum = st->sum * Exp2((st->ref - from) * kLog2e) + ((s[0] + s[1]) + (s[2] + s[3]));
-  st->ref = ref;
-  if (static_cast<unsigned>(st->label - c0) < 32u) {
-    const int at = st->label - c0;
-    float z = v[0];
-#pragma unroll
-    for (int i = 1; i < 32; ++i) z = i == at ? v[i] : z;
-    *label_logit = z;
-  }
+/*! \brief the group's outgoing box is free again */
+__device__ __forceinline__ void BoxFree(const Half &t) {
+  if (t.thread == 0) tc5::WaitStoresRead();
+  tc5::NamedBarrier(1 + t.group, 128);
+}
+/*! \brief 16 bytes of this thread's row of the box, in the place the 128-byte swizzle gives them */
+__device__ __forceinline__ void BoxPut(const Half &t, int chunk, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  const uint32_t at = t.box + t.thread * 128 + ((chunk ^ (t.thread & 7)) << 4);
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+/*! \brief the box is full: one thread sends it to column x, row y of the output */
+template <bool kAdd>
+__device__ __forceinline__ void BoxSend(const Half &t, const CUtensorMap *map, int x, int y) {
+  tma::FenceAsyncShared();
+  tc5::NamedBarrier(1 + t.group, 128);
+  if (t.thread == 0) tc5::StoreBox<kAdd>(map, x, y, t.box);
 }
 
-__device__ __forceinline__ void DeltaColumns(const uint32_t (&r)[32], int c0, int limit, int label, float lse2,
-                                             float scale, const GemmArgs &a, uint16_t *out) {
+/*!
+ * \brief maximum and sum of exponentials of the half row.  The difference to the maximum is taken before the change of
+ *  base (a product with log2 e folded into one multiply-add would save an addition, but it rounds at
+ *  the size of the logit): the largest term is then exactly 1, and the loss of a token whose label has the
+ *  largest logit is log(sum) with nothing cancelled, never negative.  The exponentials' rate (16 a
+ *  cycle and SM) leaves room for the addition.
+ */
+__device__ __forceinline__ void StatHalf(float (&v)[kHalfN], const Half &t, int limit, int label, int64_t at, const GemmArgs &a) {
+  if (a.part_sum != nullptr) {
+    float total = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kHalfN; ++i) total += i < limit ? v[i] : 0.0f;
+    a.part_sum[at] = total;
+  }
+  if (limit < kHalfN) {  // columns past the vocabulary weigh nothing
+#pragma unroll
+    for (int i = 0; i < kHalfN; ++i) v[i] = i < limit ? v[i] : -INFINITY;
+  }
+  float m[8];
+#pragma unroll
+  for (int i = 0; i < kHalfN; ++i) m[i & 7] = i < 8 ? v[i] : fmaxf(m[i & 7], v[i]);
+#pragma unroll
+  for (int i = 4; i > 0; i >>= 1) {
+#pragma unroll
+    for (int j = 0; j < i; ++j) m[j] = fmaxf(m[j], m[j + i]);
+  }
+  const float from = m[0] == -INFINITY ? 0.0f : m[0];  // nothing but -infinity: any finite reference serves
+  if (label >= 0 && label < min(limit, kHalfN)) {
+    float z = v[0];
+#pragma unroll
+    for (int i = 1; i < kHalfN; ++i) z = i == label ? v[i] : z;
+    a.label_logit[t.row] = z;
+  }
+  float s[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int i = 0; i < kHalfN; ++i) s[i & 7] += Exp2((v[i] - from) * kLog2e);
+#pragma unroll
+  for (int i = 4; i > 0; i >>= 1) {
+#pragma unroll
+    for (int j = 0; j < i; ++j) s[j] += s[j + i];
+  }
+  a.part[at] = make_float2(m[0], s[0]);
+}
+
+/*! \brief d' of 32 columns */
+__device__ __forceinline__ void DeltaColumns(const uint32_t (&r)[32], int limit, int label, float lse2, float scale,
+                                             const GemmArgs &a, uint32_t (&out)[16]) {
   float d[32];
 #pragma unroll
   for (int i = 0; i < 32; ++i) d[i] = (Exp2(__fmaf_rn(__uint_as_float(r[i]), kLog2e, -lse2)) - a.q_other) * scale;
-  if (static_cast<unsigned>(label - c0) < 32u) {
-    const int at = label - c0;
+  if (static_cast<unsigned>(label) < 32u) {
 #pragma unroll
     for (int i = 0; i < 32; ++i) {
-      if (i == at) d[i] = (Exp2(__fmaf_rn(__uint_as_float(r[i]), kLog2e, -lse2)) - a.q_label) * scale;
+      if (i == label) d[i] = (Exp2(__fmaf_rn(__uint_as_float(r[i]), kLog2e, -lse2)) - a.q_label) * scale;
     }
   }
-  if (c0 + 32 > limit) {
+  if (limit < 32) {
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      if (c0 + i >= limit) d[i] = 0.0f;
-    }
+    for (int i = 0; i < 32; ++i) d[i] = i < limit ? d[i] : 0.0f;
   }
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    uint4 p;
-    p.x = PackPair(d[8 * q], d[8 * q + 1], a.bf16);
-    p.y = PackPair(d[8 * q + 2], d[8 * q + 3], a.bf16);
-    p.z = PackPair(d[8 * q + 4], d[8 * q + 5], a.bf16);
-    p.w = PackPair(d[8 * q + 6], d[8 * q + 7], a.bf16);
-    reinterpret_cast<uint4 *>(out)[q] = p;
+  for (int i = 0; i < 16; ++i) out[i] = PackPair(d[2 * i], d[2 * i + 1], a.bf16);
+}
+
+__device__ __forceinline__ void DeltaHalf(const Half &t, int limit, int label, float lse2, float scale, const CUtensorMap *map,
+                                          int row0, const GemmArgs &a) {
+#pragma unroll 1
+  for (int b = 0; b < kHalfN / 64; ++b) {
+    uint32_t r0[32], r1[32], p0[16], p1[16];
+    tc5::LoadColumns(t.acc + b * 64, r0);
+    tc5::LoadColumns(t.acc + b * 64 + 32, r1);
+    tc5::WaitColumns(r0);
+    tc5::WaitColumns(r1);
+    DeltaColumns(r0, limit - b * 64, label - b * 64, lse2, scale, a, p0);
+    DeltaColumns(r1, limit - b * 64 - 32, label - b * 64 - 32, lse2, scale, a, p1);
+    BoxFree(t);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      BoxPut(t, q, p0[4 * q], p0[4 * q + 1], p0[4 * q + 2], p0[4 * q + 3]);
+      BoxPut(t, 4 + q, p1[4 * q], p1[4 * q + 1], p1[4 * q + 2], p1[4 * q + 3]);
+    }
+    BoxSend<false>(t, map, t.col + b * 64, row0);
   }
 }
 
-__device__ __forceinline__ void AccColumns(const uint32_t (&r)[32], float *out, int accumulate) {
+/*! \brief the half tile as binary32, times `factor`, stored or added */
+template <bool kAdd>
+__device__ __forceinline__ void FloatHalf(const Half &t, float factor, const CUtensorMap *map, int row0, int row1) {
+#pragma unroll 1
+  for (int b = 0; b < kHalfN / 32; ++b) {
+    uint32_t r[32];
+    tc5::LoadColumns(t.acc + b * 32, r);
+    tc5::WaitColumns(r);
 #pragma unroll
-  for (int q = 0; q < 8; ++q) {
-    float4 v = make_float4(__uint_as_float(r[4 * q]), __uint_as_float(r[4 * q + 1]), __uint_as_float(r[4 * q + 2]),
-                           __uint_as_float(r[4 * q + 3]));
-    float4 *p = reinterpret_cast<float4 *>(out) + q;
-    if (accumulate) {
-      const float4 o = *p;
-      v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
-    }
-    *p = v;
+    for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * factor);
+    BoxFree(t);
+#pragma unroll
+    for (int q = 0; q < 8; ++q) BoxPut(t, q, r[4 * q], r[4 * q + 1], r[4 * q + 2], r[4 * q + 3]);
+    BoxSend<kAdd>(t, map, t.col + b * 32, row0 + row1);
   }
 }
 
+/*! \brief the half tile in the operands' type, times `factor` */
+__device__ __forceinline__ void PackedHalf(const Half &t, float factor, int bf16, const CUtensorMap *map, int row0) {
+#pragma unroll 1
+  for (int b = 0; b < kHalfN / 64; ++b) {
+    uint32_t r0[32], r1[32];
+    tc5::LoadColumns(t.acc + b * 64, r0);
+    tc5::LoadColumns(t.acc + b * 64 + 32, r1);
+    tc5::WaitColumns(r0);
+    tc5::WaitColumns(r1);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      r0[i] = PackPair(__uint_as_float(r0[2 * i]) * factor, __uint_as_float(r0[2 * i + 1]) * factor, bf16);
+      r1[i] = PackPair(__uint_as_float(r1[2 * i]) * factor, __uint_as_float(r1[2 * i + 1]) * factor, bf16);
+    }
+    BoxFree(t);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      BoxPut(t, q, r0[4 * q], r0[4 * q + 1], r0[4 * q + 2], r0[4 * q + 3]);
+      BoxPut(t, 4 + q, r1[4 * q], r1[4 * q + 1], r1[4 * q + 2], r1[4 * q + 3]);
+    }
+    BoxSend<false>(t, map, t.col + b * 64, row0);
+  }
+}
+
+/*! \brief 32 columns of a row of grad W by plain accesses: rows that the tiled copy cannot address, and additions */
 __device__ __forceinline__ void WeightColumns(const uint32_t (&r)[32], int64_t row, int col, float inv, const GemmArgs &a) {
   const int left = a.out_cols - col;
   if (left <= 0) return;
@@ -307,59 +376,20 @@ __device__ __forceinline__ void WeightColumns(const uint32_t (&r)[32], int64_t r
   }
 }
 
-template <int kMode>
-__device__ __forceinline__ void FinishTile(const Unit &u, uint32_t acc, int64_t row, int live, const GemmArgs &a) {
-  uint32_t r[32];
-  if (kMode == kStat || kMode == kDelta) {
-    const int limit = a.cols - u.n * kTileN;  // columns of this tile that exist
-    const int col = a.col0 + u.n * kTileN;    // class of its first column
-    const int label = row < live ? a.label[row] : -1;
-    if (kMode == kStat) {
-      RowStat st = {-INFINITY, 0.0f, 0.0f, label < 0 ? -1 : label - col};
-      const int chunks = min(kTileN / 32, (limit + 31) / 32);
-      for (int c = 0; c < chunks; ++c) {
-        tc5::LoadColumns(acc + c * 32, r);
-        tc5::WaitColumns(r);
-        if (a.part_sum != nullptr) StatColumns<true>(r, c * 32, limit, &st, a.label_logit + row);
-        else StatColumns<false>(r, c * 32, limit, &st, a.label_logit + row);
-      }
-      const int64_t at = static_cast<int64_t>(a.tile0 + u.n) * a.pad_rows + row;
-      a.part[at] = make_float2(st.ref, st.sum);
-      if (a.part_sum != nullptr) a.part_sum[at] = st.total;
-    } else {
-      const int at = label < 0 ? -1 : label - col;
-      const float lse2 = a.lse2[row], scale = a.row_scale[row];  // rows past the live ones: 0 and 0
-      uint16_t *out = a.delta + row * a.ld_delta + u.n * kTileN;
-      for (int c = 0; c < kTileN / 32; ++c) {
-        tc5::LoadColumns(acc + c * 32, r);
-        tc5::WaitColumns(r);
-        DeltaColumns(r, c * 32, limit, at, lse2, scale, a, out + c * 32);
-      }
-    }
-  } else if (kMode == kDataGrad) {
-    float *out = a.acc + u.slice * a.acc_slice + row * a.ld_acc + u.n * kTileN;
-    for (int c = 0; c < kTileN / 32; ++c) {
-      tc5::LoadColumns(acc + c * 32, r);
-      tc5::WaitColumns(r);
-      AccColumns(r, out + c * 32, a.accumulate);
-    }
-  } else {
-    const float inv = a.inv_scale[0];
-    for (int c = 0; c < kTileN / 32; ++c) {
-      tc5::LoadColumns(acc + c * 32, r);
-      tc5::WaitColumns(r);
-      if (row < a.out_rows) WeightColumns(r, row, u.n * kTileN + c * 32, inv, a);
-    }
-  }
-}
-
 /*!
  * \brief persistent product kernel of all four modes.  kCtas CTAs (a cluster) share a tile of
- *  128 * kCtas rows by 256 columns.  Block of 256 threads; dynamic shared memory StageShape<kCtas>::kSmem.
+ *  128 * kCtas rows by 256 columns (kStat: a.tile_n).  Dynamic shared memory StageShape<kCtas>::kSmem.
+ *
+ *  Tensor memory holds two sets of accumulators; the products of one run into them while the epilogue empties the
+ *  other.  A set is a whole tile, except in kStat: there the contraction is cut into runs of at most
+ *  1024 elements, which the epilogue adds up in registers.  The tensor cores cut off, rather than
+ *  round, each time they add to an accumulator, always towards zero: over 4096 elements that moved
+ *  the loss by 1.8e-6 of its value, against 6e-7 for a product in plain binary32.
  */
 template <int kMode, int kCtas>
 __global__ void __launch_bounds__(kThreads, 1)
-VocabGemmKernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const GemmArgs a) {
+VocabGemmKernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                const __grid_constant__ CUtensorMap map_out, const GemmArgs a) {
   typedef StageShape<kCtas> S;
   typedef Layout<kMode> L;
   extern __shared__ uint8_t raw[];
@@ -376,10 +406,11 @@ VocabGemmKernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
     }
     for (int s = 0; s < 2; ++s) {
       tma::BarrierInit(&acc_full[s], 1);
-      tma::BarrierInit(&acc_empty[s], 128 * kCtas);
+      tma::BarrierInit(&acc_empty[s], 8 * kCtas);
     }
     tc5::PrefetchMap(&map_a);
     tc5::PrefetchMap(&map_b);
+    if (kMode != kStat) tc5::PrefetchMap(&map_out);
   }
   if (warp == 2) tc5::AllocTensorMemory<kCtas>(&tmem_slot);
   tc5::FenceBefore();
@@ -391,23 +422,26 @@ VocabGemmKernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
 
   const int live = a.live != nullptr ? *a.live : a.tokens;
   const int tile_m = 128 * kCtas;
+  const int tile_n = kMode == kStat ? a.tile_n : kTileN;
+  const int rows_n = tile_n / kCtas;  // rows of B that this CTA loads
   // an empty batch still passes one tile of zeros through the products that end in d and in grad W
   const int m_tiles = kMode == kWeightGrad ? a.m_tiles
                       : kMode == kDelta    ? max(1, (live + tile_m - 1) / tile_m)
                                            : (live + tile_m - 1) / tile_m;
   const int k_blocks = kMode == kWeightGrad ? max(1, (live + kStepK - 1) / kStepK) : a.k_blocks;
+  const int runs = kMode == kStat ? (k_blocks + kChunkSteps - 1) / kChunkSteps : 1;
   const int units = m_tiles * a.n_tiles * a.slices;
   const int first = blockIdx.x / kCtas, step = gridDim.x / kCtas;
 
-  if (warp == 0) {
-    if (lane == 0) {
+  if (warp < 4) {
+    if (warp == 0 && lane == 0) {
       uint32_t fill = 0;  // stages filled so far
       bool ok = true;
       for (int w = first; ok && w < units; w += step) {
         const Unit u = UnitOf(w, m_tiles, a.n_tiles, a.group);
         const int k_begin = u.slice * k_blocks / a.slices, k_end = (u.slice + 1) * k_blocks / a.slices;
         const int m0 = u.m * tile_m + static_cast<int>(rank) * 128;
-        const int n0 = u.n * kTileN + static_cast<int>(rank) * S::kRowsN;
+        const int n0 = u.n * tile_n + static_cast<int>(rank) * rows_n;
         for (int kb = k_begin; kb < k_end; ++kb, ++fill) {
           const int s = fill % S::kStages;
           const uint32_t use = fill / S::kStages;
@@ -416,7 +450,7 @@ VocabGemmKernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
             break;
           }
           const uint32_t bar = kCtas == 2 ? tc5::MapToRank(tma::SharedAddr(&full[s]), 0) : tma::SharedAddr(&full[s]);
-          if (rank == 0) tma::BarrierExpect(&full[s], S::kStage * kCtas);
+          if (rank == 0) tma::BarrierExpect(&full[s], (S::kBytesA + rows_n * kStepK * 2) * kCtas);
           const uint32_t sa = smem + s * S::kStage, sb = sa + S::kBytesA;
           const int k0 = kb * kStepK;
           if (L::kAAcross) {
@@ -440,60 +474,122 @@ VocabGemmKernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
       for (uint32_t i = fill > S::kStages ? fill - S::kStages : 0; i < fill; ++i) {
         if (!tma::WaitBounded(&empty[i % S::kStages], (i / S::kStages) & 1u)) atomicExch(a.status, tma::kStatusBulkCopyTimeout);
       }
-    }
-  } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
-      uint32_t fill = 0, tile = 0;
+    } else if (warp == 1 && lane == 0 && rank == 0) {
+      uint32_t fill = 0, turn = 0;
       bool ok = true;
-      for (int w = first; ok && w < units; w += step, ++tile) {
-        const Unit u = UnitOf(w, m_tiles, a.n_tiles, a.group);
-        const int k_begin = u.slice * k_blocks / a.slices, k_end = (u.slice + 1) * k_blocks / a.slices;
-        const uint32_t half = tile & 1u, use = tile >> 1;
-        if (use > 0 && !tma::WaitBounded(&acc_empty[half], (use - 1) & 1u)) {
-          ok = false;
-          break;
-        }
-        tc5::FenceAfter();
-        const uint32_t acc = tmem + half * kTileN;
-        for (int kb = k_begin; kb < k_end; ++kb, ++fill) {
-          const int s = fill % S::kStages;
-          if (!tma::WaitBounded(&full[s], (fill / S::kStages) & 1u)) {
+      for (int w = first; ok && w < units; w += step) {
+        const int slice = w / (m_tiles * a.n_tiles);
+        const int k_first = slice * k_blocks / a.slices, k_count = (slice + 1) * k_blocks / a.slices - k_first;
+        for (int run = 0; ok && run < runs; ++run, ++turn) {
+          const int k_begin = k_first + run * k_count / runs, k_end = k_first + (run + 1) * k_count / runs;
+          const uint32_t half = turn & 1u, use = turn >> 1;
+          if (use > 0 && !tma::WaitBounded(&acc_empty[half], (use - 1) & 1u)) {
             ok = false;
             break;
           }
           tc5::FenceAfter();
-          const uint32_t sa = smem + s * S::kStage, sb = sa + S::kBytesA;
-          const uint64_t da = L::kAAcross ? tc5::DescAcrossK(sa) : tc5::DescAlongK(sa);
-          const uint64_t db = L::kBAcross ? tc5::DescAcrossK(sb) : tc5::DescAlongK(sb);
-          const uint32_t step_a = L::kAAcross ? 2048 >> 4 : 32 >> 4, step_b = L::kBAcross ? 2048 >> 4 : 32 >> 4;
+          const uint32_t acc = tmem + half * kTileN;
+          for (int kb = k_begin; kb < k_end; ++kb, ++fill) {
+            const int s = fill % S::kStages;
+            if (!tma::WaitBounded(&full[s], (fill / S::kStages) & 1u)) {
+              ok = false;
+              break;
+            }
+            tc5::FenceAfter();
+            const uint32_t sa = smem + s * S::kStage, sb = sa + S::kBytesA;
+            const uint64_t da = L::kAAcross ? tc5::DescAcrossK(sa) : tc5::DescAlongK(sa);
+            const uint64_t db = L::kBAcross ? tc5::DescAcrossK(sb) : tc5::DescAlongK(sb);
+            const uint32_t step_a = L::kAAcross ? 2048 >> 4 : 32 >> 4, step_b = L::kBAcross ? 2048 >> 4 : 32 >> 4;
 #pragma unroll
-          for (int j = 0; j < kStepK / 16; ++j) {
-            tc5::Multiply<kCtas>(acc, da + j * step_a, db + j * step_b, a.instr, kb > k_begin || j > 0);
+            for (int j = 0; j < kStepK / 16; ++j) {
+              tc5::Multiply<kCtas>(acc, da + j * step_a, db + j * step_b, a.instr, kb > k_begin || j > 0);
+            }
+            tc5::CommitTo<kCtas>(&empty[s]);
           }
-          tc5::CommitTo<kCtas>(&empty[s]);
+          if (ok) tc5::CommitTo<kCtas>(&acc_full[half]);
         }
-        if (ok) tc5::CommitTo<kCtas>(&acc_full[half]);
       }
       if (!ok) atomicExch(a.status, tma::kStatusBulkCopyTimeout);
     }
-  } else if (warp >= 4) {
-    const int quarter = warp - 4;
-    uint32_t tile = 0;
-    for (int w = first; w < units; w += step, ++tile) {
-      const Unit u = UnitOf(w, m_tiles, a.n_tiles, a.group);
-      const uint32_t half = tile & 1u;
-      const bool ready = tma::WaitBounded(&acc_full[half], (tile >> 1) & 1u);
-      if (!__all_sync(0xffffffffu, ready)) {
-        if (lane == 0) atomicExch(a.status, tma::kStatusBulkCopyTimeout);
-        break;
-      }
+  } else {
+    Half t;
+    t.group = (warp - 4) >> 2;
+    t.thread = threadIdx.x - 128 - t.group * 128;
+    t.box = smem + S::kOut + t.group * kBoxOut;
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    uint32_t turn = 0;
+    bool ok = true;
+    // accumulators ready / handed back: the group acts as one, so that its barriers stay matched if a wait gives up
+    auto ready = [&]() {
+      const bool mine = tma::WaitBounded(&acc_full[turn & 1u], (turn >> 1) & 1u);
+      ok = tc5::NamedBarrierAnd(1 + t.group, 128, mine);
       tc5::FenceAfter();
-      const int64_t row = static_cast<int64_t>(u.m) * tile_m + static_cast<int>(rank) * 128 + quarter * 32 + lane;
-      FinishTile<kMode>(u, tmem + half * kTileN + (static_cast<uint32_t>(quarter * 32) << 16), row, live, a);
+      t.acc = tmem + (turn & 1u) * kTileN + t.group * kHalfN + lanes;
+      return ok;
+    };
+    auto release = [&]() {
       tc5::FenceBefore();
-      if (kCtas == 2) tc5::ArriveCluster(tc5::MapToRank(tma::SharedAddr(&acc_empty[half]), 0));
-      else tma::BarrierArrive(&acc_empty[half]);
+      __syncwarp();
+      if (lane == 0) {
+        if (kCtas == 2) tc5::ArriveCluster(tc5::MapToRank(tma::SharedAddr(&acc_empty[turn & 1u]), 0));
+        else tma::BarrierArrive(&acc_empty[turn & 1u]);
+      }
+      ++turn;
+    };
+    for (int w = first; w < units; w += step) {
+      const Unit u = UnitOf(w, m_tiles, a.n_tiles, a.group);
+      const int row0 = u.m * tile_m + static_cast<int>(rank) * 128;
+      t.row = row0 + t.thread;
+      t.col = u.n * tile_n + t.group * kHalfN;
+      const int limit = min(a.cols - t.col, tile_n - t.group * kHalfN);  // columns of this half that exist
+      if (kMode == kStat) {
+        float v[kHalfN];
+        for (int run = 0; run < runs; ++run) {
+          if (!ready()) break;
+#pragma unroll
+          for (int c = 0; c < kHalfN / 16; ++c) {
+            uint32_t r[16];
+            tc5::LoadColumns(t.acc + c * 16, r);
+            tc5::WaitColumns(r);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[c * 16 + i] = run == 0 ? __uint_as_float(r[i]) : v[c * 16 + i] + __uint_as_float(r[i]);
+          }
+          release();
+        }
+        if (!ok) break;
+        const int label = t.row < live ? a.label[t.row] : -1;
+        const int64_t at = (static_cast<int64_t>(a.tile0 + u.n) * 2 + t.group) * a.pad_rows + t.row;
+        StatHalf(v, t, limit, label < 0 ? -1 : label - a.col0 - t.col, at, a);
+        continue;
+      }
+      if (!ready()) break;
+      if (kMode == kDelta) {
+        const int label = t.row < live ? a.label[t.row] : -1;
+        // rows past the live ones: lse and scale are 0, the data row is zero, and so is d'
+        DeltaHalf(t, limit, label < 0 ? -1 : label - a.col0 - t.col, a.lse2[t.row], a.row_scale[t.row], &map_out, row0, a);
+      } else if (kMode == kDataGrad) {
+        const int part = static_cast<int>(u.slice * a.pad_rows);
+        if (a.accumulate) FloatHalf<true>(t, 1.0f, &map_out, row0, part);
+        else FloatHalf<false>(t, 1.0f, &map_out, row0, part);
+      } else {
+        const float inv = a.inv_scale[0];
+        if (a.out_tiled) {
+          if (a.out_type == kFloat32) FloatHalf<false>(t, inv, &map_out, row0, 0);
+          else PackedHalf(t, inv, a.out_type == kBfloat16, &map_out, row0);
+        } else {
+#pragma unroll 1
+          for (int c = 0; c < kHalfN / 32; ++c) {
+            uint32_t r[32];
+            tc5::LoadColumns(t.acc + c * 32, r);
+            tc5::WaitColumns(r);
+            if (t.row < a.out_rows) WeightColumns(r, t.row, t.col + c * 32, inv, a);
+          }
+        }
+      }
+      release();
     }
+    if (!ok && t.thread == 0) atomicExch(a.status, tma::kStatusBulkCopyTimeout);
+    if (kMode != kStat && t.thread == 0) tc5::WaitStores();
   }
   __syncwarp();
   tc5::FenceBefore();
@@ -514,14 +610,14 @@ struct PackArgs {
   int64_t pad_rows;      // n rounded up to kPadRows
   uint16_t *packed;      // [pad_rows][ld_packed]
   int64_t ld_packed;
-  int32_t *words;        // [0] = live rows, [1] = inv_scale (a float)
+  int32_t *words;        // [0] = live rows, [1] = what takes d' to d (a float)
   int32_t *row_of;       // [pad_rows] token of packed row (forward)
   int32_t *pos_of;       // [n] packed row of token, or -1 (backward)
   int32_t *label_of;     // [pad_rows] label of packed row
   float *loss, *lse_out; // forward: rows that do not count become 0
   const float *lse;      // backward
   const float *gloss;    // backward, may be null
-  float scale;
+  float scale, q_label;
   float *lse2, *row_scale;  // [pad_rows], backward
   int vec;               // 16-byte copies possible
   int rows_per_cta;
@@ -568,7 +664,7 @@ __global__ void __launch_bounds__(256) PackRowsKernel(const PackArgs a) {
   // the power of two that brings the largest row scale to [2^14, 2^15)
   float up = 1.0f, down = 1.0f;
   if (a.row_scale != nullptr) {
-    const float largest = fabsf(a.scale) * (a.gloss != nullptr ? top : 1.0f);
+    const float largest = (a.gloss != nullptr ? top : 1.0f) / a.q_label;
     if (largest > 0.0f && largest < INFINITY) {
       const int e = min(100, max(-100, 14 - ilogbf(largest)));
       up = __int_as_float((127 + e) << 23);
@@ -590,7 +686,7 @@ __global__ void __launch_bounds__(256) PackRowsKernel(const PackArgs a) {
     a.label_of[pos] = label;
     if (a.row_of != nullptr) a.row_of[pos] = i;
     if (a.row_scale != nullptr) {
-      a.row_scale[pos] = a.scale * (a.gloss != nullptr ? a.gloss[i] : 1.0f) * up;
+      a.row_scale[pos] = (a.gloss != nullptr ? a.gloss[i] : 1.0f) / a.q_label * up;
       a.lse2[pos] = a.lse[i] * kLog2e;
     }
   }
@@ -602,7 +698,7 @@ __global__ void __launch_bounds__(256) PackRowsKernel(const PackArgs a) {
   }
   if (blockIdx.x == 0 && tid == 0) {
     a.words[0] = total;
-    reinterpret_cast<float *>(a.words)[1] = down;
+    reinterpret_cast<float *>(a.words)[1] = a.scale * a.q_label * down;
   }
   __syncthreads();
   for (int t = warp; t < a.rows_per_cta; t += 8) {
@@ -636,7 +732,7 @@ AlignRowsKernel(uint16_t *dst, int64_t ld_dst, const uint16_t *src, int64_t ld_s
 
 struct JoinArgs {
   const int32_t *live;
-  int32_t tokens, tiles, v;
+  int32_t tokens, parts, v;
   int64_t pad_rows;
   const float2 *part;
   const float *part_sum, *label_logit;
@@ -646,34 +742,41 @@ struct JoinArgs {
   float *loss, *lse;
 };
 
-/*! \brief joins the tiles' maxima and sums row by row: 32 rows per CTA, eight threads of a row share its tiles */
+/*!
+ * \brief joins the maxima and sums of the tile halves row by row: 32 rows per CTA, sixteen threads of a row take
+ *  every sixteenth part and are joined pairwise
+ */
 template <int kUnused>
-__global__ void __launch_bounds__(256) JoinTilesKernel(const JoinArgs a) {
+__global__ void __launch_bounds__(512) JoinTilesKernel(const JoinArgs a) {
   gpu_rt::GridDependencySync();
-  __shared__ float s_ref[8][33], s_sum[8][33], s_total[8][33];
+  __shared__ float s_ref[16][32], s_sum[16][32], s_total[16][32];
   const int live = a.live != nullptr ? *a.live : a.tokens;
   const int r = threadIdx.x & 31, q = threadIdx.x >> 5;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * 32 + r;
   if (blockIdx.x * 32 >= live) return;
   float ref = -INFINITY, sum = 0.0f, total = 0.0f;
+  auto join = [&](float other, float other_sum) {
+    const float top = fmaxf(ref, other), from = top == -INFINITY ? 0.0f : top;
+    sum = sum * Exp2((ref - from) * kLog2e) + other_sum * Exp2((other - from) * kLog2e);
+    ref = top;
+  };
   if (row < live) {
-    for (int t = q; t < a.tiles; t += 8) {
+    for (int t = q; t < a.parts; t += 16) {
       const float2 p = a.part[t * a.pad_rows + row];
-      const float top = fmaxf(ref, p.x), from = top == -INFINITY ? 0.0f : top;
-      sum = sum * Exp2((ref - from) * kLog2e) + p.y * Exp2((p.x - from) * kLog2e);
-      ref = top;
+      join(p.x, p.y);
       if (a.part_sum != nullptr) total += a.part_sum[t * a.pad_rows + row];
     }
   }
-  s_ref[q][r] = ref, s_sum[q][r] = sum, s_total[q][r] = total;
-  __syncthreads();
-  if (q != 0 || row >= live) return;
-  for (int w = 1; w < 8; ++w) {
-    const float other = s_ref[w][r], top = fmaxf(ref, other), from = top == -INFINITY ? 0.0f : top;
-    sum = sum * Exp2((ref - from) * kLog2e) + s_sum[w][r] * Exp2((other - from) * kLog2e);
-    ref = top;
-    total += s_total[w][r];
+  for (int half = 8; half > 0; half >>= 1) {
+    s_ref[q][r] = ref, s_sum[q][r] = sum, s_total[q][r] = total;
+    __syncthreads();
+    if (q < half) {
+      join(s_ref[q + half][r], s_sum[q + half][r]);
+      total += s_total[q + half][r];
+    }
+    __syncthreads();
   }
+  if (q != 0 || row >= live) return;
   const int32_t label = a.label[row];
   const int64_t to = a.row_of != nullptr ? a.row_of[row] : row;
   if (!IsLive(label, a.ignore, a.v)) {
@@ -747,14 +850,7 @@ const int64_t kDeltaBytes = int64_t(512) << 20;  // piece of d: larger pieces me
 const int64_t kCopyBytes = int64_t(128) << 20;   // piece of W copied to aligned rows where the caller's are not
 
 inline int64_t RoundUp(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
-
-/*! \brief how a call is cut, and where its scratch matrices lie (offsets in bytes) */
-struct Plan {
-  bool pack, copy_w;
-  int64_t pad_rows, ld_x, ld_w, piece, ld_acc, tiles;
-  int slices, ctas;
-  int64_t words, row_of, pos_of, label_of, lse2, row_scale, x, w, part, part_sum, label_logit, delta, acc, bytes;
-};
+inline int64_t Ceil(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 struct Problem {
   const uint16_t *x, *w;
@@ -763,32 +859,61 @@ struct Problem {
   bool bf16;
   int32_t ignore;
   float smooth;
+  int type() const { return bf16 ? kBfloat16 : kFloat16; }
 };
 
 inline bool Aligned16(const void *p, int64_t ld, int64_t elem) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * elem % 16 == 0;
 }
 
+/*!
+ * \brief one CTA or a pair per tile.  A pair reads each operand half as often and runs a long grid of tiles
+ *  about 6 % faster (8192 x 131072 x 4096: 6.06 against 6.50 ms), but its tiles are twice as high: where that
+ *  costs more rounds of tiles over the SMs than it saves (257 rows: two pairs high for three CTAs'
+ *  worth of rows), single CTAs are used.
+ */
+inline int CtasFor(int64_t rows, int64_t other_tiles, int sms) {
+  const int64_t single = Ceil(Ceil(rows, 128) * other_tiles, sms), pair = Ceil(Ceil(rows, 256) * other_tiles, sms / 2);
+  return single * 107 < pair * 100 ? 1 : 2;
+}
+
+/*! \brief how a call is cut, and where its scratch matrices lie (offsets in bytes) */
+struct Plan {
+  bool pack, copy_w;
+  int64_t pad_rows, ld_x, ld_w, piece, ld_acc, tile_n, tiles;
+  int slices, ctas, ctas_gx;
+  int64_t words, row_of, pos_of, label_of, lse2, row_scale, x, w, part, part_sum, label_logit, delta, acc, bytes;
+};
+
 /*! \brief layout of a call; sms = multiprocessors of the device */
 inline Plan MakePlan(int64_t n, int64_t v, int64_t h, bool gradient, bool want_gx, bool smooth, bool pack, bool copy_w,
-                     int sms, int ctas) {
+                     int sms) {
   Plan p = {};
   p.pack = pack;
   p.copy_w = copy_w;
-  p.ctas = ctas;
   p.pad_rows = RoundUp(n, kPadRows);
   p.ld_x = RoundUp(h, 8);
   p.ld_w = RoundUp(h, 8);
   p.ld_acc = RoundUp(h, kTileN);
-  p.tiles = (v + kTileN - 1) / kTileN;
-  p.piece = p.tiles * kTileN;
+  p.tile_n = kTileN;
+  p.piece = RoundUp(v, kTileN);
   if (gradient) p.piece = std::min(p.piece, std::max<int64_t>(kTileN, kDeltaBytes / (2 * p.pad_rows) / kTileN * kTileN));
   if (copy_w) p.piece = std::min(p.piece, std::max<int64_t>(kTileN, kCopyBytes / (2 * p.ld_w) / kTileN * kTileN));
+  p.ctas = CtasFor(n, p.piece / kTileN, sms);
+  if (!gradient && n <= 128 && p.piece >= v) {
+    // a call bound by reading W once: as many columns per tile as make whole rounds over the SMs (32000 classes: 143
+    // tiles of 224 columns instead of 125 of 256)
+    p.ctas = 1;
+    const int64_t rounds = Ceil(Ceil(v, kTileN), sms);
+    p.tile_n = std::min<int64_t>(kTileN, RoundUp(Ceil(v, rounds * sms), 16));
+  }
+  p.tiles = Ceil(v, p.tile_n);
   p.slices = 1;
+  p.ctas_gx = CtasFor(n, p.ld_acc / kTileN, sms);
   if (gradient && want_gx) {
     // enough parts of the contraction to give every SM a tile, each at least eight steps long
-    const int64_t tiles = RoundUp(p.pad_rows, 128 * ctas) / (128 * ctas) * (p.ld_acc / kTileN);
-    const int64_t want = (sms / ctas + tiles - 1) / tiles, most = p.piece / kStepK / 8;
+    const int64_t tiles = Ceil(n, 128 * p.ctas_gx) * (p.ld_acc / kTileN);
+    const int64_t want = Ceil(sms / p.ctas_gx, tiles), most = p.piece / kStepK / 8;
     p.slices = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(16, std::min(want, most))));
   }
   int64_t at = 0;
@@ -809,36 +934,33 @@ inline Plan MakePlan(int64_t n, int64_t v, int64_t h, bool gradient, bool want_g
     p.delta = take(p.pad_rows * p.piece * 2);
     p.acc = take(want_gx ? p.slices * p.pad_rows * p.ld_acc * 4 : 0);
   } else {
-    p.part = take(p.tiles * p.pad_rows * 8);
-    p.part_sum = take(smooth ? p.tiles * p.pad_rows * 4 : 0);
+    p.part = take(2 * p.tiles * p.pad_rows * 8);
+    p.part_sum = take(smooth ? 2 * p.tiles * p.pad_rows * 4 : 0);
     p.label_logit = take(p.pad_rows * 4);
   }
   p.bytes = at;
   return p;
 }
 
-#ifndef MSHADOW_B200_VLOSS_CTAS
-#define MSHADOW_B200_VLOSS_CTAS 1
-#endif
 inline Plan PlanForward(const Problem &q, int sms) {
   const bool pack = q.n > 256 || !Aligned16(q.x, q.ld_x, 2);
-  return MakePlan(q.n, q.v, q.h, false, false, q.smooth != 0.0f, pack, !Aligned16(q.w, q.ld_w, 2), sms, MSHADOW_B200_VLOSS_CTAS);
+  return MakePlan(q.n, q.v, q.h, false, false, q.smooth != 0.0f, pack, !Aligned16(q.w, q.ld_w, 2), sms);
 }
 inline Plan PlanBackward(const Problem &q, bool want_gx, int sms) {
-  return MakePlan(q.n, q.v, q.h, true, want_gx, q.smooth != 0.0f, true, !Aligned16(q.w, q.ld_w, 2), sms, MSHADOW_B200_VLOSS_CTAS);
+  return MakePlan(q.n, q.v, q.h, true, want_gx, q.smooth != 0.0f, true, !Aligned16(q.w, q.ld_w, 2), sms);
 }
 /*! \brief scratch that suffices for every call of these sizes, whatever its layouts and options */
 inline size_t WorkspaceNeed(int64_t n, int64_t v, int64_t h, bool gradient, int sms) {
   int64_t most = 0;
   for (int copy_w = 0; copy_w < 2; ++copy_w) {
-    most = std::max(most, MakePlan(n, v, h, gradient, true, true, true, copy_w != 0, sms, MSHADOW_B200_VLOSS_CTAS).bytes);
+    most = std::max(most, MakePlan(n, v, h, gradient, true, true, true, copy_w != 0, sms).bytes);
   }
   return static_cast<size_t>(most);
 }
 
 template <int kMode, int kCtas>
-inline void LaunchGemm(const CUtensorMap &ma, const CUtensorMap &mb, const GemmArgs &args, int64_t units, int sms,
-                       cudaStream_t stream) {
+inline void LaunchGemm(const CUtensorMap &ma, const CUtensorMap &mb, const CUtensorMap &mo, const GemmArgs &args, int64_t units,
+                       int sms, cudaStream_t stream) {
   auto kernel = VocabGemmKernel<kMode, kCtas>;
   const size_t smem = StageShape<kCtas>::kSmem;
   MSHADOW_CUDA_CALL(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
@@ -856,15 +978,15 @@ inline void LaunchGemm(const CUtensorMap &ma, const CUtensorMap &mb, const GemmA
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = kCtas > 1 ? 2 : 1;
-  MSHADOW_CUDA_CALL(cudaLaunchKernelEx(&cfg, kernel, ma, mb, args));
+  MSHADOW_CUDA_CALL(cudaLaunchKernelEx(&cfg, kernel, ma, mb, mo, args));
   MSHADOW_CUDA_POST_KERNEL_CHECK(VocabGemmKernel);
 }
 
 template <int kMode>
-inline void Gemm(const CUtensorMap &ma, const CUtensorMap &mb, const GemmArgs &args, int64_t units, int ctas, int sms,
-                 cudaStream_t stream) {
-  if (ctas == 2) LaunchGemm<kMode, 2>(ma, mb, args, units, sms, stream);
-  else LaunchGemm<kMode, 1>(ma, mb, args, units, sms, stream);
+inline void Gemm(const CUtensorMap &ma, const CUtensorMap &mb, const CUtensorMap &mo, const GemmArgs &args, int64_t units,
+                 int ctas, int sms, cudaStream_t stream) {
+  if (ctas == 2) LaunchGemm<kMode, 2>(ma, mb, mo, args, units, sms, stream);
+  else LaunchGemm<kMode, 1>(ma, mb, mo, args, units, sms, stream);
 }
 
 /*! \brief row tiles walked before the next column tile: together their operand rows stay in the L2 */
@@ -875,7 +997,7 @@ inline CUtensorMap WeightMap(const Problem &q, const Plan &p, char *ws, int64_t 
                              cudaStream_t stream, bool copy_now, int32_t *row0) {
   if (!p.copy_w) {
     *row0 = static_cast<int32_t>(p0);
-    return tc5::MatrixMap(q.w, q.bf16, q.v, q.h, q.ld_w, box_rows);
+    return tc5::MatrixMap(q.w, q.type(), q.v, q.h, q.ld_w, box_rows);
   }
   uint16_t *w = reinterpret_cast<uint16_t *>(ws + p.w);
   if (copy_now) {
@@ -884,7 +1006,7 @@ inline CUtensorMap WeightMap(const Problem &q, const Plan &p, char *ws, int64_t 
     MSHADOW_CUDA_POST_KERNEL_CHECK(AlignRowsKernel);
   }
   *row0 = 0;
-  return tc5::MatrixMap(w, q.bf16, rows, q.h, p.ld_w, box_rows);
+  return tc5::MatrixMap(w, q.type(), rows, q.h, p.ld_w, box_rows);
 }
 
 inline void PackLaunch(const Problem &q, const Plan &p, char *ws, PackArgs a, cudaStream_t stream) {
@@ -910,11 +1032,12 @@ inline void ForwardLaunch(float *loss, float *lse, const Problem &q, const Plan 
   GemmArgs a = {};
   a.live = p.pack ? reinterpret_cast<const int32_t *>(ws + p.words) : nullptr;
   a.tokens = static_cast<int32_t>(q.n);
-  a.k_blocks = gpu_rt::CeilDiv(q.h, kStepK);
+  a.k_blocks = static_cast<int32_t>(Ceil(q.h, kStepK));
   a.slices = 1;
-  const int64_t m_tiles = (q.n + 128 * p.ctas - 1) / (128 * p.ctas);
+  const int64_t m_tiles = Ceil(q.n, 128 * p.ctas);
   a.group = GroupOf(m_tiles);
-  a.instr = tc5::InstrDesc(q.bf16, false, false, 128 * p.ctas, kTileN);
+  a.instr = tc5::InstrDesc(q.bf16, false, false, 128 * p.ctas, static_cast<int>(p.tile_n));
+  a.tile_n = static_cast<int32_t>(p.tile_n);
   a.pad_rows = p.pad_rows;
   a.label = p.pack ? reinterpret_cast<const int32_t *>(ws + p.label_of) : q.label;
   a.part = reinterpret_cast<float2 *>(ws + p.part);
@@ -922,23 +1045,23 @@ inline void ForwardLaunch(float *loss, float *lse, const Problem &q, const Plan 
   a.label_logit = reinterpret_cast<float *>(ws + p.label_logit);
   a.bf16 = q.bf16;
   a.status = gpu_rt::StatusWord();
-  const CUtensorMap ma = p.pack ? tc5::MatrixMap(ws + p.x, q.bf16, p.pad_rows, q.h, p.ld_x, 128)
-                                : tc5::MatrixMap(q.x, q.bf16, q.n, q.h, q.ld_x, 128);
+  const CUtensorMap ma = p.pack ? tc5::MatrixMap(ws + p.x, q.type(), p.pad_rows, q.h, p.ld_x, 128)
+                                : tc5::MatrixMap(q.x, q.type(), q.n, q.h, q.ld_x, 128);
   for (int64_t p0 = 0; p0 < q.v; p0 += p.piece) {
     const int64_t cols = std::min(p.piece, q.v - p0);
-    const CUtensorMap mb = WeightMap(q, p, ws, p0, cols, kTileN / p.ctas, stream, true, &a.b_row0);
+    const CUtensorMap mb = WeightMap(q, p, ws, p0, cols, static_cast<int>(p.tile_n) / p.ctas, stream, true, &a.b_row0);
     a.cols = static_cast<int32_t>(cols);
     a.col0 = static_cast<int32_t>(p0);
-    a.tile0 = static_cast<int32_t>(p0 / kTileN);
-    a.n_tiles = gpu_rt::CeilDiv(cols, kTileN);
-    Gemm<kStat>(ma, mb, a, m_tiles * a.n_tiles, p.ctas, sms, stream);
+    a.tile0 = static_cast<int32_t>(p0 / p.tile_n);
+    a.n_tiles = static_cast<int32_t>(Ceil(cols, p.tile_n));
+    Gemm<kStat>(ma, mb, mb, a, m_tiles * a.n_tiles, p.ctas, sms, stream);
   }
   JoinArgs j = {};
-  j.live = a.live, j.tokens = a.tokens, j.tiles = static_cast<int32_t>(p.tiles), j.v = static_cast<int32_t>(q.v);
+  j.live = a.live, j.tokens = a.tokens, j.parts = static_cast<int32_t>(2 * p.tiles), j.v = static_cast<int32_t>(q.v);
   j.pad_rows = p.pad_rows, j.part = a.part, j.part_sum = a.part_sum, j.label_logit = a.label_logit;
   j.label = a.label, j.row_of = p.pack ? reinterpret_cast<const int32_t *>(ws + p.row_of) : nullptr;
   j.ignore = q.ignore, j.smooth = q.smooth, j.loss = loss, j.lse = lse;
-  gpu_rt::LaunchAfterDrain(JoinTilesKernel<0>, dim3(gpu_rt::CeilDiv(q.n, 32)), dim3(256), 0, stream, j);
+  gpu_rt::LaunchAfterDrain(JoinTilesKernel<0>, dim3(gpu_rt::CeilDiv(q.n, 32)), dim3(512), 0, stream, j);
   MSHADOW_CUDA_POST_KERNEL_CHECK(JoinTilesKernel);
 }
 
@@ -956,14 +1079,15 @@ struct GradOut {
 inline void BackwardLaunch(const GradOut &g, const Problem &q, const Plan &p, char *ws, int sms, cudaStream_t stream) {
   PackArgs k = {};
   k.pos_of = reinterpret_cast<int32_t *>(ws + p.pos_of);
-  k.lse = g.lse, k.gloss = g.gloss, k.scale = g.scale;
+  k.lse = g.lse, k.gloss = g.gloss, k.scale = g.scale, k.q_label = static_cast<float>(1.0 - q.smooth);
   k.lse2 = reinterpret_cast<float *>(ws + p.lse2);
   k.row_scale = reinterpret_cast<float *>(ws + p.row_scale);
   PackLaunch(q, p, ws, k, stream);
 
-  const int rows = 128 * p.ctas;
-  const int64_t m_tiles = (q.n + rows - 1) / rows;
-  const int h_tiles = static_cast<int>(p.ld_acc / kTileN);
+  const int32_t h_tiles = static_cast<int32_t>(p.ld_acc / kTileN);
+  const int type = q.type();
+  float *acc = reinterpret_cast<float *>(ws + p.acc);
+  char *delta = ws + p.delta;
   GemmArgs a = {};
   a.live = reinterpret_cast<const int32_t *>(ws + p.words);
   a.inv_scale = reinterpret_cast<const float *>(ws + p.words) + 1;
@@ -974,44 +1098,44 @@ inline void BackwardLaunch(const GradOut &g, const Problem &q, const Plan &p, ch
   a.q_label = static_cast<float>(1.0 - q.smooth);
   a.q_other = q.smooth != 0.0f ? static_cast<float>(static_cast<double>(q.smooth) / (q.v - 1)) : 0.0f;
   a.bf16 = q.bf16;
-  a.delta = reinterpret_cast<uint16_t *>(ws + p.delta);
-  a.ld_delta = p.piece;
-  a.acc = reinterpret_cast<float *>(ws + p.acc);
-  a.ld_acc = p.ld_acc;
-  a.acc_slice = p.pad_rows * p.ld_acc;
   a.status = gpu_rt::StatusWord();
-  const CUtensorMap x_along = tc5::MatrixMap(ws + p.x, q.bf16, p.pad_rows, q.h, p.ld_x, 128);
-  const CUtensorMap x_across = tc5::MatrixMap(ws + p.x, q.bf16, p.pad_rows, q.h, p.ld_x, 64);
-  const CUtensorMap d_along = tc5::MatrixMap(a.delta, q.bf16, p.pad_rows, p.piece, p.piece, 128);
-  const CUtensorMap d_across = tc5::MatrixMap(a.delta, q.bf16, p.pad_rows, p.piece, p.piece, 64);
+  const CUtensorMap x_along = tc5::MatrixMap(ws + p.x, type, p.pad_rows, q.h, p.ld_x, 128);
+  const CUtensorMap x_across = tc5::MatrixMap(ws + p.x, type, p.pad_rows, q.h, p.ld_x, 64);
+  const CUtensorMap d_along = tc5::MatrixMap(delta, type, p.pad_rows, p.piece, p.piece, 128);
+  const CUtensorMap d_across = tc5::MatrixMap(delta, type, p.pad_rows, p.piece, p.piece, 64);
   for (int64_t p0 = 0; p0 < q.v; p0 += p.piece) {
     const int64_t cols = std::min(p.piece, q.v - p0);
+    const int64_t m_tiles = Ceil(q.n, 128 * p.ctas);
     a.cols = static_cast<int32_t>(cols);
     a.col0 = static_cast<int32_t>(p0);
     a.slices = 1;
-    a.n_tiles = gpu_rt::CeilDiv(cols, kTileN);
-    a.k_blocks = gpu_rt::CeilDiv(q.h, kStepK);
+    a.n_tiles = static_cast<int32_t>(Ceil(cols, kTileN));
+    a.k_blocks = static_cast<int32_t>(Ceil(q.h, kStepK));
     a.group = GroupOf(m_tiles);
-    a.instr = tc5::InstrDesc(q.bf16, false, false, rows, kTileN);
+    a.instr = tc5::InstrDesc(q.bf16, false, false, 128 * p.ctas, kTileN);
     const CUtensorMap w_along = WeightMap(q, p, ws, p0, cols, kTileN / p.ctas, stream, true, &a.b_row0);
-    Gemm<kDelta>(x_along, w_along, a, m_tiles * a.n_tiles, p.ctas, sms, stream);
+    Gemm<kDelta>(x_along, w_along, d_along, a, m_tiles * a.n_tiles, p.ctas, sms, stream);
     if (g.gx != nullptr) {
       const CUtensorMap w_across = WeightMap(q, p, ws, p0, cols, 64, stream, false, &a.b_row0);
+      const CUtensorMap out = tc5::MatrixMap(acc, kFloat32, p.slices * p.pad_rows, p.ld_acc, p.ld_acc, 128);
+      const int64_t x_tiles = Ceil(q.n, 128 * p.ctas_gx);
       a.n_tiles = h_tiles;
-      a.k_blocks = gpu_rt::CeilDiv(cols, kStepK);
+      a.k_blocks = static_cast<int32_t>(Ceil(cols, kStepK));
       a.slices = std::min(p.slices, a.k_blocks);  // the last piece may be shorter than the parts are many
       a.accumulate = p0 > 0;
-      a.instr = tc5::InstrDesc(q.bf16, false, true, rows, kTileN);
-      Gemm<kDataGrad>(d_along, w_across, a, m_tiles * a.n_tiles * a.slices, p.ctas, sms, stream);
+      a.group = GroupOf(x_tiles);
+      a.instr = tc5::InstrDesc(q.bf16, false, true, 128 * p.ctas_gx, kTileN);
+      Gemm<kDataGrad>(d_along, w_across, out, a, x_tiles * a.n_tiles * a.slices, p.ctas_gx, sms, stream);
     }
     if (g.gw != nullptr) {
       const int64_t elem = g.gw_type == kFloat32 ? 4 : 2;
-      a.m_tiles = gpu_rt::CeilDiv(cols, rows);
+      const int ctas = CtasFor(cols, h_tiles, sms);
+      a.m_tiles = static_cast<int32_t>(Ceil(cols, 128 * ctas));
       a.n_tiles = h_tiles;
       a.slices = 1;
       a.b_row0 = 0;
       a.group = GroupOf(a.m_tiles);
-      a.instr = tc5::InstrDesc(q.bf16, true, true, rows, kTileN);
+      a.instr = tc5::InstrDesc(q.bf16, true, true, 128 * ctas, kTileN);
       a.out = static_cast<char *>(g.gw) + p0 * g.ld_gw * elem;
       a.ld_out = g.ld_gw;
       a.out_rows = static_cast<int32_t>(cols);
@@ -1019,12 +1143,16 @@ inline void BackwardLaunch(const GradOut &g, const Problem &q, const Plan &p, ch
       a.out_type = g.gw_type;
       a.out_add = g.gw_add;
       a.out_vec = Aligned16(a.out, g.ld_gw, elem);
-      Gemm<kWeightGrad>(d_across, x_across, a, static_cast<int64_t>(a.m_tiles) * a.n_tiles, p.ctas, sms, stream);
+      // (a tiled copy leaves out columns past the matrix in units of 16 bytes: rows that do not end on such a
+      // boundary would lose up to 14 bytes behind them to zeros)
+      a.out_tiled = a.out_vec && !a.out_add && q.h * elem % 16 == 0;
+      const CUtensorMap out = a.out_tiled ? tc5::MatrixMap(a.out, g.gw_type, cols, q.h, g.ld_gw, 128) : x_across;
+      Gemm<kWeightGrad>(d_across, x_across, out, a, static_cast<int64_t>(a.m_tiles) * a.n_tiles, ctas, sms, stream);
     }
   }
   if (g.gx != nullptr) {
     FinishArgs f = {};
-    f.acc = a.acc, f.ld_acc = p.ld_acc, f.acc_slice = a.acc_slice, f.slices = p.slices;
+    f.acc = acc, f.ld_acc = p.ld_acc, f.acc_slice = p.pad_rows * p.ld_acc, f.slices = p.slices;
     f.pos_of = k.pos_of, f.inv_scale = a.inv_scale;
     f.out = g.gx, f.ld_out = g.ld_gx, f.n = static_cast<int32_t>(q.n), f.h = static_cast<int32_t>(q.h);
     f.bf16 = q.bf16, f.vec = Aligned16(g.gx, g.ld_gx, 2);
