@@ -19,7 +19,7 @@ STATUS_NAMES = {0: "MSB_OK", 1: "MSB_ERR_ARGUMENT", 2: "MSB_ERR_SHAPE", 3: "MSB_
 
 SAVETO, PLUSTO, MINUSTO, MULTO, DIVTO = range(5)
 RED_SUM, RED_MAX, RED_MIN = range(3)
-FLOAT32, FLOAT16, BFLOAT16 = 0, 2, 12
+FLOAT32, FLOAT16, INT32, BFLOAT16 = 0, 2, 4, 12
 H2D, D2H, D2D = 1, 2, 3
 
 
@@ -106,48 +106,46 @@ def _ptr(t):
     return vp(t.data_ptr() if hasattr(t, "data_ptr") else int(t))
 
 
-_DTYPE_FLAGS = {"float32": FLOAT32, "float16": FLOAT16, "bfloat16": BFLOAT16}
+_TAGS = {"float32": FLOAT32, "float16": FLOAT16, "bfloat16": BFLOAT16, "int32": INT32}
+_tag_of = {}  # dtype object -> type tag; a look-up per tensor is all the checks below cost
 
 
-def _dtype(d):
-    """Type tag of a torch / numpy dtype (or of its name)."""
-    name = str(d).rsplit(".", 1)[-1]
-    if name not in _DTYPE_FLAGS:
-        raise MsbError(1, "element type %s is not one of %s" % (d, sorted(_DTYPE_FLAGS)))
-    return _DTYPE_FLAGS[name]
+def _tag(dtype):
+    """mshadow's type tag of a torch / numpy dtype; -1 for one the entries below do not take."""
+    tag = _tag_of.get(dtype)
+    if tag is None:
+        tag = _tag_of[dtype] = _TAGS.get(str(dtype).rsplit(".", 1)[-1], -1)
+    return tag
 
 
-def _same(what, expected, *tensors):
-    for t in tensors:
-        if t is not None and tuple(t.shape) != tuple(expected):
-            raise MsbError(2, "%s: shape %s where %s is expected" % (what, tuple(t.shape), tuple(expected)))
+def _matrix(what, t, rows, cols, tag):
+    """(address, leading dimension) of a rows x cols matrix with dense rows that do not overlap."""
+    if t.shape != (rows, cols):
+        raise MsbError(2, "%s: shape %s where %s is expected" % (what, tuple(t.shape), (rows, cols)))
+    if _tag(t.dtype) != tag:
+        raise MsbError(1, "%s: element type %s does not fit" % (what, t.dtype))
+    ld, inner = t.stride()
+    if rows <= 1:
+        ld = max(ld, cols)
+    if (inner != 1 and cols > 1) or ld < cols:
+        raise MsbError(3, "%s: rows must be dense and must not overlap" % what)
+    return t.data_ptr(), ld
 
 
-def _kind(what, dtype, *tensors):
-    for t in tensors:
-        if t is not None and str(t.dtype) != str(dtype):
-            raise MsbError(1, "%s: %s where %s is expected" % (what, t.dtype, dtype))
-
-
-def _dense(what, *tensors):
-    for t in tensors:
-        if t is not None and t.shape[0] > 1 and t.stride(0) != 1:
-            raise MsbError(3, "%s: vectors must be dense" % what)
-
-
-def _row_ld(what, t):
-    """Leading dimension of a matrix whose rows are dense and do not overlap."""
-    if t.shape[1] > 1 and t.stride(1) != 1:
-        raise MsbError(3, "%s: the last axis must be dense" % what)
-    ld = t.stride(0) if t.shape[0] > 1 else max(t.shape[1], t.stride(0))
-    if ld < t.shape[1]:
-        raise MsbError(3, "%s: rows overlap" % what)
-    return ld
+def _vector(what, t, n, tag):
+    """Address of a dense vector of n elements."""
+    if t.shape != (n,):
+        raise MsbError(2, "%s: shape %s where %s is expected" % (what, tuple(t.shape), (n,)))
+    if _tag(t.dtype) != tag:
+        raise MsbError(1, "%s: element type %s does not fit" % (what, t.dtype))
+    if n > 1 and t.stride(0) != 1:
+        raise MsbError(3, "%s: vectors must be dense" % what)
+    return t.data_ptr()
 
 
 def _workspace(t):
-    """(address, bytes) of an optional one-dimensional workspace tensor."""
-    return (None, 0) if t is None else (vp(t.data_ptr()), t.numel() * t.element_size())
+    """(address, bytes) of an optional workspace tensor."""
+    return (None, 0) if t is None else (t.data_ptr(), t.numel() * t.element_size())
 
 
 def _ld(t):
@@ -455,14 +453,11 @@ class Library:
     # ---- the vocabulary table's two ends ---------------------------------------------------
     def embed_take(self, dst, table, index, scale=1.0, stream=None):
         """dst[i] = scale * table[index[i]]; an index outside the table gives a row of zeros."""
-        n, width = dst.shape
-        _same("embed_take", (n,), index)
-        _same("embed_take", (table.shape[0], width), table)
-        _kind("embed_take", dst.dtype, table)
-        _kind("embed_take", "torch.int32", index)
-        _dense("embed_take", index)
-        self.call("msb_embed_take", _ptr(dst), _ptr(table), _ptr(index), n, table.shape[0], width,
-                  _row_ld("embed_take", dst), _row_ld("embed_take", table), _dtype(dst.dtype), scale, stream)
+        (n, width), rows, tag = dst.shape, table.shape[0], _tag(dst.dtype)
+        out, ld_out = _matrix("embed_take", dst, n, width, tag)
+        tab, ld_tab = _matrix("embed_take", table, rows, width, tag)
+        self.call("msb_embed_take", out, tab, _vector("embed_take", index, n, INT32), n, rows, width, ld_out, ld_tab, tag,
+                  scale, stream)
         return dst
 
     def embed_take_grad_workspace(self, n, rows, width, dtype=None):
@@ -473,16 +468,12 @@ class Library:
 
     def embed_take_grad(self, dst, src, index, scale=1.0, saver=SAVETO, workspace=None, stream=None):
         """dst[r] = (saver PLUSTO: +=) scale * sum of the rows of src whose index is r."""
-        n, width = src.shape
-        _same("embed_take_grad", (n,), index)
-        _same("embed_take_grad", (dst.shape[0], width), dst)
-        _kind("embed_take_grad", dst.dtype, src)
-        _kind("embed_take_grad", "torch.int32", index)
-        _dense("embed_take_grad", index)
+        (n, width), rows, tag = src.shape, dst.shape[0], _tag(dst.dtype)
+        out, ld_out = _matrix("embed_take_grad", dst, rows, width, tag)
+        g, ld_g = _matrix("embed_take_grad", src, n, width, tag)
         ws, size = _workspace(workspace)
-        self.call("msb_embed_take_grad", _ptr(dst), _ptr(src), _ptr(index), n, dst.shape[0], width,
-                  _row_ld("embed_take_grad", dst), _row_ld("embed_take_grad", src), _dtype(dst.dtype), scale, saver, ws, size,
-                  stream)
+        self.call("msb_embed_take_grad", out, g, _vector("embed_take_grad", index, n, INT32), n, rows, width, ld_out, ld_g, tag,
+                  scale, saver, ws, size, stream)
         return dst
 
     def linear_softmax_loss_workspace(self, n, v, h, dtype=None, gradient=False):
@@ -496,38 +487,30 @@ class Library:
 
     def linear_softmax_loss(self, loss, lse, data, weight, label, ignore_label=-1, smooth=0.0, workspace=None, stream=None):
         """Cross entropy of softmax(data . weight^T) and the log of its normaliser, per token."""
-        (n, h), v = data.shape, weight.shape[0]
-        what = "linear_softmax_loss"
-        _same(what, (n,), loss, lse, label)
-        _same(what, (v, h), weight)
-        _kind(what, data.dtype, weight)
-        _kind(what, "torch.int32", label)
-        _kind(what, "torch.float32", loss, lse)
-        _dense(what, loss, lse, label)
+        what, (n, h), v, tag = "linear_softmax_loss", data.shape, weight.shape[0], _tag(data.dtype)
+        x, ld_x = _matrix(what, data, n, h, tag)
+        w, ld_w = _matrix(what, weight, v, h, tag)
         ws, size = _workspace(workspace)
-        self.call("msb_linear_softmax_loss", _ptr(loss), _ptr(lse), _ptr(data), _ptr(weight), _ptr(label), n, v, h,
-                  _row_ld(what, data), _row_ld(what, weight), _dtype(data.dtype), ignore_label, smooth, ws, size, stream)
+        self.call("msb_linear_softmax_loss", _vector(what, loss, n, FLOAT32), _vector(what, lse, n, FLOAT32), x, w,
+                  _vector(what, label, n, INT32), n, v, h, ld_x, ld_w, tag, ignore_label, smooth, ws, size, stream)
         return loss, lse
 
     def linear_softmax_loss_grad(self, gdata, gweight, data, weight, label, lse, gloss=None, scale=1.0, ignore_label=-1,
                                  smooth=0.0, saver=SAVETO, workspace=None, stream=None):
         """Gradients of sum(scale * gloss * loss); gdata or gweight may be None.  saver PLUSTO adds to gweight."""
-        (n, h), v = data.shape, weight.shape[0]
-        what = "linear_softmax_loss_grad"
-        _same(what, (n,), lse, label, gloss)
-        _same(what, (v, h), weight, gweight)
-        _same(what, (n, h), gdata)
-        _kind(what, data.dtype, weight, gdata)
-        _kind(what, "torch.int32", label)
-        _kind(what, "torch.float32", lse, gloss)
-        _dense(what, lse, label, gloss)
+        what, (n, h), v, tag = "linear_softmax_loss_grad", data.shape, weight.shape[0], _tag(data.dtype)
+        x, ld_x = _matrix(what, data, n, h, tag)
+        w, ld_w = _matrix(what, weight, v, h, tag)
+        gx, ld_gx, gw, ld_gw, gtag = None, h, None, h, tag
+        if gdata is not None:
+            gx, ld_gx = _matrix(what, gdata, n, h, tag)
+        if gweight is not None:
+            gtag = FLOAT32 if _tag(gweight.dtype) == FLOAT32 else tag
+            gw, ld_gw = _matrix(what, gweight, v, h, gtag)
         ws, size = _workspace(workspace)
-        self.call("msb_linear_softmax_loss_grad", None if gdata is None else _ptr(gdata),
-                  None if gweight is None else _ptr(gweight), _ptr(data), _ptr(weight), _ptr(label), _ptr(lse),
-                  None if gloss is None else _ptr(gloss), scale, n, v, h, h if gdata is None else _row_ld(what, gdata),
-                  h if gweight is None else _row_ld(what, gweight), _row_ld(what, data), _row_ld(what, weight),
-                  _dtype(data.dtype), _dtype(data.dtype if gweight is None else gweight.dtype), saver, ignore_label, smooth,
-                  ws, size, stream)
+        self.call("msb_linear_softmax_loss_grad", gx, gw, x, w, _vector(what, label, n, INT32),
+                  _vector(what, lse, n, FLOAT32), None if gloss is None else _vector(what, gloss, n, FLOAT32), scale, n, v, h,
+                  ld_gx, ld_gw, ld_x, ld_w, tag, gtag, saver, ignore_label, smooth, ws, size, stream)
         return gdata, gweight
 
 

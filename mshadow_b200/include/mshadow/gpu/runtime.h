@@ -322,6 +322,20 @@ inline int ResidentPerSM(Kernel kernel, int threads, size_t smem = 0) {
 }
 #endif
 
+#ifdef __CUDACC__
+/*! \brief lets `kKernel` use `bytes` (always the same) of dynamic shared memory; asks the driver once per device */
+template <auto kKernel>
+inline void AllowSharedMemory(size_t bytes) {
+  static std::atomic<unsigned long long> done[4] = {};
+  int dev = 0;
+  MSHADOW_CUDA_CALL(cudaGetDevice(&dev));
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (dev < 256 && (done[dev >> 6].load(std::memory_order_acquire) & bit)) return;
+  MSHADOW_CUDA_CALL(cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)));
+  if (dev < 256) done[dev >> 6].fetch_or(bit, std::memory_order_release);
+}
+#endif
+
 /*! \brief exact division of an index by a divisor fixed per launch, without a divide instruction */
 typedef expr::FastDiv FastDiv;
 
