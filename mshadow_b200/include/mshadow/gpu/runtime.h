@@ -323,16 +323,22 @@ inline int ResidentPerSM(Kernel kernel, int threads, size_t smem = 0) {
 #endif
 
 #ifdef __CUDACC__
-/*! \brief lets `kKernel` use `bytes` (always the same) of dynamic shared memory; asks the driver once per device */
-template <auto kKernel>
-inline void AllowSharedMemory(size_t bytes) {
-  static std::atomic<unsigned long long> done[4] = {};
+/*!
+ * \brief lets `kernel` use `bytes` (always the same for a kernel) of dynamic shared memory; the driver is asked once
+ *  per (device, kernel).  Kept by the kernel's address: two libraries built from these headers in one
+ *  process share the table, but not the kernels.
+ */
+template <typename Kernel>
+inline void AllowSharedMemory(Kernel kernel, size_t bytes) {
+  static std::mutex mu;
+  static std::map<std::pair<int, const void *>, bool> done;
   int dev = 0;
   MSHADOW_CUDA_CALL(cudaGetDevice(&dev));
-  const unsigned long long bit = 1ull << (dev & 63);
-  if (dev < 256 && (done[dev >> 6].load(std::memory_order_acquire) & bit)) return;
-  MSHADOW_CUDA_CALL(cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)));
-  if (dev < 256) done[dev >> 6].fetch_or(bit, std::memory_order_release);
+  std::lock_guard<std::mutex> lock(mu);
+  bool &set = done[std::make_pair(dev, reinterpret_cast<const void *>(kernel))];
+  if (set) return;
+  MSHADOW_CUDA_CALL(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)));
+  set = true;
 }
 #endif
 

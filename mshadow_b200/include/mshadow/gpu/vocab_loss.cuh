@@ -389,7 +389,7 @@ __device__ __forceinline__ void WeightColumns(const uint32_t (&r)[32], int64_t r
 template <int kMode, int kCtas>
 __global__ void __launch_bounds__(kThreads, 1)
 VocabGemmKernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-                const __grid_constant__ CUtensorMap map_out, const GemmArgs a) {
+                const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_out, const GemmArgs a) {
   typedef StageShape<kCtas> S;
   typedef Layout<kMode> L;
   extern __shared__ uint8_t raw[];
@@ -410,6 +410,7 @@ VocabGemmKernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
     }
     tc5::PrefetchMap(&map_a);
     tc5::PrefetchMap(&map_b);
+    if (kMode != kDataGrad) tc5::PrefetchMap(&map_x);
     if (kMode != kStat) tc5::PrefetchMap(&map_out);
   }
   if (warp == 2) tc5::AllocTensorMemory<kCtas>(&tmem_slot);
@@ -420,7 +421,11 @@ VocabGemmKernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
   const uint32_t tmem = tmem_slot;
   gpu_rt::GridDependencySync();
 
-  const int live = a.live != nullptr ? *a.live : a.tokens;
+  const int live = a.live != nullptr ? a.live[0] : a.tokens;
+  // every token counts: the rows of x were not packed, and are read from where the caller has them
+  const bool in_place = kMode != kDataGrad && a.live != nullptr && a.live[2] != 0;
+  const CUtensorMap *from_a = (kMode == kStat || kMode == kDelta) && in_place ? &map_x : &map_a;
+  const CUtensorMap *from_b = kMode == kWeightGrad && in_place ? &map_x : &map_b;
   const int tile_m = 128 * kCtas;
   const int tile_n = kMode == kStat ? a.tile_n : kTileN;
   const int rows_n = tile_n / kCtas;  // rows of B that this CTA loads
@@ -455,16 +460,16 @@ VocabGemmKernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
           const int k0 = kb * kStepK;
           if (L::kAAcross) {
 #pragma unroll
-            for (int j = 0; j < 2; ++j) tc5::LoadBox<kCtas>(sa + j * tc5::kBoxBytes, &map_a, m0 + 64 * j, k0, bar);
+            for (int j = 0; j < 2; ++j) tc5::LoadBox<kCtas>(sa + j * tc5::kBoxBytes, from_a, m0 + 64 * j, k0, bar);
           } else {
-            tc5::LoadBox<kCtas>(sa, &map_a, k0, m0, bar);
+            tc5::LoadBox<kCtas>(sa, from_a, k0, m0, bar);
           }
           if (L::kBAcross) {
 #pragma unroll
             for (int j = 0; j < S::kRowsN / 64; ++j)
-              tc5::LoadBox<kCtas>(sb + j * tc5::kBoxBytes, &map_b, n0 + 64 * j, a.b_row0 + k0, bar);
+              tc5::LoadBox<kCtas>(sb + j * tc5::kBoxBytes, from_b, n0 + 64 * j, a.b_row0 + k0, bar);
           } else {
-            tc5::LoadBox<kCtas>(sb, &map_b, k0, a.b_row0 + n0, bar);
+            tc5::LoadBox<kCtas>(sb, from_b, k0, a.b_row0 + n0, bar);
           }
         }
       }
@@ -610,7 +615,7 @@ struct PackArgs {
   int64_t pad_rows;      // n rounded up to kPadRows
   uint16_t *packed;      // [pad_rows][ld_packed]
   int64_t ld_packed;
-  int32_t *words;        // [0] = live rows, [1] = what takes d' to d (a float)
+  int32_t *words;        // [0] = live rows, [1] = what takes d' to d (a float), [2] = rows of x left where they are
   int32_t *row_of;       // [pad_rows] token of packed row (forward)
   int32_t *pos_of;       // [n] packed row of token, or -1 (backward)
   int32_t *label_of;     // [pad_rows] label of packed row
@@ -620,6 +625,7 @@ struct PackArgs {
   float scale, q_label;
   float *lse2, *row_scale;  // [pad_rows], backward
   int vec;               // 16-byte copies possible
+  int tiled;             // the tiled copies can read x itself: nothing is packed if all its rows count
   int rows_per_cta;
 };
 
@@ -631,7 +637,8 @@ __device__ __forceinline__ bool IsLive(int32_t label, int32_t ignore, int32_t v)
  * \brief packs the live rows of x and what belongs to them, in token order.  A CTA takes
  *  rows_per_cta tokens (at most 256); where its first live row goes it finds by counting the labels before it
  *  itself (4 bytes per token from the L2), which spares a scan kernel and its launch.  The rows
- *  from the last live one up to the next multiple of kPadRows become zeros.
+ *  from the last live one up to the next multiple of kPadRows become zeros.  Where all rows are live and the
+ *  products can read x as it is, nothing is copied.
  */
 template <int kUnused>
 __global__ void __launch_bounds__(256) PackRowsKernel(const PackArgs a) {
@@ -699,7 +706,9 @@ __global__ void __launch_bounds__(256) PackRowsKernel(const PackArgs a) {
   if (blockIdx.x == 0 && tid == 0) {
     a.words[0] = total;
     reinterpret_cast<float *>(a.words)[1] = a.scale * a.q_label * down;
+    a.words[2] = a.tiled && total == a.n;
   }
+  if (a.tiled && total == a.n) return;
   __syncthreads();
   for (int t = warp; t < a.rows_per_cta; t += 8) {
     const int from = base + t;
@@ -743,26 +752,28 @@ struct JoinArgs {
 };
 
 /*!
- * \brief joins the maxima and sums of the tile halves row by row: 32 rows per CTA, sixteen threads of a row take
- *  every sixteenth part and are joined pairwise
+ * \brief joins the maxima and sums of the tile halves row by row.  512 threads share kRows rows: a thread takes every
+ *  (512 / kRows)-th part of its row, eight at a time with their loads in flight together, and the threads of a row are
+ *  joined pairwise.  Bound by the latency of a few round trips: few rows per CTA (4) while there are few tokens (834
+ *  parts of 48 rows: 15 us with 32 rows per CTA), 32 rows (256-byte loads) when there are many.
  */
-template <int kUnused>
+template <int kRows>
 __global__ void __launch_bounds__(512) JoinTilesKernel(const JoinArgs a) {
   gpu_rt::GridDependencySync();
-  __shared__ float s_ref[16][32], s_sum[16][32], s_total[16][32];
+  constexpr int kShare = 512 / kRows;
+  __shared__ float s_ref[kShare / 2][kRows], s_sum[kShare / 2][kRows], s_total[kShare / 2][kRows];
   const int live = a.live != nullptr ? *a.live : a.tokens;
-  const int r = threadIdx.x & 31, q = threadIdx.x >> 5;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * 32 + r;
-  if (blockIdx.x * 32 >= live) return;
+  const int r = threadIdx.x % kRows, q = threadIdx.x / kRows;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + r;
+  if (static_cast<int64_t>(blockIdx.x) * kRows >= live) return;
   float ref = -INFINITY, sum = 0.0f, total = 0.0f;
   if (row < live) {
-    // eight parts at a time: their loads are in flight together (one after the other, 834 parts of a row took 11 us)
-    for (int t0 = q; t0 < a.parts; t0 += 16 * 8) {
+    for (int t0 = q; t0 < a.parts; t0 += kShare * 8) {
       float2 p[8];
       float top = ref;
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
-        const int t = t0 + 16 * u;
+        const int t = t0 + kShare * u;
         p[u] = t < a.parts ? a.part[t * a.pad_rows + row] : make_float2(-INFINITY, 0.0f);
         if (a.part_sum != nullptr && t < a.parts) total += a.part_sum[t * a.pad_rows + row];
       }
@@ -775,14 +786,15 @@ __global__ void __launch_bounds__(512) JoinTilesKernel(const JoinArgs a) {
       ref = top;
     }
   }
-  for (int half = 8; half > 0; half >>= 1) {
-    s_ref[q][r] = ref, s_sum[q][r] = sum, s_total[q][r] = total;
+#pragma unroll
+  for (int half = kShare / 2; half > 0; half >>= 1) {
+    if (q >= half && q < 2 * half) s_ref[q - half][r] = ref, s_sum[q - half][r] = sum, s_total[q - half][r] = total;
     __syncthreads();
     if (q < half) {
-      const float other = s_ref[q + half][r], top = fmaxf(ref, other), from = top == -INFINITY ? 0.0f : top;
-      sum = sum * Exp2((ref - from) * kLog2e) + s_sum[q + half][r] * Exp2((other - from) * kLog2e);
+      const float other = s_ref[q][r], top = fmaxf(ref, other), from = top == -INFINITY ? 0.0f : top;
+      sum = sum * Exp2((ref - from) * kLog2e) + s_sum[q][r] * Exp2((other - from) * kLog2e);
       ref = top;
-      total += s_total[q + half][r];
+      total += s_total[q][r];
     }
     __syncthreads();
   }
@@ -919,12 +931,21 @@ inline Plan MakePlan(int64_t n, int64_t v, int64_t h, bool gradient, bool want_g
   }
   p.tiles = Ceil(v, p.tile_n);
   p.slices = 1;
-  p.ctas_gx = CtasFor(n, p.ld_acc / kTileN, sms);
+  p.ctas_gx = 2;
   if (gradient && want_gx) {
-    // enough parts of the contraction to give every SM a tile, each at least eight steps long
-    const int64_t tiles = Ceil(n, 128 * p.ctas_gx) * (p.ld_acc / kTileN);
-    const int64_t want = Ceil(sms / p.ctas_gx, tiles), most = p.piece / kStepK / 8;
-    p.slices = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(16, std::min(want, most))));
+    // n x h has few tiles and a contraction as long as the piece: it is cut into parts (at least eight steps
+    // long) that give every SM work.  The cheapest of all cuts by this count: rounds of tiles, 512 cycles a step, some
+    // 4000 to begin and end a tile, and the parts written and read again at about 2400 bytes a cycle.
+    double best = 0.0;
+    for (int ctas = 1; ctas <= 2; ++ctas) {
+      const int64_t tiles = Ceil(n, 128 * ctas) * (p.ld_acc / kTileN);
+      for (int64_t slices = 1; slices <= 16 && (slices == 1 || p.piece / kStepK >= 8 * slices); ++slices) {
+        const double rounds = static_cast<double>(Ceil(tiles * slices, sms / ctas));
+        const double steps = static_cast<double>(Ceil(p.piece / kStepK, slices));
+        const double cost = rounds * (steps * (ctas == 1 ? 560.0 : 512.0) + 4000.0) + slices * n * p.ld_acc * 8 / 2400.0;
+        if (best == 0.0 || cost < best) best = cost, p.slices = static_cast<int>(slices), p.ctas_gx = ctas;
+      }
+    }
   }
   int64_t at = 0;
   auto take = [&at](int64_t bytes) {
@@ -969,11 +990,11 @@ inline size_t WorkspaceNeed(int64_t n, int64_t v, int64_t h, bool gradient, int 
 }
 
 template <int kMode, int kCtas>
-inline void LaunchGemm(const CUtensorMap &ma, const CUtensorMap &mb, const CUtensorMap &mo, const GemmArgs &args, int64_t units,
+inline void LaunchGemm(const CUtensorMap &ma, const CUtensorMap &mb, const CUtensorMap &mx, const CUtensorMap &mo, const GemmArgs &args, int64_t units,
                        int sms, cudaStream_t stream) {
   auto kernel = VocabGemmKernel<kMode, kCtas>;
   const size_t smem = StageShape<kCtas>::kSmem;
-  gpu_rt::AllowSharedMemory<VocabGemmKernel<kMode, kCtas>>(smem);
+  gpu_rt::AllowSharedMemory(kernel, smem);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>(std::max<int64_t>(units, 1), sms / kCtas)) * kCtas);
   cfg.blockDim = dim3(kThreads);
@@ -988,15 +1009,15 @@ inline void LaunchGemm(const CUtensorMap &ma, const CUtensorMap &mb, const CUten
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = kCtas > 1 ? 2 : 1;
-  MSHADOW_CUDA_CALL(cudaLaunchKernelEx(&cfg, kernel, ma, mb, mo, args));
+  MSHADOW_CUDA_CALL(cudaLaunchKernelEx(&cfg, kernel, ma, mb, mx, mo, args));
   MSHADOW_CUDA_POST_KERNEL_CHECK(VocabGemmKernel);
 }
 
 template <int kMode>
-inline void Gemm(const CUtensorMap &ma, const CUtensorMap &mb, const CUtensorMap &mo, const GemmArgs &args, int64_t units,
+inline void Gemm(const CUtensorMap &ma, const CUtensorMap &mb, const CUtensorMap &mx, const CUtensorMap &mo, const GemmArgs &args, int64_t units,
                  int ctas, int sms, cudaStream_t stream) {
-  if (ctas == 2) LaunchGemm<kMode, 2>(ma, mb, mo, args, units, sms, stream);
-  else LaunchGemm<kMode, 1>(ma, mb, mo, args, units, sms, stream);
+  if (ctas == 2) LaunchGemm<kMode, 2>(ma, mb, mx, mo, args, units, sms, stream);
+  else LaunchGemm<kMode, 1>(ma, mb, mx, mo, args, units, sms, stream);
 }
 
 #ifndef MSHADOW_B200_VLOSS_GROUP
@@ -1029,7 +1050,7 @@ inline void PackLaunch(const Problem &q, const Plan &p, char *ws, PackArgs a, cu
   a.packed = reinterpret_cast<uint16_t *>(ws + p.x), a.ld_packed = p.ld_x;
   a.words = reinterpret_cast<int32_t *>(ws + p.words);
   a.label_of = reinterpret_cast<int32_t *>(ws + p.label_of);
-  a.vec = Aligned16(q.x, q.ld_x, 2);
+  a.vec = a.tiled = Aligned16(q.x, q.ld_x, 2);
   a.rows_per_cta = p.pad_rows >= 65536 ? 64 : 16;
   gpu_rt::LaunchAfterDrain(PackRowsKernel<0>, dim3(static_cast<unsigned>(p.pad_rows / a.rows_per_cta)), dim3(256), 0, stream, a);
   MSHADOW_CUDA_POST_KERNEL_CHECK(PackRowsKernel);
@@ -1060,6 +1081,7 @@ inline void ForwardLaunch(float *loss, float *lse, const Problem &q, const Plan 
   a.status = gpu_rt::StatusWord();
   const CUtensorMap ma = p.pack ? tc5::MatrixMap(ws + p.x, q.type(), p.pad_rows, q.h, p.ld_x, 128)
                                 : tc5::MatrixMap(q.x, q.type(), q.n, q.h, q.ld_x, 128);
+  const CUtensorMap mx = Aligned16(q.x, q.ld_x, 2) ? tc5::MatrixMap(q.x, q.type(), q.n, q.h, q.ld_x, 128) : ma;
   for (int64_t p0 = 0; p0 < q.v; p0 += p.piece) {
     const int64_t cols = std::min(p.piece, q.v - p0);
     const CUtensorMap mb = WeightMap(q, p, ws, p0, cols, static_cast<int>(p.tile_n) / p.ctas, stream, true, &a.b_row0);
@@ -1067,14 +1089,18 @@ inline void ForwardLaunch(float *loss, float *lse, const Problem &q, const Plan 
     a.col0 = static_cast<int32_t>(p0);
     a.tile0 = static_cast<int32_t>(p0 / p.tile_n);
     a.n_tiles = static_cast<int32_t>(Ceil(cols, p.tile_n));
-    Gemm<kStat>(ma, mb, mb, a, m_tiles * a.n_tiles, p.ctas, sms, stream);
+    Gemm<kStat>(ma, mb, mx, mb, a, m_tiles * a.n_tiles, p.ctas, sms, stream);
   }
   JoinArgs j = {};
   j.live = a.live, j.tokens = a.tokens, j.parts = static_cast<int32_t>(2 * p.tiles), j.v = static_cast<int32_t>(q.v);
   j.pad_rows = p.pad_rows, j.part = a.part, j.part_sum = a.part_sum, j.label_logit = a.label_logit;
   j.label = a.label, j.row_of = p.pack ? reinterpret_cast<const int32_t *>(ws + p.row_of) : nullptr;
   j.ignore = q.ignore, j.smooth = q.smooth, j.loss = loss, j.lse = lse;
-  gpu_rt::LaunchAfterDrain(JoinTilesKernel<0>, dim3(gpu_rt::CeilDiv(q.n, 32)), dim3(512), 0, stream, j);
+  if (q.n <= 1024) {
+    gpu_rt::LaunchAfterDrain(JoinTilesKernel<4>, dim3(gpu_rt::CeilDiv(q.n, 4)), dim3(512), 0, stream, j);
+  } else {
+    gpu_rt::LaunchAfterDrain(JoinTilesKernel<32>, dim3(gpu_rt::CeilDiv(q.n, 32)), dim3(512), 0, stream, j);
+  }
   MSHADOW_CUDA_POST_KERNEL_CHECK(JoinTilesKernel);
 }
 
@@ -1114,6 +1140,9 @@ inline void BackwardLaunch(const GradOut &g, const Problem &q, const Plan &p, ch
   a.status = gpu_rt::StatusWord();
   const CUtensorMap x_along = tc5::MatrixMap(ws + p.x, type, p.pad_rows, q.h, p.ld_x, 128);
   const CUtensorMap x_across = tc5::MatrixMap(ws + p.x, type, p.pad_rows, q.h, p.ld_x, 64);
+  const bool tiled = Aligned16(q.x, q.ld_x, 2);
+  const CUtensorMap x_along_in_place = tiled ? tc5::MatrixMap(q.x, type, q.n, q.h, q.ld_x, 128) : x_along;
+  const CUtensorMap x_across_in_place = tiled ? tc5::MatrixMap(q.x, type, q.n, q.h, q.ld_x, 64) : x_across;
   const CUtensorMap d_along = tc5::MatrixMap(delta, type, p.pad_rows, p.piece, p.piece, 128);
   const CUtensorMap d_across = tc5::MatrixMap(delta, type, p.pad_rows, p.piece, p.piece, 64);
   for (int64_t p0 = 0; p0 < q.v; p0 += p.piece) {
@@ -1127,7 +1156,7 @@ inline void BackwardLaunch(const GradOut &g, const Problem &q, const Plan &p, ch
     a.group = GroupOf(m_tiles);
     a.instr = tc5::InstrDesc(q.bf16, false, false, 128 * p.ctas, kTileN);
     const CUtensorMap w_along = WeightMap(q, p, ws, p0, cols, kTileN / p.ctas, stream, true, &a.b_row0);
-    Gemm<kDelta>(x_along, w_along, d_along, a, m_tiles * a.n_tiles, p.ctas, sms, stream);
+    Gemm<kDelta>(x_along, w_along, x_along_in_place, d_along, a, m_tiles * a.n_tiles, p.ctas, sms, stream);
     if (g.gx != nullptr) {
       const CUtensorMap w_across = WeightMap(q, p, ws, p0, cols, 64, stream, false, &a.b_row0);
       const CUtensorMap out = tc5::MatrixMap(acc, kFloat32, p.slices * p.pad_rows, p.ld_acc, p.ld_acc, 128);
@@ -1138,7 +1167,7 @@ inline void BackwardLaunch(const GradOut &g, const Problem &q, const Plan &p, ch
       a.accumulate = p0 > 0;
       a.group = GroupOf(x_tiles);
       a.instr = tc5::InstrDesc(q.bf16, false, true, 128 * p.ctas_gx, kTileN);
-      Gemm<kDataGrad>(d_along, w_across, out, a, x_tiles * a.n_tiles * a.slices, p.ctas_gx, sms, stream);
+      Gemm<kDataGrad>(d_along, w_across, d_along, out, a, x_tiles * a.n_tiles * a.slices, p.ctas_gx, sms, stream);
     }
     if (g.gw != nullptr) {
       const int64_t elem = g.gw_type == kFloat32 ? 4 : 2;
@@ -1160,7 +1189,7 @@ inline void BackwardLaunch(const GradOut &g, const Problem &q, const Plan &p, ch
       // boundary would lose up to 14 bytes behind them to zeros)
       a.out_tiled = a.out_vec && !a.out_add && q.h * elem % 16 == 0;
       const CUtensorMap out = a.out_tiled ? tc5::MatrixMap(a.out, g.gw_type, cols, q.h, g.ld_gw, 128) : x_across;
-      Gemm<kWeightGrad>(d_across, x_across, out, a, static_cast<int64_t>(a.m_tiles) * a.n_tiles, ctas, sms, stream);
+      Gemm<kWeightGrad>(d_across, x_across, x_across_in_place, out, a, static_cast<int64_t>(a.m_tiles) * a.n_tiles, ctas, sms, stream);
     }
   }
   if (g.gx != nullptr) {
