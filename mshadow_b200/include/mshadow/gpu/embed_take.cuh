@@ -38,6 +38,7 @@ namespace embtake {
 const int kChunk = 64;        // sorted entries per CTA; also the longest run that is not split
 const int kFewTokens = 512;   // lists up to this are not sorted
 const int kDepth = 8;         // source rows in flight per thread
+const uint32_t kManyParts = 32;  // a split run of more chunks than this is shared by a CTA's warps
 const int kZeroRows = 32;     // table rows per CTA that writes zeros
 
 // ---- element types: groups of 16 bytes (or single elements) as binary32 ----------------------------
@@ -231,7 +232,8 @@ struct GradArgs {
   uint32_t chunks, slabs;      // CTAs that sum; the ones after them write zeros
   float *parts;                // [2 * chunks][width_pad]: parts of split runs
   int64_t ld_parts;
-  int32_t *spans;              // [0] = number of split runs, then the chunk each begins in
+  int32_t *spans;              // [0], [1] = number of split runs of few / many parts, then (first, last chunk) of
+                               // the runs of few parts from the front, of many parts from the back
 };
 
 template <typename T, bool kVec>
@@ -267,18 +269,7 @@ __device__ __forceinline__ void WriteZeros(const GradArgs<T> &a, uint32_t first,
   }
 }
 
-/*! \brief first position of keys[0, n) that is not below k */
-__device__ __forceinline__ uint32_t LowerBound(const int32_t *keys, uint32_t n, int32_t k) {
-  uint32_t lo = 0, hi = n;
-  while (lo < hi) {
-    const uint32_t mid = (lo + hi) / 2;
-    if (keys[mid] < k) lo = mid + 1;
-    else hi = mid;
-  }
-  return lo;
-}
-
-/*! \brief the same by one warp, 31 places looked at per step */
+/*! \brief first position of keys[0, n) that is not below k; by one warp, 32 places looked at per step */
 __device__ __forceinline__ uint32_t WarpLowerBound(const int32_t *keys, uint32_t n, int32_t k) {
   const uint32_t lane = threadIdx.x & 31;
   uint32_t lo = 0, hi = n;  // the answer lies in [lo, hi]
@@ -403,50 +394,73 @@ __global__ void __launch_bounds__(256) EmbedSumKernel(const GradArgs<T> a) {
         WriteRow<T, kVec>(a, key, col, acc);
       }
     }
-    if (split && lead) a.spans[1 + atomicAdd(a.spans, 1)] = static_cast<int32_t>(chunk);
+    if (split && slab == 0 && threadIdx.x < 32) {
+      const uint32_t last = (WarpLowerBound(a.keys, a.n, key + 1) - 1) / kChunk;  // key < rows <= 2^31 - 1
+      if (lead) {
+        const bool many = last - chunk >= kManyParts;
+        const uint32_t place = static_cast<uint32_t>(atomicAdd(a.spans + (many ? 1 : 0), 1));
+        int2 *list = reinterpret_cast<int2 *>(a.spans + 2);
+        list[many ? a.chunks - 1 - place : place] = make_int2(static_cast<int>(chunk), static_cast<int>(last));
+      }
+    }
     at = stop;
   }
 }
 
+/*! \brief adds the parts c, c + step, ... up to `last` of a run that begins in `chunk`, 4 columns, eight in flight */
+template <typename T>
+__device__ __forceinline__ void AddParts(const GradArgs<T> &a, uint32_t c, uint32_t step, uint32_t chunk, uint32_t last,
+                                         uint32_t col, float (&acc)[4]) {
+  for (; c <= last; c += step * 8) {
+    float4 p[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const uint32_t q = c + step * u;
+      p[u] = make_float4(-0.0f, -0.0f, -0.0f, -0.0f);
+      if (q <= last) {
+        const int64_t row = q == chunk ? 2 * static_cast<int64_t>(q) + 1 : 2 * static_cast<int64_t>(q);
+        p[u] = __ldcs(reinterpret_cast<const float4 *>(a.parts + row * a.ld_parts + col));
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      acc[0] = __fadd_rn(acc[0], p[u].x);
+      acc[1] = __fadd_rn(acc[1], p[u].y);
+      acc[2] = __fadd_rn(acc[2], p[u].z);
+      acc[3] = __fadd_rn(acc[3], p[u].w);
+    }
+  }
+}
+template <typename T>
+__device__ __forceinline__ void WriteFour(const GradArgs<T> &a, int32_t key, uint32_t col, const float (&acc)[4]) {
+#pragma unroll
+  for (int l = 0; l < 4; ++l) {
+    const float one[1] = {acc[l]};
+    if (col + l < a.width) WriteRow<T, false>(a, key, col + l, one);
+  }
+}
+
 /*!
- * \brief adds the parts of the split runs.  A CTA takes one run and 128 columns at a time; its sixteen warps take every
- *  sixteenth part each, eight in flight, and are joined in warp order.  (With eight warps and four in flight the run of
- *  the most frequent of 2^20 Zipf(1.1) tokens, 2300 parts, alone took 100 us.)
+ * \brief adds the parts of the split runs.  A run of few parts is one warp's, 128 columns at a time.  A run of many is
+ *  shared: a CTA takes 128 of its columns, each of its sixteen warps every sixteenth part, and the warps are
+ *  joined in order.  (One list of runs, a CTA of eight warps and 128 columns at a time for each: 118 us
+ *  behind the sums of 2^20 Zipf(1.1) tokens, half of it for the 2300 parts of the most frequent one.)
  */
-template <typename T, bool kVec>
+template <typename T>
 __global__ void __launch_bounds__(512) EmbedSpanKernel(const GradArgs<T> a) {
   gpu_rt::GridDependencySync();
   __shared__ float s_sum[16][128];
-  const uint32_t count = static_cast<uint32_t>(a.spans[0]);
+  const uint32_t few = static_cast<uint32_t>(a.spans[0]), many = static_cast<uint32_t>(a.spans[1]);
+  const int2 *list = reinterpret_cast<const int2 *>(a.spans + 2);
   const uint32_t slabs = (a.width + 127) / 128;
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (uint32_t w = blockIdx.x; w < count * slabs; w += gridDim.x) {
-    const uint32_t chunk = static_cast<uint32_t>(a.spans[1 + w / slabs]);
+  for (uint32_t w = blockIdx.x; w < many * slabs; w += gridDim.x) {
+    const int2 run = list[a.chunks - 1 - w / slabs];
+    const uint32_t chunk = static_cast<uint32_t>(run.x), last = static_cast<uint32_t>(run.y);
+    const int32_t key = a.keys[last * kChunk];
     const uint32_t col = (w % slabs) * 128 + lane * 4;
-    const uint32_t end = min(a.n, (chunk + 1) * kChunk);
-    const int32_t key = a.keys[end - 1];
-    const uint32_t stop = WarpLowerBound(a.keys, a.n, key + 1);  // key < rows <= 2^31 - 1
-    const uint32_t last = (stop - 1) / kChunk;
     float acc[4] = {-0.0f, -0.0f, -0.0f, -0.0f};
-    for (uint32_t c = chunk + warp; c <= last; c += 16 * 8) {
-      float4 p[8];
-#pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const uint32_t q = c + 16 * u;
-        p[u] = make_float4(-0.0f, -0.0f, -0.0f, -0.0f);
-        if (q <= last) {
-          const int64_t row = q == chunk ? 2 * static_cast<int64_t>(q) + 1 : 2 * static_cast<int64_t>(q);
-          p[u] = __ldcs(reinterpret_cast<const float4 *>(a.parts + row * a.ld_parts + col));
-        }
-      }
-#pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        acc[0] = __fadd_rn(acc[0], p[u].x);
-        acc[1] = __fadd_rn(acc[1], p[u].y);
-        acc[2] = __fadd_rn(acc[2], p[u].z);
-        acc[3] = __fadd_rn(acc[3], p[u].w);
-      }
-    }
+    AddParts(a, chunk + warp, 16, chunk, last, col, acc);
     *reinterpret_cast<float4 *>(&s_sum[warp][lane * 4]) = make_float4(acc[0], acc[1], acc[2], acc[3]);
     __syncthreads();
     const uint32_t c = (w % slabs) * 128 + threadIdx.x;
@@ -456,6 +470,15 @@ __global__ void __launch_bounds__(512) EmbedSpanKernel(const GradArgs<T> a) {
       WriteRow<T, false>(a, key, c, sum);
     }
     __syncthreads();
+  }
+  for (uint32_t w = blockIdx.x * 16 + warp; w < few * slabs; w += gridDim.x * 16) {
+    const int2 run = list[w / slabs];
+    const uint32_t chunk = static_cast<uint32_t>(run.x), last = static_cast<uint32_t>(run.y);
+    const int32_t key = a.keys[last * kChunk];
+    const uint32_t col = (w % slabs) * 128 + lane * 4;
+    float acc[4] = {-0.0f, -0.0f, -0.0f, -0.0f};
+    AddParts(a, chunk, 1, chunk, last, col, acc);
+    WriteFour(a, key, col, acc);
   }
 }
 
@@ -598,7 +621,7 @@ inline GradPlan MakeGradPlan(int64_t n, int64_t width) {
   p.rows = take(n * 4);
   p.sort = take(static_cast<int64_t>(sortdetail::ScratchBytes(n)));
   p.parts = take(2ll * p.chunks * p.ld_parts * 4);
-  p.spans = take((1ll + p.chunks) * 4);
+  p.spans = take((1ll + p.chunks) * 8);
   p.bytes = at;
   return p;
 }
@@ -620,8 +643,11 @@ inline void GradGo(GradArgs<T> a, const GradPlan &p, char *ws, cudaStream_t stre
   int bits = 1;
   while (bits < 31 && (int64_t(1) << bits) < a.table_rows) ++bits;
   a.spans = reinterpret_cast<int32_t *>(ws + p.spans);
-  MSHADOW_CUDA_CALL(cudaMemsetAsync(a.spans, 0, 4, stream));
+  MSHADOW_CUDA_CALL(cudaMemsetAsync(a.spans, 0, 8, stream));
   const sortdetail::Source named = {static_cast<int>(a.table_rows), 1};
+  // (Writing the zeros by further CTAs of the sort's launches instead was slower: 186 against 165 us for 16384 indices
+  // into 131072 x 2048 bf16 -- writes alone run at 3.9 TB/s however they are issued, and each of the six launches
+  // drained its share of them before the next began.)
   sortdetail::SortPairs<int32_t, int32_t>(keys, rows, a.index, a.n, bits, true, named, ws + p.sort, stream);
   a.keys = keys, a.rows = rows;
   a.chunks = p.chunks;
@@ -630,7 +656,7 @@ inline void GradGo(GradArgs<T> a, const GradPlan &p, char *ws, cudaStream_t stre
   MSHADOW_CUDA_POST_KERNEL_CHECK(EmbedSumKernel);
   const int64_t most = static_cast<int64_t>(p.chunks) * ((a.width + 127) / 128);
   const int64_t cap = static_cast<int64_t>(gpu_rt::CurrentDevice().sm_count) * 4;
-  gpu_rt::LaunchAfterDrain(EmbedSpanKernel<T, kVec>, dim3(static_cast<unsigned>(std::min(most, cap))), dim3(512), 0, stream, a);
+  gpu_rt::LaunchAfterDrain(EmbedSpanKernel<T>, dim3(static_cast<unsigned>(std::min(most, cap))), dim3(512), 0, stream, a);
   MSHADOW_CUDA_POST_KERNEL_CHECK(EmbedSpanKernel);
 }
 

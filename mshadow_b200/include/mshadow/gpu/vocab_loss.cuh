@@ -89,7 +89,8 @@ struct GemmArgs {
   int32_t m_tiles;       // kWeightGrad: row tiles of the piece (else from the live rows)
   int32_t n_tiles;
   int32_t k_blocks;      // kWeightGrad: from the live rows
-  int32_t slices;        // kDataGrad: the contraction is cut into this many parts
+  int32_t k_plan;        // kDataGrad: k_blocks of the first piece, by which all pieces are cut into the same parts
+  int32_t acc_tiles;     // kDataGrad: row tiles that the partial gradients have room for
   int32_t group;         // row tiles that are walked before the next column tile
   int32_t b_row0;        // first row of B (the piece's first vocabulary row)
   uint32_t instr;
@@ -143,6 +144,35 @@ __device__ __forceinline__ float Widen(uint16_t bits, int bf16) {
 struct Unit {
   int m, n, slice;
 };
+
+/*!
+ * \brief parts into which the contraction of grad x is cut, the same in every thread of a warp that asks.  n x h has few
+ *  tiles and a contraction as long as the vocabulary piece: the cheapest of 1 .. 16 parts by this count
+ *  -- rounds of tiles over the `slots` of the GPU, `cycles` a step, some 4000 to begin and end a tile,
+ *  and the parts written and read again at about 2400 bytes a cycle -- among those of at least eight steps
+ *  for which there is room.  Decided on the device, by the tokens that count.
+ */
+__device__ __forceinline__ int PartsOf(int m_tiles, int n_tiles, int k_blocks, int room, int slots, int tile_m, float cycles) {
+  const int parts = (threadIdx.x & 15) + 1;
+  const int tiles = m_tiles * n_tiles;
+  const bool fits = parts == 1 || (parts * 8 <= k_blocks && parts * m_tiles <= room);
+  const float rounds = static_cast<float>((tiles * parts + slots - 1) / slots);
+  const float steps = static_cast<float>((k_blocks + parts - 1) / parts);
+  // (each operation rounded by itself: the two kernels that ask must not differ by how theirs is compiled)
+  const float tile_cycles = static_cast<float>(tile_m * kTileN * 8 / 2400);
+  float cost = __fadd_rn(__fmul_rn(rounds, __fadd_rn(__fmul_rn(steps, cycles), 4000.0f)),
+                         __fmul_rn(static_cast<float>(parts * tiles), tile_cycles));
+  if (!fits) cost = INFINITY;
+  int best = parts;
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) {
+    const float other = __shfl_xor_sync(0xffffffffu, cost, o);
+    const int which = __shfl_xor_sync(0xffffffffu, best, o);
+    if (other < cost || (other == cost && which < best)) cost = other, best = which;
+  }
+  return best;
+}
+__device__ __forceinline__ float CyclesPerStep(int ctas) { return ctas == 1 ? 560.0f : 512.0f; }
 
 /*! \brief unit u of the walk: `group` row tiles by all column tiles, then the next group; slices outermost */
 __device__ __forceinline__ Unit UnitOf(int u, int m_tiles, int n_tiles, int group) {
@@ -434,8 +464,11 @@ VocabGemmKernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                       : kMode == kDelta    ? max(1, (live + tile_m - 1) / tile_m)
                                            : (live + tile_m - 1) / tile_m;
   const int k_blocks = kMode == kWeightGrad ? max(1, (live + kStepK - 1) / kStepK) : a.k_blocks;
+  const int slices = kMode != kDataGrad ? 1
+                                        : min(k_blocks, PartsOf(max(m_tiles, 1), a.n_tiles, a.k_plan, a.acc_tiles,
+                                                                gridDim.x / kCtas, tile_m, CyclesPerStep(kCtas)));
   const int runs = kMode == kStat ? (k_blocks + kChunkSteps - 1) / kChunkSteps : 1;
-  const int units = m_tiles * a.n_tiles * a.slices;
+  const int units = m_tiles * a.n_tiles * slices;
   const int first = blockIdx.x / kCtas, step = gridDim.x / kCtas;
 
   if (warp < 4) {
@@ -444,7 +477,7 @@ VocabGemmKernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
       bool ok = true;
       for (int w = first; ok && w < units; w += step) {
         const Unit u = UnitOf(w, m_tiles, a.n_tiles, a.group);
-        const int k_begin = u.slice * k_blocks / a.slices, k_end = (u.slice + 1) * k_blocks / a.slices;
+        const int k_begin = u.slice * k_blocks / slices, k_end = (u.slice + 1) * k_blocks / slices;
         const int m0 = u.m * tile_m + static_cast<int>(rank) * 128;
         const int n0 = u.n * tile_n + static_cast<int>(rank) * rows_n;
         for (int kb = k_begin; kb < k_end; ++kb, ++fill) {
@@ -484,7 +517,7 @@ VocabGemmKernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
       bool ok = true;
       for (int w = first; ok && w < units; w += step) {
         const int slice = w / (m_tiles * a.n_tiles);
-        const int k_first = slice * k_blocks / a.slices, k_count = (slice + 1) * k_blocks / a.slices - k_first;
+        const int k_first = slice * k_blocks / slices, k_count = (slice + 1) * k_blocks / slices - k_first;
         for (int run = 0; ok && run < runs; ++run, ++turn) {
           const int k_begin = k_first + run * k_count / runs, k_end = k_first + (run + 1) * k_count / runs;
           const uint32_t half = turn & 1u, use = turn >> 1;
@@ -547,6 +580,7 @@ VocabGemmKernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
       t.row = row0 + t.thread;
       t.col = u.n * tile_n + t.group * kHalfN;
       const int limit = min(a.cols - t.col, tile_n - t.group * kHalfN);  // columns of this half that exist
+      const int label = (kMode == kStat || kMode == kDelta) && t.row < live ? a.label[t.row] : -1;
       if (kMode == kStat) {
         float v[kHalfN];
         for (int run = 0; run < runs; ++run) {
@@ -562,18 +596,17 @@ VocabGemmKernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
           release();
         }
         if (!ok) break;
-        const int label = t.row < live ? a.label[t.row] : -1;
+        if (row0 + (warp & 3) * 32 >= live) continue;  // no row of this warp's exists
         const int64_t at = (static_cast<int64_t>(a.tile0 + u.n) * 2 + t.group) * a.pad_rows + t.row;
         StatHalf(v, t, limit, label < 0 ? -1 : label - a.col0 - t.col, at, a);
         continue;
       }
       if (!ready()) break;
       if (kMode == kDelta) {
-        const int label = t.row < live ? a.label[t.row] : -1;
         // rows past the live ones: lse and scale are 0, the data row is zero, and so is d'
         DeltaHalf(t, limit, label < 0 ? -1 : label - a.col0 - t.col, a.lse2[t.row], a.row_scale[t.row], &map_out, row0, a);
       } else if (kMode == kDataGrad) {
-        const int part = static_cast<int>(u.slice * a.pad_rows);
+        const int part = u.slice * m_tiles * tile_m;
         if (a.accumulate) FloatHalf<true>(t, 1.0f, &map_out, row0, part);
         else FloatHalf<false>(t, 1.0f, &map_out, row0, part);
       } else {
@@ -767,6 +800,8 @@ __global__ void __launch_bounds__(512) JoinTilesKernel(const JoinArgs a) {
   const int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + r;
   if (static_cast<int64_t>(blockIdx.x) * kRows >= live) return;
   float ref = -INFINITY, sum = 0.0f, total = 0.0f;
+  const int32_t label = q == 0 && row < live ? a.label[row] : -1;
+  const double z = q == 0 && row < live ? a.label_logit[row] : 0.0f;  // of no meaning for a row that does not count
   if (row < live) {
     for (int t0 = q; t0 < a.parts; t0 += kShare * 8) {
       float2 p[8];
@@ -799,14 +834,13 @@ __global__ void __launch_bounds__(512) JoinTilesKernel(const JoinArgs a) {
     __syncthreads();
   }
   if (q != 0 || row >= live) return;
-  const int32_t label = a.label[row];
   const int64_t to = a.row_of != nullptr ? a.row_of[row] : row;
   if (!IsLive(label, a.ignore, a.v)) {
     a.loss[to] = 0.0f, a.lse[to] = 0.0f;
     return;
   }
   // a handful of operations per row, in 64 bits: the maximum is tens of units large, the loss may be small
-  const double log_sum = log(static_cast<double>(sum)), z = a.label_logit[row];
+  const double log_sum = log(static_cast<double>(sum));
   double loss = (ref - z) + log_sum;
   if (a.part_sum != nullptr) {
     const double smooth = a.smooth;
@@ -818,8 +852,9 @@ __global__ void __launch_bounds__(512) JoinTilesKernel(const JoinArgs a) {
 
 struct FinishArgs {
   const float *acc;
-  int64_t ld_acc, acc_slice;
-  int slices;
+  int64_t ld_acc;
+  const int32_t *live;
+  int k_plan, acc_tiles, slots, ctas;  // of the kernel that wrote the parts
   const int32_t *pos_of;
   const float *inv_scale;
   uint16_t *out;
@@ -834,14 +869,18 @@ __global__ void __launch_bounds__(256) DataGradFinishKernel(const FinishArgs a) 
   gpu_rt::GridDependencySync();
   const float inv = a.inv_scale[0];
   const int groups = (a.h + 7) / 8;
+  const int tile_m = 128 * a.ctas, m_tiles = (a.live[0] + tile_m - 1) / tile_m;
+  const int slices = PartsOf(max(m_tiles, 1), static_cast<int>(a.ld_acc) / kTileN, a.k_plan, a.acc_tiles, a.slots, tile_m,
+                             CyclesPerStep(a.ctas));
+  const int64_t stride = static_cast<int64_t>(m_tiles) * tile_m * a.ld_acc;
   for (int64_t i = blockIdx.x; i < a.n; i += gridDim.x) {
     const int pos = a.pos_of[i];
     uint16_t *out = a.out + i * a.ld_out;
     for (int g = threadIdx.x; g < groups; g += 256) {
       float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
       if (pos >= 0) {
-        for (int s = 0; s < a.slices; ++s) {
-          const float4 *p = reinterpret_cast<const float4 *>(a.acc + s * a.acc_slice + pos * a.ld_acc) + 2 * g;
+        for (int s = 0; s < slices; ++s) {
+          const float4 *p = reinterpret_cast<const float4 *>(a.acc + s * stride + pos * a.ld_acc) + 2 * g;
           const float4 lo = __ldcs(p), hi = __ldcs(p + 1);
           v[0] += lo.x, v[1] += lo.y, v[2] += lo.z, v[3] += lo.w;
           v[4] += hi.x, v[5] += hi.y, v[6] += hi.z, v[7] += hi.w;
@@ -903,7 +942,7 @@ inline int CtasFor(int64_t rows, int64_t other_tiles, int sms) {
 struct Plan {
   bool pack, copy_w;
   int64_t pad_rows, ld_x, ld_w, piece, ld_acc, tile_n, tiles;
-  int slices, ctas, ctas_gx;
+  int acc_tiles, ctas, ctas_gx;
   int64_t words, row_of, pos_of, label_of, lse2, row_scale, x, w, part, part_sum, label_logit, delta, acc, bytes;
 };
 
@@ -930,23 +969,11 @@ inline Plan MakePlan(int64_t n, int64_t v, int64_t h, bool gradient, bool want_g
     p.tile_n = std::min<int64_t>(kTileN, RoundUp(Ceil(v, rounds * sms), 16));
   }
   p.tiles = Ceil(v, p.tile_n);
-  p.slices = 1;
-  p.ctas_gx = 2;
-  if (gradient && want_gx) {
-    // n x h has few tiles and a contraction as long as the piece: it is cut into parts (at least eight steps
-    // long) that give every SM work.  The cheapest of all cuts by this count: rounds of tiles, 512 cycles a step, some
-    // 4000 to begin and end a tile, and the parts written and read again at about 2400 bytes a cycle.
-    double best = 0.0;
-    for (int ctas = 1; ctas <= 2; ++ctas) {
-      const int64_t tiles = Ceil(n, 128 * ctas) * (p.ld_acc / kTileN);
-      for (int64_t slices = 1; slices <= 16 && (slices == 1 || p.piece / kStepK >= 8 * slices); ++slices) {
-        const double rounds = static_cast<double>(Ceil(tiles * slices, sms / ctas));
-        const double steps = static_cast<double>(Ceil(p.piece / kStepK, slices));
-        const double cost = rounds * (steps * (ctas == 1 ? 560.0 : 512.0) + 4000.0) + slices * n * p.ld_acc * 8 / 2400.0;
-        if (best == 0.0 || cost < best) best = cost, p.slices = static_cast<int>(slices), p.ctas_gx = ctas;
-      }
-    }
-  }
+  p.ctas_gx = CtasFor(n, p.ld_acc / kTileN, sms);
+  // room for as many parts of the gradient of x as give every SM a tile when all tokens count (PartsOf cuts it)
+  const int64_t x_tiles = Ceil(n, 128 * p.ctas_gx);
+  const int64_t parts = std::min<int64_t>(16, Ceil(2 * sms / p.ctas_gx, x_tiles * (p.ld_acc / kTileN)));
+  p.acc_tiles = static_cast<int>(x_tiles * std::max<int64_t>(1, std::min<int64_t>(parts, p.piece / kStepK / 8)));
   int64_t at = 0;
   auto take = [&at](int64_t bytes) {
     const int64_t was = at;
@@ -963,7 +990,7 @@ inline Plan MakePlan(int64_t n, int64_t v, int64_t h, bool gradient, bool want_g
     p.lse2 = take(p.pad_rows * 4);
     p.row_scale = take(p.pad_rows * 4);
     p.delta = take(p.pad_rows * p.piece * 2);
-    p.acc = take(want_gx ? p.slices * p.pad_rows * p.ld_acc * 4 : 0);
+    p.acc = take(want_gx ? static_cast<int64_t>(p.acc_tiles) * 128 * p.ctas_gx * p.ld_acc * 4 : 0);
   } else {
     p.part = take(2 * p.tiles * p.pad_rows * 8);
     p.part_sum = take(smooth ? 2 * p.tiles * p.pad_rows * 4 : 0);
@@ -996,7 +1023,9 @@ inline void LaunchGemm(const CUtensorMap &ma, const CUtensorMap &mb, const CUten
   const size_t smem = StageShape<kCtas>::kSmem;
   gpu_rt::AllowSharedMemory(kernel, smem);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>(std::max<int64_t>(units, 1), sms / kCtas)) * kCtas);
+  // (the parts of kDataGrad are counted by the kernel: it gets every slot)
+  const int64_t slots = kMode == kDataGrad ? sms / kCtas : std::min<int64_t>(std::max<int64_t>(units, 1), sms / kCtas);
+  cfg.gridDim = dim3(static_cast<unsigned>(slots) * kCtas);
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
@@ -1067,7 +1096,6 @@ inline void ForwardLaunch(float *loss, float *lse, const Problem &q, const Plan 
   a.live = p.pack ? reinterpret_cast<const int32_t *>(ws + p.words) : nullptr;
   a.tokens = static_cast<int32_t>(q.n);
   a.k_blocks = static_cast<int32_t>(Ceil(q.h, kStepK));
-  a.slices = 1;
   const int64_t m_tiles = Ceil(q.n, 128 * p.ctas);
   a.group = GroupOf(m_tiles);
   a.instr = tc5::InstrDesc(q.bf16, false, false, 128 * p.ctas, static_cast<int>(p.tile_n));
@@ -1150,8 +1178,7 @@ inline void BackwardLaunch(const GradOut &g, const Problem &q, const Plan &p, ch
     const int64_t m_tiles = Ceil(q.n, 128 * p.ctas);
     a.cols = static_cast<int32_t>(cols);
     a.col0 = static_cast<int32_t>(p0);
-    a.slices = 1;
-    a.n_tiles = static_cast<int32_t>(Ceil(cols, kTileN));
+      a.n_tiles = static_cast<int32_t>(Ceil(cols, kTileN));
     a.k_blocks = static_cast<int32_t>(Ceil(q.h, kStepK));
     a.group = GroupOf(m_tiles);
     a.instr = tc5::InstrDesc(q.bf16, false, false, 128 * p.ctas, kTileN);
@@ -1159,23 +1186,23 @@ inline void BackwardLaunch(const GradOut &g, const Problem &q, const Plan &p, ch
     Gemm<kDelta>(x_along, w_along, x_along_in_place, d_along, a, m_tiles * a.n_tiles, p.ctas, sms, stream);
     if (g.gx != nullptr) {
       const CUtensorMap w_across = WeightMap(q, p, ws, p0, cols, 64, stream, false, &a.b_row0);
-      const CUtensorMap out = tc5::MatrixMap(acc, kFloat32, p.slices * p.pad_rows, p.ld_acc, p.ld_acc, 128);
+      const CUtensorMap out = tc5::MatrixMap(acc, kFloat32, static_cast<int64_t>(p.acc_tiles) * 128 * p.ctas_gx, p.ld_acc, p.ld_acc, 128);
       const int64_t x_tiles = Ceil(q.n, 128 * p.ctas_gx);
       a.n_tiles = h_tiles;
       a.k_blocks = static_cast<int32_t>(Ceil(cols, kStepK));
-      a.slices = std::min(p.slices, a.k_blocks);  // the last piece may be shorter than the parts are many
+      a.k_plan = static_cast<int32_t>(Ceil(std::min(p.piece, q.v), kStepK));
+      a.acc_tiles = p.acc_tiles;
       a.accumulate = p0 > 0;
       a.group = GroupOf(x_tiles);
       a.instr = tc5::InstrDesc(q.bf16, false, true, 128 * p.ctas_gx, kTileN);
-      Gemm<kDataGrad>(d_along, w_across, d_along, out, a, x_tiles * a.n_tiles * a.slices, p.ctas_gx, sms, stream);
+      Gemm<kDataGrad>(d_along, w_across, d_along, out, a, x_tiles * a.n_tiles, p.ctas_gx, sms, stream);
     }
     if (g.gw != nullptr) {
       const int64_t elem = g.gw_type == kFloat32 ? 4 : 2;
       const int ctas = CtasFor(cols, h_tiles, sms);
       a.m_tiles = static_cast<int32_t>(Ceil(cols, 128 * ctas));
       a.n_tiles = h_tiles;
-      a.slices = 1;
-      a.b_row0 = 0;
+          a.b_row0 = 0;
       a.group = GroupOf(a.m_tiles);
       a.instr = tc5::InstrDesc(q.bf16, true, true, 128 * ctas, kTileN);
       a.out = static_cast<char *>(g.gw) + p0 * g.ld_gw * elem;
@@ -1194,7 +1221,8 @@ inline void BackwardLaunch(const GradOut &g, const Problem &q, const Plan &p, ch
   }
   if (g.gx != nullptr) {
     FinishArgs f = {};
-    f.acc = acc, f.ld_acc = p.ld_acc, f.acc_slice = p.pad_rows * p.ld_acc, f.slices = p.slices;
+    f.acc = acc, f.ld_acc = p.ld_acc, f.live = a.live;
+    f.k_plan = a.k_plan, f.acc_tiles = p.acc_tiles, f.slots = sms / p.ctas_gx, f.ctas = p.ctas_gx;
     f.pos_of = k.pos_of, f.inv_scale = a.inv_scale;
     f.out = g.gx, f.ld_out = g.ld_gx, f.n = static_cast<int32_t>(q.n), f.h = static_cast<int32_t>(q.h);
     f.bf16 = q.bf16, f.vec = Aligned16(g.gx, g.ld_gx, 2);
