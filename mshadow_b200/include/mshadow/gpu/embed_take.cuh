@@ -442,32 +442,38 @@ __device__ __forceinline__ void WriteFour(const GradArgs<T> &a, int32_t key, uin
 
 /*!
  * \brief adds the parts of the split runs.  A run of few parts is one warp's, 128 columns at a time.  A run of many is
- *  shared: a CTA takes 128 of its columns, each of its sixteen warps every sixteenth part, and the warps are
- *  joined in order.  (One list of runs, a CTA of eight warps and 128 columns at a time for each: 118 us
- *  behind the sums of 2^20 Zipf(1.1) tokens, half of it for the 2300 parts of the most frequent one.)
+ *  shared: a CTA takes 32 of its columns, each quarter of its sixteen warps every 64th part, and they are
+ *  joined in order.  Bound by the latency of dependent loads, so what counts is parts in flight.  (One list of runs, a
+ *  CTA of eight warps and 128 columns at a time for each: 118 us behind the sums of 2^20 Zipf(1.1) tokens, most
+ *  of it for the 2300 parts of the most frequent one; shared by 128 columns and sixteen warps: 59 us.)
  */
 template <typename T>
 __global__ void __launch_bounds__(512) EmbedSpanKernel(const GradArgs<T> a) {
   gpu_rt::GridDependencySync();
-  __shared__ float s_sum[16][128];
+  __shared__ float s_sum[16][32];
   const uint32_t few = static_cast<uint32_t>(a.spans[0]), many = static_cast<uint32_t>(a.spans[1]);
   const int2 *list = reinterpret_cast<const int2 *>(a.spans + 2);
-  const uint32_t slabs = (a.width + 127) / 128;
+  const uint32_t slabs = (a.width + 127) / 128, strips = (a.width + 31) / 32;
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (uint32_t w = blockIdx.x; w < many * slabs; w += gridDim.x) {
-    const int2 run = list[a.chunks - 1 - w / slabs];
+  for (uint32_t w = blockIdx.x; w < many * strips; w += gridDim.x) {
+    const int2 run = list[a.chunks - 1 - w / strips];
     const uint32_t chunk = static_cast<uint32_t>(run.x), last = static_cast<uint32_t>(run.y);
     const int32_t key = a.keys[last * kChunk];
-    const uint32_t col = (w % slabs) * 128 + lane * 4;
+    const uint32_t strip = (w % strips) * 32;
     float acc[4] = {-0.0f, -0.0f, -0.0f, -0.0f};
-    AddParts(a, chunk + warp, 16, chunk, last, col, acc);
-    *reinterpret_cast<float4 *>(&s_sum[warp][lane * 4]) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+    AddParts(a, chunk + warp * 4 + lane / 8, 64, chunk, last, strip + (lane & 7) * 4, acc);
+#pragma unroll
+    for (int l = 0; l < 4; ++l) {
+      acc[l] = __fadd_rn(acc[l], __shfl_xor_sync(0xffffffffu, acc[l], 8));
+      acc[l] = __fadd_rn(acc[l], __shfl_xor_sync(0xffffffffu, acc[l], 16));
+    }
+    if (lane < 8) *reinterpret_cast<float4 *>(&s_sum[warp][lane * 4]) = make_float4(acc[0], acc[1], acc[2], acc[3]);
     __syncthreads();
-    const uint32_t c = (w % slabs) * 128 + threadIdx.x;
-    if (threadIdx.x < 128 && c < a.width) {
+    if (threadIdx.x < 32 && strip + threadIdx.x < a.width) {
       float sum[1] = {s_sum[0][threadIdx.x]};
+#pragma unroll
       for (int q = 1; q < 16; ++q) sum[0] = __fadd_rn(sum[0], s_sum[q][threadIdx.x]);
-      WriteRow<T, false>(a, key, c, sum);
+      WriteRow<T, false>(a, key, strip + threadIdx.x, sum);
     }
     __syncthreads();
   }
