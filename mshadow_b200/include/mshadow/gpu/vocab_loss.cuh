@@ -71,13 +71,15 @@ struct Layout {
   static const bool kBAcross = kMode == kDataGrad || kMode == kWeightGrad;
 };
 
-template <int kCtas>
+/*! \brief kWide: a pair's tile is 512 columns wide, two sets of 256, and fills the tensor memory */
+template <int kCtas, bool kWide>
 struct StageShape {
-  static const int kRowsN = kTileN / kCtas;                          // rows of B that a CTA holds
+  static const int kRowsN = kTileN / kCtas;                          // rows of B that a CTA holds, of a set
+  static const int kSets = kWide ? 2 : 1;                            // sets of accumulators per tile
   static const uint32_t kBytesA = 128 * kStepK * 2;
   static const uint32_t kBytesB = kRowsN * kStepK * 2;
-  static const uint32_t kStage = kBytesA + kBytesB;
-  static const int kStages = kCtas == 2 ? 6 : 4;
+  static const uint32_t kStage = kBytesA + kSets * kBytesB;
+  static const int kStages = kCtas == 2 && !kWide ? 6 : 4;
   static const uint32_t kOut = kStage * kStages;                     // a box per epilogue group
   static const size_t kSmem = kOut + 2 * kBoxOut + 1024;  // + alignment to the swizzle's 1024 bytes
 };
@@ -91,6 +93,7 @@ struct GemmArgs {
   int32_t k_blocks;      // kWeightGrad: from the live rows
   int32_t k_plan;        // kDataGrad: k_blocks of the first piece, by which all pieces are cut into the same parts
   int32_t acc_tiles;     // kDataGrad: row tiles that the partial gradients have room for
+  float step_cycles, tile_cycles;  // kDataGrad: what PartsOf counts
   int32_t group;         // row tiles that are walked before the next column tile
   int32_t b_row0;        // first row of B (the piece's first vocabulary row)
   uint32_t instr;
@@ -148,19 +151,19 @@ struct Unit {
 /*!
  * \brief parts into which the contraction of grad x is cut, the same in every thread of a warp that asks.  n x h has few
  *  tiles and a contraction as long as the vocabulary piece: the cheapest of 1 .. 16 parts by this count
- *  -- rounds of tiles over the `slots` of the GPU, `cycles` a step, some 4000 to begin and end a tile,
- *  and the parts written and read again at about 2400 bytes a cycle -- among those of at least eight steps
+ *  -- rounds of tiles over the `slots` of the GPU, step_cycles a step, some 4000 to begin and end a tile,
+ *  and tile_cycles to write a part of a tile and read it again -- among those of at least eight steps
  *  for which there is room.  Decided on the device, by the tokens that count.
  */
-__device__ __forceinline__ int PartsOf(int m_tiles, int n_tiles, int k_blocks, int room, int slots, int tile_m, float cycles) {
+__device__ __forceinline__ int PartsOf(int m_tiles, int n_tiles, int k_blocks, int room, int slots, float step_cycles,
+                                       float tile_cycles) {
   const int parts = (threadIdx.x & 15) + 1;
   const int tiles = m_tiles * n_tiles;
   const bool fits = parts == 1 || (parts * 8 <= k_blocks && parts * m_tiles <= room);
   const float rounds = static_cast<float>((tiles * parts + slots - 1) / slots);
   const float steps = static_cast<float>((k_blocks + parts - 1) / parts);
   // (each operation rounded by itself: the two kernels that ask must not differ by how theirs is compiled)
-  const float tile_cycles = static_cast<float>(tile_m * kTileN * 8 / 2400);
-  float cost = __fadd_rn(__fmul_rn(rounds, __fadd_rn(__fmul_rn(steps, cycles), 4000.0f)),
+  float cost = __fadd_rn(__fmul_rn(rounds, __fadd_rn(__fmul_rn(steps, step_cycles), 4000.0f)),
                          __fmul_rn(static_cast<float>(parts * tiles), tile_cycles));
   if (!fits) cost = INFINITY;
   int best = parts;
@@ -172,7 +175,6 @@ __device__ __forceinline__ int PartsOf(int m_tiles, int n_tiles, int k_blocks, i
   }
   return best;
 }
-__device__ __forceinline__ float CyclesPerStep(int ctas) { return ctas == 1 ? 560.0f : 512.0f; }
 
 /*! \brief unit u of the walk: `group` row tiles by all column tiles, then the next group; slices outermost */
 __device__ __forceinline__ Unit UnitOf(int u, int m_tiles, int n_tiles, int group) {
@@ -408,19 +410,23 @@ __device__ __forceinline__ void WeightColumns(const uint32_t (&r)[32], int64_t r
 
 /*!
  * \brief persistent product kernel of all four modes.  kCtas CTAs (a cluster) share a tile of
- *  128 * kCtas rows by 256 columns (kStat: a.tile_n).  Dynamic shared memory StageShape<kCtas>::kSmem.
+ *  128 * kCtas rows by 256 columns (kStat: a.tile_n; kWide: 512).  Dynamic shared memory StageShape::kSmem.
  *
  *  Tensor memory holds two sets of accumulators; the products of one run into them while the epilogue empties the
  *  other.  A set is a whole tile, except in kStat: there the contraction is cut into runs of at most
  *  1024 elements, which the epilogue adds up in registers.  The tensor cores cut off, rather than
  *  round, each time they add to an accumulator, always towards zero: over 4096 elements that moved
  *  the loss by 1.8e-6 of its value, against 6e-7 for a product in plain binary32.
+ *
+ *  kWide: both sets belong to one tile.  A step's rows of A then serve 512 columns, a quarter less is read from the L2
+ *  and, where A is d', from memory; in return the products wait while a tile is emptied.  For the gradients
+ *  with long contractions.
  */
-template <int kMode, int kCtas>
+template <int kMode, int kCtas, bool kWide>
 __global__ void __launch_bounds__(kThreads, 1)
 VocabGemmKernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                 const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_out, const GemmArgs a) {
-  typedef StageShape<kCtas> S;
+  typedef StageShape<kCtas, kWide> S;
   typedef Layout<kMode> L;
   extern __shared__ uint8_t raw[];
   __shared__ uint64_t full[S::kStages], empty[S::kStages], acc_full[2], acc_empty[2];
@@ -457,8 +463,8 @@ VocabGemmKernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
   const CUtensorMap *from_a = (kMode == kStat || kMode == kDelta) && in_place ? &map_x : &map_a;
   const CUtensorMap *from_b = kMode == kWeightGrad && in_place ? &map_x : &map_b;
   const int tile_m = 128 * kCtas;
-  const int tile_n = kMode == kStat ? a.tile_n : kTileN;
-  const int rows_n = tile_n / kCtas;  // rows of B that this CTA loads
+  const int tile_n = kMode == kStat ? a.tile_n : S::kSets * kTileN;
+  const int rows_n = kMode == kStat ? tile_n / kCtas : S::kRowsN;  // rows of B that this CTA loads, of a set
   // an empty batch still passes one tile of zeros through the products that end in d and in grad W
   const int m_tiles = kMode == kWeightGrad ? a.m_tiles
                       : kMode == kDelta    ? max(1, (live + tile_m - 1) / tile_m)
@@ -466,7 +472,7 @@ VocabGemmKernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
   const int k_blocks = kMode == kWeightGrad ? max(1, (live + kStepK - 1) / kStepK) : a.k_blocks;
   const int slices = kMode != kDataGrad ? 1
                                         : min(k_blocks, PartsOf(max(m_tiles, 1), a.n_tiles, a.k_plan, a.acc_tiles,
-                                                                gridDim.x / kCtas, tile_m, CyclesPerStep(kCtas)));
+                                                                gridDim.x / kCtas, a.step_cycles, a.tile_cycles));
   const int runs = kMode == kStat ? (k_blocks + kChunkSteps - 1) / kChunkSteps : 1;
   const int units = m_tiles * a.n_tiles * slices;
   const int first = blockIdx.x / kCtas, step = gridDim.x / kCtas;
@@ -488,7 +494,7 @@ VocabGemmKernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
             break;
           }
           const uint32_t bar = kCtas == 2 ? tc5::MapToRank(tma::SharedAddr(&full[s]), 0) : tma::SharedAddr(&full[s]);
-          if (rank == 0) tma::BarrierExpect(&full[s], (S::kBytesA + rows_n * kStepK * 2) * kCtas);
+          if (rank == 0) tma::BarrierExpect(&full[s], (S::kBytesA + S::kSets * rows_n * kStepK * 2) * kCtas);
           const uint32_t sa = smem + s * S::kStage, sb = sa + S::kBytesA;
           const int k0 = kb * kStepK;
           if (L::kAAcross) {
@@ -499,8 +505,10 @@ VocabGemmKernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
           }
           if (L::kBAcross) {
 #pragma unroll
-            for (int j = 0; j < S::kRowsN / 64; ++j)
-              tc5::LoadBox<kCtas>(sb + j * tc5::kBoxBytes, from_b, n0 + 64 * j, a.b_row0 + k0, bar);
+            for (int j = 0; j < S::kSets * S::kRowsN / 64; ++j) {
+              const int set = j / (S::kRowsN / 64), x = n0 + set * kTileN + 64 * (j % (S::kRowsN / 64));
+              tc5::LoadBox<kCtas>(sb + j * tc5::kBoxBytes, from_b, x, a.b_row0 + k0, bar);
+            }
           } else {
             tc5::LoadBox<kCtas>(sb, from_b, k0, a.b_row0 + n0, bar);
           }
@@ -518,33 +526,31 @@ VocabGemmKernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
       for (int w = first; ok && w < units; w += step) {
         const int slice = w / (m_tiles * a.n_tiles);
         const int k_first = slice * k_blocks / slices, k_count = (slice + 1) * k_blocks / slices - k_first;
-        for (int run = 0; ok && run < runs; ++run, ++turn) {
+        for (int run = 0; ok && run < runs; ++run, turn += S::kSets) {
           const int k_begin = k_first + run * k_count / runs, k_end = k_first + (run + 1) * k_count / runs;
-          const uint32_t half = turn & 1u, use = turn >> 1;
-          if (use > 0 && !tma::WaitBounded(&acc_empty[half], (use - 1) & 1u)) {
-            ok = false;
-            break;
-          }
-          tc5::FenceAfter();
-          const uint32_t acc = tmem + half * kTileN;
-          for (int kb = k_begin; kb < k_end; ++kb, ++fill) {
+          for (int kb = k_begin; ok && kb < k_end; ++kb, ++fill) {
             const int s = fill % S::kStages;
-            if (!tma::WaitBounded(&full[s], (fill / S::kStages) & 1u)) {
-              ok = false;
-              break;
-            }
-            tc5::FenceAfter();
-            const uint32_t sa = smem + s * S::kStage, sb = sa + S::kBytesA;
-            const uint64_t da = L::kAAcross ? tc5::DescAcrossK(sa) : tc5::DescAlongK(sa);
-            const uint64_t db = L::kBAcross ? tc5::DescAcrossK(sb) : tc5::DescAlongK(sb);
-            const uint32_t step_a = L::kAAcross ? 2048 >> 4 : 32 >> 4, step_b = L::kBAcross ? 2048 >> 4 : 32 >> 4;
+            const uint32_t sa = smem + s * S::kStage;
 #pragma unroll
-            for (int j = 0; j < kStepK / 16; ++j) {
-              tc5::Multiply<kCtas>(acc, da + j * step_a, db + j * step_b, a.instr, kb > k_begin || j > 0);
+            for (int set = 0; set < S::kSets; ++set) {
+              // the set's accumulators have been emptied (asked once per run), the stage has been filled
+              const uint32_t half = (turn + set) & 1u, use = (turn + set) >> 1;
+              if (ok && kb == k_begin && use > 0) ok = tma::WaitBounded(&acc_empty[half], (use - 1) & 1u);
+              if (ok && set == 0) ok = tma::WaitBounded(&full[s], (fill / S::kStages) & 1u);
+              if (!ok) break;
+              tc5::FenceAfter();
+              const uint32_t acc = tmem + half * kTileN, sb = sa + S::kBytesA + set * S::kBytesB;
+              const uint64_t da = L::kAAcross ? tc5::DescAcrossK(sa) : tc5::DescAlongK(sa);
+              const uint64_t db = L::kBAcross ? tc5::DescAcrossK(sb) : tc5::DescAlongK(sb);
+              const uint32_t step_a = L::kAAcross ? 2048 >> 4 : 32 >> 4, step_b = L::kBAcross ? 2048 >> 4 : 32 >> 4;
+#pragma unroll
+              for (int j = 0; j < kStepK / 16; ++j) {
+                tc5::Multiply<kCtas>(acc, da + j * step_a, db + j * step_b, a.instr, kb > k_begin || j > 0);
+              }
+              if (set == S::kSets - 1) tc5::CommitTo<kCtas>(&empty[s]);
+              if (kb == k_end - 1) tc5::CommitTo<kCtas>(&acc_full[half]);
             }
-            tc5::CommitTo<kCtas>(&empty[s]);
           }
-          if (ok) tc5::CommitTo<kCtas>(&acc_full[half]);
         }
       }
       if (!ok) atomicExch(a.status, tma::kStatusBulkCopyTimeout);
@@ -601,30 +607,37 @@ VocabGemmKernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         StatHalf(v, t, limit, label < 0 ? -1 : label - a.col0 - t.col, at, a);
         continue;
       }
-      if (!ready()) break;
       if (kMode == kDelta) {
+        if (!ready()) break;
         // rows past the live ones: lse and scale are 0, the data row is zero, and so is d'
         DeltaHalf(t, limit, label < 0 ? -1 : label - a.col0 - t.col, a.lse2[t.row], a.row_scale[t.row], &map_out, row0, a);
-      } else if (kMode == kDataGrad) {
-        const int part = u.slice * m_tiles * tile_m;
-        if (a.accumulate) FloatHalf<true>(t, 1.0f, &map_out, row0, part);
-        else FloatHalf<false>(t, 1.0f, &map_out, row0, part);
-      } else {
-        const float inv = a.inv_scale[0];
-        if (a.out_tiled) {
-          if (a.out_type == kFloat32) FloatHalf<false>(t, inv, &map_out, row0, 0);
-          else PackedHalf(t, inv, a.out_type == kBfloat16, &map_out, row0);
+        release();
+        continue;
+      }
+      for (int set = 0; set < S::kSets; ++set, t.col += kTileN) {
+        if (!ready()) break;
+        if (kMode == kDataGrad) {
+          const int part = u.slice * m_tiles * tile_m;
+          if (a.accumulate) FloatHalf<true>(t, 1.0f, &map_out, row0, part);
+          else FloatHalf<false>(t, 1.0f, &map_out, row0, part);
         } else {
+          const float inv = a.inv_scale[0];
+          if (a.out_tiled) {
+            if (a.out_type == kFloat32) FloatHalf<false>(t, inv, &map_out, row0, 0);
+            else PackedHalf(t, inv, a.out_type == kBfloat16, &map_out, row0);
+          } else {
 #pragma unroll 1
-          for (int c = 0; c < kHalfN / 32; ++c) {
-            uint32_t r[32];
-            tc5::LoadColumns(t.acc + c * 32, r);
-            tc5::WaitColumns(r);
-            if (t.row < a.out_rows) WeightColumns(r, t.row, t.col + c * 32, inv, a);
+            for (int c = 0; c < kHalfN / 32; ++c) {
+              uint32_t r[32];
+              tc5::LoadColumns(t.acc + c * 32, r);
+              tc5::WaitColumns(r);
+              if (t.row < a.out_rows) WeightColumns(r, t.row, t.col + c * 32, inv, a);
+            }
           }
         }
+        release();
       }
-      release();
+      if (!ok) break;
     }
     if (!ok && t.thread == 0) atomicExch(a.status, tma::kStatusBulkCopyTimeout);
     if (kMode != kStat && t.thread == 0) tc5::WaitStores();
@@ -854,7 +867,8 @@ struct FinishArgs {
   const float *acc;
   int64_t ld_acc;
   const int32_t *live;
-  int k_plan, acc_tiles, slots, ctas;  // of the kernel that wrote the parts
+  int n_tiles, k_plan, acc_tiles, slots, ctas;  // of the kernel that wrote the parts
+  float step_cycles, tile_cycles;
   const int32_t *pos_of;
   const float *inv_scale;
   uint16_t *out;
@@ -870,8 +884,7 @@ __global__ void __launch_bounds__(256) DataGradFinishKernel(const FinishArgs a) 
   const float inv = a.inv_scale[0];
   const int groups = (a.h + 7) / 8;
   const int tile_m = 128 * a.ctas, m_tiles = (a.live[0] + tile_m - 1) / tile_m;
-  const int slices = PartsOf(max(m_tiles, 1), static_cast<int>(a.ld_acc) / kTileN, a.k_plan, a.acc_tiles, a.slots, tile_m,
-                             CyclesPerStep(a.ctas));
+  const int slices = PartsOf(max(m_tiles, 1), a.n_tiles, a.k_plan, a.acc_tiles, a.slots, a.step_cycles, a.tile_cycles);
   const int64_t stride = static_cast<int64_t>(m_tiles) * tile_m * a.ld_acc;
   for (int64_t i = blockIdx.x; i < a.n; i += gridDim.x) {
     const int pos = a.pos_of[i];
@@ -927,6 +940,9 @@ inline bool Aligned16(const void *p, int64_t ld, int64_t elem) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * elem % 16 == 0;
 }
 
+#ifndef MSHADOW_B200_VLOSS_WIDE
+#define MSHADOW_B200_VLOSS_WIDE 96
+#endif
 /*!
  * \brief one CTA or a pair per tile.  A pair reads each operand half as often and runs a long grid of tiles
  *  about 6 % faster (8192 x 131072 x 4096: 6.06 against 6.50 ms), but its tiles are twice as high: where that
@@ -938,11 +954,21 @@ inline int CtasFor(int64_t rows, int64_t other_tiles, int sms) {
   return single * 107 < pair * 100 ? 1 : 2;
 }
 
+/*!
+ * \brief tiles of 512 columns (kWide) for a gradient with `tiles` tiles of 256, `h_tiles` side by side, and a contraction
+ *  of `steps`: enough of them that whole rounds over the SMs lose little, and steps enough that emptying a tile
+ *  while nothing multiplies (some 8000 cycles) costs less than the quarter of the loads that is saved
+ */
+inline bool WideFor(int64_t tiles, int64_t h_tiles, int64_t steps, int sms) {
+  return h_tiles % 2 == 0 && tiles / 2 >= sms && steps >= MSHADOW_B200_VLOSS_WIDE;
+}
+
 /*! \brief how a call is cut, and where its scratch matrices lie (offsets in bytes) */
 struct Plan {
   bool pack, copy_w;
   int64_t pad_rows, ld_x, ld_w, piece, ld_acc, tile_n, tiles;
   int acc_tiles, ctas, ctas_gx;
+  bool wide_gx;
   int64_t words, row_of, pos_of, label_of, lse2, row_scale, x, w, part, part_sum, label_logit, delta, acc, bytes;
 };
 
@@ -969,10 +995,12 @@ inline Plan MakePlan(int64_t n, int64_t v, int64_t h, bool gradient, bool want_g
     p.tile_n = std::min<int64_t>(kTileN, RoundUp(Ceil(v, rounds * sms), 16));
   }
   p.tiles = Ceil(v, p.tile_n);
-  p.ctas_gx = CtasFor(n, p.ld_acc / kTileN, sms);
-  // room for as many parts of the gradient of x as give every SM a tile when all tokens count (PartsOf cuts it)
+  const int64_t h_tiles = p.ld_acc / kTileN;
+  p.ctas_gx = CtasFor(n, h_tiles, sms);
   const int64_t x_tiles = Ceil(n, 128 * p.ctas_gx);
-  const int64_t parts = std::min<int64_t>(16, Ceil(2 * sms / p.ctas_gx, x_tiles * (p.ld_acc / kTileN)));
+  p.wide_gx = p.ctas_gx == 2 && WideFor(x_tiles * h_tiles, h_tiles, Ceil(p.piece, kStepK), sms);
+  // room for as many parts of the gradient of x as give every SM two tiles when all tokens count (PartsOf cuts it)
+  const int64_t parts = std::min<int64_t>(16, Ceil(2 * sms / p.ctas_gx, x_tiles * h_tiles / (p.wide_gx ? 2 : 1)));
   p.acc_tiles = static_cast<int>(x_tiles * std::max<int64_t>(1, std::min<int64_t>(parts, p.piece / kStepK / 8)));
   int64_t at = 0;
   auto take = [&at](int64_t bytes) {
@@ -1016,11 +1044,11 @@ inline size_t WorkspaceNeed(int64_t n, int64_t v, int64_t h, bool gradient, int 
   return static_cast<size_t>(most);
 }
 
-template <int kMode, int kCtas>
+template <int kMode, int kCtas, bool kWide>
 inline void LaunchGemm(const CUtensorMap &ma, const CUtensorMap &mb, const CUtensorMap &mx, const CUtensorMap &mo, const GemmArgs &args, int64_t units,
                        int sms, cudaStream_t stream) {
-  auto kernel = VocabGemmKernel<kMode, kCtas>;
-  const size_t smem = StageShape<kCtas>::kSmem;
+  auto kernel = VocabGemmKernel<kMode, kCtas, kWide>;
+  const size_t smem = StageShape<kCtas, kWide>::kSmem;
   gpu_rt::AllowSharedMemory(kernel, smem);
   cudaLaunchConfig_t cfg = {};
   // (the parts of kDataGrad are counted by the kernel: it gets every slot)
@@ -1043,17 +1071,20 @@ inline void LaunchGemm(const CUtensorMap &ma, const CUtensorMap &mb, const CUten
 }
 
 template <int kMode>
-inline void Gemm(const CUtensorMap &ma, const CUtensorMap &mb, const CUtensorMap &mx, const CUtensorMap &mo, const GemmArgs &args, int64_t units,
-                 int ctas, int sms, cudaStream_t stream) {
-  if (ctas == 2) LaunchGemm<kMode, 2>(ma, mb, mx, mo, args, units, sms, stream);
-  else LaunchGemm<kMode, 1>(ma, mb, mx, mo, args, units, sms, stream);
+inline void Gemm(const CUtensorMap &ma, const CUtensorMap &mb, const CUtensorMap &mx, const CUtensorMap &mo, const GemmArgs &args,
+                 int64_t units, int ctas, int sms, cudaStream_t stream) {
+  if (ctas == 2) LaunchGemm<kMode, 2, false>(ma, mb, mx, mo, args, units, sms, stream);
+  else LaunchGemm<kMode, 1, false>(ma, mb, mx, mo, args, units, sms, stream);
 }
 
-#ifndef MSHADOW_B200_VLOSS_GROUP
-#define MSHADOW_B200_VLOSS_GROUP 16
-#endif
-/*! \brief row tiles walked before the next column tile: together their operand rows stay in the L2 */
-inline int GroupOf(int64_t m_tiles) { return static_cast<int>(std::min<int64_t>(std::max<int64_t>(m_tiles, 1), MSHADOW_B200_VLOSS_GROUP)); }
+/*!
+ * \brief row tiles walked before the next column tile, so that what the tiles in flight read again stays in the L2.
+ *  8192 x 131072 x 4096: the two products over h take 6 % less time in bands of 16 row tiles than of 4 or 32, the
+ *  two gradients 2 % less in bands of 8 than of 16.
+ */
+inline int GroupOf(int64_t m_tiles, int64_t most) {
+  return static_cast<int>(std::min<int64_t>(std::max<int64_t>(m_tiles, 1), most));
+}
 
 /*! \brief the weight rows [p0, p0 + rows) as the products read them: map over W itself, or over an aligned copy */
 inline CUtensorMap WeightMap(const Problem &q, const Plan &p, char *ws, int64_t p0, int64_t rows, int box_rows,
@@ -1097,7 +1128,7 @@ inline void ForwardLaunch(float *loss, float *lse, const Problem &q, const Plan 
   a.tokens = static_cast<int32_t>(q.n);
   a.k_blocks = static_cast<int32_t>(Ceil(q.h, kStepK));
   const int64_t m_tiles = Ceil(q.n, 128 * p.ctas);
-  a.group = GroupOf(m_tiles);
+  a.group = GroupOf(m_tiles, 16);
   a.instr = tc5::InstrDesc(q.bf16, false, false, 128 * p.ctas, static_cast<int>(p.tile_n));
   a.tile_n = static_cast<int32_t>(p.tile_n);
   a.pad_rows = p.pad_rows;
@@ -1180,7 +1211,7 @@ inline void BackwardLaunch(const GradOut &g, const Problem &q, const Plan &p, ch
     a.col0 = static_cast<int32_t>(p0);
       a.n_tiles = static_cast<int32_t>(Ceil(cols, kTileN));
     a.k_blocks = static_cast<int32_t>(Ceil(q.h, kStepK));
-    a.group = GroupOf(m_tiles);
+    a.group = GroupOf(m_tiles, 16);
     a.instr = tc5::InstrDesc(q.bf16, false, false, 128 * p.ctas, kTileN);
     const CUtensorMap w_along = WeightMap(q, p, ws, p0, cols, kTileN / p.ctas, stream, true, &a.b_row0);
     Gemm<kDelta>(x_along, w_along, x_along_in_place, d_along, a, m_tiles * a.n_tiles, p.ctas, sms, stream);
@@ -1188,14 +1219,17 @@ inline void BackwardLaunch(const GradOut &g, const Problem &q, const Plan &p, ch
       const CUtensorMap w_across = WeightMap(q, p, ws, p0, cols, 64, stream, false, &a.b_row0);
       const CUtensorMap out = tc5::MatrixMap(acc, kFloat32, static_cast<int64_t>(p.acc_tiles) * 128 * p.ctas_gx, p.ld_acc, p.ld_acc, 128);
       const int64_t x_tiles = Ceil(q.n, 128 * p.ctas_gx);
-      a.n_tiles = h_tiles;
+      a.n_tiles = p.wide_gx ? h_tiles / 2 : h_tiles;
+      a.step_cycles = p.wide_gx ? 1024.0f : p.ctas_gx == 1 ? 560.0f : 512.0f;
+      a.tile_cycles = static_cast<float>(128 * p.ctas_gx * kTileN * (p.wide_gx ? 2 : 1) * 8) / 2400.0f;
       a.k_blocks = static_cast<int32_t>(Ceil(cols, kStepK));
       a.k_plan = static_cast<int32_t>(Ceil(std::min(p.piece, q.v), kStepK));
       a.acc_tiles = p.acc_tiles;
       a.accumulate = p0 > 0;
-      a.group = GroupOf(x_tiles);
+      a.group = GroupOf(x_tiles, 8);
       a.instr = tc5::InstrDesc(q.bf16, false, true, 128 * p.ctas_gx, kTileN);
-      Gemm<kDataGrad>(d_along, w_across, d_along, out, a, x_tiles * a.n_tiles, p.ctas_gx, sms, stream);
+      if (p.wide_gx) LaunchGemm<kDataGrad, 2, true>(d_along, w_across, d_along, out, a, x_tiles * a.n_tiles, sms, stream);
+      else Gemm<kDataGrad>(d_along, w_across, d_along, out, a, x_tiles * a.n_tiles, p.ctas_gx, sms, stream);
     }
     if (g.gw != nullptr) {
       const int64_t elem = g.gw_type == kFloat32 ? 4 : 2;
@@ -1203,7 +1237,7 @@ inline void BackwardLaunch(const GradOut &g, const Problem &q, const Plan &p, ch
       a.m_tiles = static_cast<int32_t>(Ceil(cols, 128 * ctas));
       a.n_tiles = h_tiles;
           a.b_row0 = 0;
-      a.group = GroupOf(a.m_tiles);
+      a.group = GroupOf(a.m_tiles, 8);
       a.instr = tc5::InstrDesc(q.bf16, true, true, 128 * ctas, kTileN);
       a.out = static_cast<char *>(g.gw) + p0 * g.ld_gw * elem;
       a.ld_out = g.ld_gw;
@@ -1216,13 +1250,21 @@ inline void BackwardLaunch(const GradOut &g, const Problem &q, const Plan &p, ch
       // boundary would lose up to 14 bytes behind them to zeros)
       a.out_tiled = a.out_vec && !a.out_add && q.h * elem % 16 == 0;
       const CUtensorMap out = a.out_tiled ? tc5::MatrixMap(a.out, g.gw_type, cols, q.h, g.ld_gw, 128) : x_across;
-      Gemm<kWeightGrad>(d_across, x_across, x_across_in_place, out, a, static_cast<int64_t>(a.m_tiles) * a.n_tiles, ctas, sms, stream);
+      const int64_t tiles = static_cast<int64_t>(a.m_tiles) * h_tiles;
+      if (ctas == 2 && WideFor(tiles, h_tiles, Ceil(q.n, kStepK), sms)) {
+        a.n_tiles = h_tiles / 2;
+        LaunchGemm<kWeightGrad, 2, true>(d_across, x_across, x_across_in_place, out, a, tiles / 2, sms, stream);
+      } else {
+        Gemm<kWeightGrad>(d_across, x_across, x_across_in_place, out, a, tiles, ctas, sms, stream);
+      }
     }
   }
   if (g.gx != nullptr) {
     FinishArgs f = {};
     f.acc = acc, f.ld_acc = p.ld_acc, f.live = a.live;
+    f.n_tiles = p.wide_gx ? h_tiles / 2 : h_tiles;
     f.k_plan = a.k_plan, f.acc_tiles = p.acc_tiles, f.slots = sms / p.ctas_gx, f.ctas = p.ctas_gx;
+    f.step_cycles = a.step_cycles, f.tile_cycles = a.tile_cycles;
     f.pos_of = k.pos_of, f.inv_scale = a.inv_scale;
     f.out = g.gx, f.ld_out = g.ld_gx, f.n = static_cast<int32_t>(q.n), f.h = static_cast<int32_t>(q.h);
     f.bf16 = q.bf16, f.vec = Aligned16(g.gx, g.ld_gx, 2);

@@ -614,6 +614,14 @@ def test_loss_grad_pieces(lib):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,gw_dtype,add", [(BF16, None, False), (F16, F32, True), (BF16, F32, False)])
+def test_loss_grad_long(lib, dtype, gw_dtype, add):
+    """Contractions and tables long enough for the widest tiles, with ends that fill none of them."""
+    x, w, label = problem(8130, 8003, 2500, dtype, 5, ignored=0.05)
+    check_grad(lib, x, w, label, scale=1.0 / 8130, gw_dtype=gw_dtype, add=add)
+
+
+@pytest.mark.gpu
 def test_loss_grad_unaligned_pieces(lib):
     x, w, label = problem(300, 70001, 1001, BF16, 1)
     check_grad(lib, x, w, label, scale=1.0 / 300)
