@@ -24,6 +24,8 @@ TARGETS = [
       os.path.join(HERE, "csrc", "vocab_capi.cu")], []),
     (os.path.join(ROOT, "tests", "cxx", "libmsb_api_suite.so"),
      [os.path.join(ROOT, "tests", "cxx", "api_suite.cu")], []),
+    (os.path.join(ROOT, "tests", "cxx", "libmsb_vocab_suite.so"),
+     [os.path.join(ROOT, "tests", "cxx", "vocab_suite.cu")], []),
     # the checked build of the engine (tensor leaves refuse and record accesses outside their storage)
     (os.path.join(ROOT, "tests", "cxx", "libmsb_bounds_suite.so"),
      [os.path.join(ROOT, "tests", "cxx", "bounds_suite.cu")], ["-DMSHADOW_B200_CHECK_BOUNDS=1"]),

@@ -59,6 +59,38 @@ int CaptureCheck(const char *name, const void *workspace, bool needs_workspace, 
   if (needs_workspace && workspace == nullptr) {
     return Refuse(name, MSB_ERR_ARGUMENT, "a call captured into a graph needs a workspace of the caller's");
   }
+  if (!gpu_rt::StatusWordReady()) {
+    return Refuse(name, MSB_ERR_ARGUMENT, "the first call on a device (or msb_stream_wait) must precede a capture");
+  }
+  return MSB_OK;
+}
+
+/*!
+ * \brief every pointer that is not null names memory of the current device (or managed memory).  A kernel given host
+ *  memory, or memory of a GPU it cannot reach, faults, and takes the process's context with it; asking costs a fraction of a
+ *  microsecond.
+ */
+template <typename... Pointers>
+int PlaceCheck(const char *name, Pointers... pointers) {
+  int dev = 0;
+  cudaError_t err = cudaGetDevice(&dev);
+  if (err != cudaSuccess) return Refuse(name, MSB_ERR_CUDA, std::string("CUDA: ") + cudaGetErrorString(err));
+  const void *all[] = {static_cast<const void *>(pointers)...};
+  for (const void *p : all) {
+    if (p == nullptr) continue;
+    cudaPointerAttributes at;
+    err = cudaPointerGetAttributes(&at, p);
+    if (err != cudaSuccess) {
+      (void)cudaGetLastError();
+      return Refuse(name, MSB_ERR_CUDA, std::string("CUDA: ") + cudaGetErrorString(err));
+    }
+    if (at.type == cudaMemoryTypeManaged) continue;
+    if (at.type != cudaMemoryTypeDevice) return Refuse(name, MSB_ERR_ARGUMENT, "an operand is not device memory");
+    if (at.device != dev) {
+      return Refuse(name, MSB_ERR_ARGUMENT, "an operand is memory of device " + std::to_string(at.device) + " while device " +
+                                                std::to_string(dev) + " is current");
+    }
+  }
   return MSB_OK;
 }
 
@@ -90,6 +122,8 @@ int msb_embed_take(void *dst, const void *table, const int32_t *index, int64_t n
   VOCAB_REQUIRE(dst && index && (table || rows == 0), MSB_ERR_ARGUMENT, "null pointer");
   VOCAB_REQUIRE(ElementAligned(dst, dtype) && ElementAligned(table, dtype), MSB_ERR_LAYOUT,
                 "operands must be aligned to their elements");
+  const int rc = PlaceCheck(__func__, dst, table, index);
+  if (rc != MSB_OK) return rc;
   return Guarded(__func__, [&] {
     Borrowed st(stream);
     const Tensor<gpu, 1, int32_t> idx = Vec<int32_t>(index, n, &st.s);
@@ -129,7 +163,8 @@ int msb_embed_take_grad(void *dst, const void *src, const int32_t *index, int64_
   int rc = msb_embed_take_grad_workspace(n, width, &need);
   if (rc != MSB_OK) return rc;
   VOCAB_REQUIRE(workspace == nullptr || workspace_bytes >= need, MSB_ERR_ARGUMENT, "workspace too small");
-  rc = CaptureCheck(__func__, workspace, need > 0, stream);
+  rc = PlaceCheck(__func__, dst, src, index, workspace);
+  if (rc == MSB_OK) rc = CaptureCheck(__func__, workspace, need > 0, stream);
   if (rc != MSB_OK) return rc;
   return Guarded(__func__, [&] {
     Borrowed st(stream);
@@ -173,7 +208,8 @@ int msb_linear_softmax_loss(float *loss, float *lse, const void *data, const voi
   VOCAB_REQUIRE(loss && lse && data && weight && label, MSB_ERR_ARGUMENT, "null pointer");
   VOCAB_REQUIRE(ElementAligned(data, dtype) && ElementAligned(weight, dtype), MSB_ERR_LAYOUT,
                 "operands must be aligned to their elements");
-  const int rc = CaptureCheck(__func__, workspace, true, stream);
+  int rc = PlaceCheck(__func__, loss, lse, data, weight, label, workspace);
+  if (rc == MSB_OK) rc = CaptureCheck(__func__, workspace, true, stream);
   if (rc != MSB_OK) return rc;
   return Guarded(__func__, [&] {
     Borrowed st(stream);
@@ -210,7 +246,8 @@ int msb_linear_softmax_loss_grad(void *gdata, void *gweight, const void *data, c
   VOCAB_REQUIRE(ElementAligned(data, dtype) && ElementAligned(weight, dtype) && ElementAligned(gdata, dtype) &&
                     ElementAligned(gweight, gweight_dtype),
                 MSB_ERR_LAYOUT, "operands must be aligned to their elements");
-  const int rc = CaptureCheck(__func__, workspace, n > 0, stream);
+  int rc = PlaceCheck(__func__, gdata, gweight, data, weight, label, lse, gloss, workspace);
+  if (rc == MSB_OK) rc = CaptureCheck(__func__, workspace, n > 0, stream);
   if (rc != MSB_OK) return rc;
   return Guarded(__func__, [&] {
     Borrowed st(stream);

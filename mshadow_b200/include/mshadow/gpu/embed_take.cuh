@@ -638,6 +638,8 @@ inline void GradGo(GradArgs<T> a, const GradPlan &p, char *ws, cudaStream_t stre
   const uint32_t threads = std::min(256u, (items + 31) / 32 * 32);
   a.slabs = (items + threads - 1) / threads;
   const uint32_t zero = a.add ? 0 : (a.table_rows + kZeroRows - 1) / kZeroRows;
+  CHECK_LT(static_cast<uint64_t>(p.few ? a.n : p.chunks) * a.slabs + zero, uint64_t(1) << 31)
+      << "EmbedTakeGrad: more indices times columns than one launch covers";
   if (p.few) {
     const uint32_t grid = a.n * a.slabs + zero;
     if (grid == 0) return;

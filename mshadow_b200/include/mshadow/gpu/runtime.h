@@ -266,16 +266,26 @@ inline char *Workspace(void *given, size_t given_bytes, size_t need, cudaStream_
   return reinterpret_cast<char *>((reinterpret_cast<uintptr_t>(given) + 255) / 256 * 256);
 }
 
+namespace rtdetail {
+inline std::mutex &StatusMutex() {
+  static std::mutex mu;
+  return mu;
+}
+inline std::map<int, int *> &StatusWords() {
+  static std::map<int, int *> words;
+  return words;
+}
+}  // namespace rtdetail
+
 /*!
  * \brief one int per device in which a kernel records that a bounded wait gave up
  *  (see gpu/tma.cuh); allocated on first use, lives as long as the process
  */
 inline int *StatusWord() {
-  static std::mutex mu;
-  static std::map<int, int *> words;
   int dev = 0;
   MSHADOW_CUDA_CALL(cudaGetDevice(&dev));
-  std::lock_guard<std::mutex> lock(mu);
+  std::lock_guard<std::mutex> lock(rtdetail::StatusMutex());
+  std::map<int, int *> &words = rtdetail::StatusWords();
   auto it = words.find(dev);
   if (it == words.end()) {
     int *p = nullptr;
@@ -284,6 +294,13 @@ inline int *StatusWord() {
     it = words.insert(std::make_pair(dev, p)).first;
   }
   return it->second;
+}
+/*! \brief the current device has its status word: StatusWord() will not allocate (it must not while a stream is captured) */
+inline bool StatusWordReady() {
+  int dev = 0;
+  MSHADOW_CUDA_CALL(cudaGetDevice(&dev));
+  std::lock_guard<std::mutex> lock(rtdetail::StatusMutex());
+  return rtdetail::StatusWords().count(dev) != 0;
 }
 
 /*!

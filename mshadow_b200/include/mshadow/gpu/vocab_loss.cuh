@@ -673,10 +673,31 @@ struct PackArgs {
   int vec;               // 16-byte copies possible
   int tiled;             // the tiled copies can read x itself: nothing is packed if all its rows count
   int rows_per_cta;
+  float2 *counts;        // [pad_rows / 256] (count as bits, largest |gloss|), or null: the labels are counted directly
 };
 
 __device__ __forceinline__ bool IsLive(int32_t label, int32_t ignore, int32_t v) {
   return label != ignore && label >= 0 && label < v;
+}
+
+/*! \brief live rows, and the largest |gloss| among them, of every 256 tokens: for lists too long to be counted by each CTA below */
+template <int kUnused>
+__global__ void __launch_bounds__(256) CountRowsKernel(const PackArgs a) {
+  gpu_rt::GridDependencySync();
+  __shared__ int s_count[8];
+  __shared__ float s_top[8];
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const bool on = i < a.n && IsLive(a.label[i], a.ignore, a.v);
+  float top = on && a.gloss != nullptr ? fabsf(a.gloss[i]) : 0.0f;
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  const int count = __popc(__ballot_sync(0xffffffffu, on));
+  if ((threadIdx.x & 31) == 0) s_count[threadIdx.x >> 5] = count, s_top[threadIdx.x >> 5] = top;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  int total = 0;
+  top = 0.0f;
+  for (int w = 0; w < 8; ++w) total += s_count[w], top = fmaxf(top, s_top[w]);
+  a.counts[blockIdx.x] = make_float2(__int_as_float(total), top);
 }
 
 /*!
@@ -696,11 +717,20 @@ __global__ void __launch_bounds__(256) PackRowsKernel(const PackArgs a) {
   const int base = blockIdx.x * a.rows_per_cta;
   int before = 0, total = 0;
   float top = 0.0f;
-  for (int i = tid; i < a.n; i += 256) {
-    const int on = IsLive(a.label[i], a.ignore, a.v) ? 1 : 0;
-    total += on;
-    before += i < base ? on : 0;
-    if (a.gloss != nullptr && on) top = fmaxf(top, fabsf(a.gloss[i]));
+  if (a.counts != nullptr) {  // (then rows_per_cta is 256)
+    for (int64_t b = tid; b < a.pad_rows / 256; b += 256) {
+      const float2 c = a.counts[b];
+      total += __float_as_int(c.x);
+      before += b < blockIdx.x ? __float_as_int(c.x) : 0;
+      top = fmaxf(top, c.y);
+    }
+  } else {
+    for (int i = tid; i < a.n; i += 256) {
+      const int on = IsLive(a.label[i], a.ignore, a.v) ? 1 : 0;
+      total += on;
+      before += i < base ? on : 0;
+      if (a.gloss != nullptr && on) top = fmaxf(top, fabsf(a.gloss[i]));
+    }
   }
   for (int o = 16; o > 0; o >>= 1) {
     before += __shfl_xor_sync(0xffffffffu, before, o);
@@ -921,6 +951,7 @@ __global__ void __launch_bounds__(256) DataGradFinishKernel(const FinishArgs a) 
 // ---- host side ------------------------------------------------------------------------------------
 
 const int64_t kDeltaBytes = int64_t(512) << 20;  // piece of d: larger pieces mean fewer passes over the gradient of x
+const int64_t kCountDirectly = 16384;            // tokens up to which each CTA of PackRowsKernel counts all labels itself
 const int64_t kCopyBytes = int64_t(128) << 20;   // piece of W copied to aligned rows where the caller's are not
 
 inline int64_t RoundUp(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
@@ -969,7 +1000,7 @@ struct Plan {
   int64_t pad_rows, ld_x, ld_w, piece, ld_acc, tile_n, tiles;
   int acc_tiles, ctas, ctas_gx;
   bool wide_gx;
-  int64_t words, row_of, pos_of, label_of, lse2, row_scale, x, w, part, part_sum, label_logit, delta, acc, bytes;
+  int64_t counts, words, row_of, pos_of, label_of, lse2, row_scale, x, w, part, part_sum, label_logit, delta, acc, bytes;
 };
 
 /*! \brief layout of a call; sms = multiprocessors of the device */
@@ -1009,6 +1040,7 @@ inline Plan MakePlan(int64_t n, int64_t v, int64_t h, bool gradient, bool want_g
     return was;
   };
   p.words = take(256);
+  p.counts = take(pack && p.pad_rows > kCountDirectly ? p.pad_rows / 256 * 8 : 0);
   p.label_of = take(pack ? p.pad_rows * 4 : 0);
   p.row_of = take(pack && !gradient ? p.pad_rows * 4 : 0);
   p.pos_of = take(gradient ? p.pad_rows * 4 : 0);
@@ -1028,11 +1060,20 @@ inline Plan MakePlan(int64_t n, int64_t v, int64_t h, bool gradient, bool want_g
   return p;
 }
 
+/*! \brief the kernels count tiles in 32 bits */
+inline void CheckExtents(const Problem &q) {
+  CHECK(q.n <= (int64_t(1) << 30) && Ceil(q.n, 128) * Ceil(q.v, 16) < (int64_t(1) << 31) &&
+        Ceil(q.v, 128) * Ceil(q.h, 256) < (int64_t(1) << 31))
+      << "LinearSoftmaxLoss: more tokens times classes than one call covers";
+}
 inline Plan PlanForward(const Problem &q, int sms) {
-  const bool pack = q.n > 256 || !Aligned16(q.x, q.ld_x, 2);
+  CheckExtents(q);
+  // packing costs a launch (some 4 us), and saves whole tiles of rows that do not count: 512 rows are two pairs' worth
+  const bool pack = q.n > 512 || !Aligned16(q.x, q.ld_x, 2);
   return MakePlan(q.n, q.v, q.h, false, false, q.smooth != 0.0f, pack, !Aligned16(q.w, q.ld_w, 2), sms);
 }
 inline Plan PlanBackward(const Problem &q, bool want_gx, int sms) {
+  CheckExtents(q);
   return MakePlan(q.n, q.v, q.h, true, want_gx, q.smooth != 0.0f, true, !Aligned16(q.w, q.ld_w, 2), sms);
 }
 /*! \brief scratch that suffices for every call of these sizes, whatever its layouts and options */
@@ -1111,7 +1152,14 @@ inline void PackLaunch(const Problem &q, const Plan &p, char *ws, PackArgs a, cu
   a.words = reinterpret_cast<int32_t *>(ws + p.words);
   a.label_of = reinterpret_cast<int32_t *>(ws + p.label_of);
   a.vec = a.tiled = Aligned16(q.x, q.ld_x, 2);
-  a.rows_per_cta = p.pad_rows >= 65536 ? 64 : 16;
+  a.rows_per_cta = 16;
+  a.counts = nullptr;
+  if (p.pad_rows > kCountDirectly) {
+    a.rows_per_cta = 256;
+    a.counts = reinterpret_cast<float2 *>(ws + p.counts);
+    gpu_rt::LaunchAfterDrain(CountRowsKernel<0>, dim3(static_cast<unsigned>(p.pad_rows / 256)), dim3(256), 0, stream, a);
+    MSHADOW_CUDA_POST_KERNEL_CHECK(CountRowsKernel);
+  }
   gpu_rt::LaunchAfterDrain(PackRowsKernel<0>, dim3(static_cast<unsigned>(p.pad_rows / a.rows_per_cta)), dim3(256), 0, stream, a);
   MSHADOW_CUDA_POST_KERNEL_CHECK(PackRowsKernel);
 }

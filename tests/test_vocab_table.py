@@ -656,6 +656,46 @@ def test_loss_grad_against_differences(lib):
             assert abs(grad[r, k].item() - diff) <= bound[r, k].item() + 1e-6
 
 
+# ---- the C++ headers ----------------------------------------------------------------------------------------------
+
+def cxx_suite():
+    import os
+    return C.CDLL(os.path.join(os.path.dirname(os.path.abspath(__file__)), "cxx", "libmsb_vocab_suite.so"))
+
+
+def test_bf16_rounding():
+    """The host conversions of bf16_t against torch's, on every bit pattern, every tie, and beyond the range."""
+    bits = np.arange(1 << 16, dtype=np.uint32) << 16
+    near = np.concatenate([bits, bits | 0x8000, bits | 0x7fff, bits | 0x8001]).view(np.float32)
+    got, back = np.empty(near.size, np.uint16), np.empty(near.size, np.float32)
+    vp = lambda a: a.ctypes.data_as(C.c_void_p)  # noqa: E731
+    assert cxx_suite().msb_bf16_round(vp(near), vp(got), vp(back), near.size) == capi.BFLOAT16
+    want = torch.from_numpy(near).to(torch.bfloat16)
+    nan = np.isnan(near)
+    assert np.isnan(back[nan]).all()
+    assert np.array_equal(got[~nan].view(np.int16), want.view(torch.int16).numpy()[~nan])
+    assert np.array_equal(back[~nan], want.float().numpy()[~nan])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_cxx_headers(lib, dtype):
+    """The same step through Tensor handles and through the C entries: the same bits."""
+    n, v, h = 333, 700, 72
+    table, tokens, label, gtable, bufs, ws = tied(lib, n, v, h, dtype, 9)
+    model_step(lib, table, tokens, label, gtable, bufs, ws, None)
+    torch.cuda.synchronize()
+    want = gtable.clone(), bufs[2].clone()
+    gtable.fill_(1)
+    bufs[2].fill_(1)
+    fn = getattr(cxx_suite(), "msb_vocab_step_" + ("f16" if dtype == F16 else "bf16"))
+    fn.argtypes = [C.c_void_p] * 8 + [C.c_int] * 3 + [C.c_float]
+    torch.cuda.synchronize()
+    p = [t.data_ptr() for t in (table, tokens, label, gtable, bufs[0], bufs[1], bufs[2], bufs[3])]
+    assert fn(*p, n, v, h, 1.0 / n) == 0
+    assert torch.equal(gtable, want[0]) and torch.equal(bufs[2], want[1])
+
+
 # ---- streams, graphs, workspaces ----------------------------------------------------------------------------------
 
 def model_step(lib, table, tokens, label, gtable, bufs, workspace, stream):
@@ -787,3 +827,49 @@ def test_workspace_too_small(lib):
     lib.linear_softmax_loss(loss, lse, x, w, label, workspace=ws)
     want, wlse, e_loss, e_lse, _ = loss_oracle(x, w, label, -1, 0.0)
     within(loss, want, e_loss, "loss")
+
+
+@pytest.mark.gpu
+def test_host_memory_is_refused(lib):
+    """Pointers that a kernel could not follow are answered with an error, not with a fault."""
+    d = lambda *shape: torch.zeros(*shape, dtype=BF16, device="cuda")  # noqa: E731
+    i = torch.zeros(4, dtype=torch.int32, device="cuda")
+    f = torch.zeros(4, device="cuda")
+    bad = [lambda: lib.embed_take(d(4, 8), torch.zeros(9, 8, dtype=BF16), i),
+           lambda: lib.embed_take(d(4, 8), d(9, 8), i.cpu()),
+           lambda: lib.embed_take(d(4, 8), torch.zeros(9, 8, dtype=BF16).pin_memory(), i),
+           lambda: lib.embed_take_grad(d(9, 8), torch.zeros(4, 8, dtype=BF16), i),
+           lambda: lib.linear_softmax_loss(f, f.clone(), d(4, 8), torch.zeros(9, 8, dtype=BF16), i),
+           lambda: lib.linear_softmax_loss(f, f.cpu(), d(4, 8), d(9, 8), i),
+           lambda: lib.linear_softmax_loss(f, f.clone(), d(4, 8), d(9, 8), i, workspace=torch.empty(1 << 20, dtype=torch.uint8)),
+           lambda: lib.linear_softmax_loss_grad(d(4, 8), torch.zeros(9, 8, dtype=BF16), d(4, 8), d(9, 8), i, f)]
+    for call in bad:
+        with pytest.raises(capi.MsbError) as e:
+            call()
+        assert e.value.status == 1
+    lib.embed_take(d(4, 8), d(9, 8), i)
+    torch.cuda.synchronize()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [16300, 16500, 70000])
+def test_loss_long_token_lists(lib, n):
+    """Around the length from which the live tokens are counted by a kernel of their own."""
+    x, w, label = problem(n, 300, 24, BF16, 3, ignored=0.4)
+    gloss = torch.randn(n, device="cuda", generator=gen(1))
+    gloss[label < 0] = float("inf")
+    check_loss(lib, x, w, label)
+    check_grad(lib, x, w, label, gloss=gloss, scale=1e-3)
+
+
+@pytest.mark.gpu
+def test_gradient_in_place(lib):
+    """gdata may be data itself: its rows are written after everything has been read."""
+    for n in (40, 700):
+        x, w, label = problem(n, 900, 64, BF16, 13, ignored=0.1)
+        loss, lse = torch.empty(n, device="cuda"), torch.empty(n, device="cuda")
+        lib.linear_softmax_loss(loss, lse, x, w, label)
+        gx, gw, gw2 = torch.empty_like(x), torch.empty_like(w), torch.empty_like(w)
+        lib.linear_softmax_loss_grad(gx, gw, x, w, label, lse)
+        lib.linear_softmax_loss_grad(x, gw2, x, w, label, lse)
+        assert torch.equal(x, gx) and torch.equal(gw, gw2)
