@@ -37,6 +37,7 @@ namespace embtake {
 
 const int kChunk = 64;        // sorted entries per CTA; also the longest run that is not split
 const int kFewTokens = 512;   // lists up to this are not sorted
+const int kOneCta = 16384;    // lists up to this are sorted by one CTA
 const int kDepth = 8;         // source rows in flight per thread
 const uint32_t kManyParts = 32;  // a split run of more chunks than this is shared by a CTA's warps
 const int kZeroRows = 32;     // table rows per CTA that writes zeros
@@ -310,14 +311,111 @@ __device__ __forceinline__ void AddRows(const GradArgs<T> &a, const int32_t *row
 }
 
 /*!
+ * \brief stable sort of the (clipped index, position) pairs of up to kOneCta indices by one CTA of 1024 threads, least
+ *  significant digit first, and the start values of the list of split runs: one launch instead of six and a
+ *  memory set.  The pairs live in shared memory (4 + 2 bytes each); in a pass every warp takes a
+ *  contiguous part of them into registers, counts its digits (ranks within a round of 32 from a
+ *  warp-wide match), and after a scan over warps and digits scatters them back.  Bound by latency: 16384
+ *  pairs in two passes of nine bits MEASURED.
+ *  Dynamic shared memory: SortOneBytes(n, digit_bits).
+ */
+template <int kUnused>
+__global__ void __launch_bounds__(1024)
+EmbedSortKernel(int32_t *keys, int32_t *rows, const int32_t *index, uint32_t n, uint32_t table_rows, int passes, int digit_bits,
+                int32_t *spans) {
+  gpu_rt::GridDependencySync();
+  constexpr int kItems = kOneCta / 1024;
+  extern __shared__ uint32_t s_key[];
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rounds = (n + 1023) / 1024;  // a warp's part: `rounds` times 32 consecutive pairs
+  const uint32_t digits = 1u << digit_bits, mask = digits - 1u;
+  uint16_t *s_val = reinterpret_cast<uint16_t *>(s_key + rounds * 1024);
+  uint16_t *count = s_val + rounds * 1024;             // [32 warps][digits]
+  uint32_t *base = reinterpret_cast<uint32_t *>(count + 32 * digits);  // [digits]
+  __shared__ uint32_t s_sum[32];
+  if (threadIdx.x < 2) spans[threadIdx.x] = 0;
+  for (uint32_t i = threadIdx.x; i < n; i += 1024) {
+    const int32_t k = index[i];
+    const bool named = k >= 0 && static_cast<uint32_t>(k) < table_rows;
+    s_key[i] = named ? static_cast<uint32_t>(k) : 0u;
+    s_val[i] = named ? static_cast<uint16_t>(i) : 0xffffu;  // i < 16384
+  }
+  for (int pass = 0; pass < passes; ++pass) {
+    const int shift = pass * digit_bits;
+    for (uint32_t i = threadIdx.x; i < 16 * digits; i += 1024) reinterpret_cast<uint32_t *>(count)[i] = 0;
+    __syncthreads();
+    uint32_t key[kItems];
+    uint32_t val_rank[kItems];  // value in the upper half, rank among the warp's equal digits in the lower
+    uint16_t *mine = count + warp * digits;
+    const uint32_t first = warp * rounds * 32 + lane;
+#pragma unroll
+    for (int r = 0; r < kItems; ++r) {
+      const uint32_t i = first + r * 32;
+      if (r >= static_cast<int>(rounds)) break;
+      const bool in = i < n;
+      key[r] = in ? s_key[i] : 0u;
+      const uint32_t digit = in ? (key[r] >> shift) & mask : digits;
+      const uint32_t peers = __match_any_sync(0xffffffffu, digit);
+      const uint32_t before = __popc(peers & ((1u << lane) - 1u));
+      const uint32_t seen = in ? mine[digit] : 0u;
+      __syncwarp();
+      if (in && before == 0) mine[digit] = static_cast<uint16_t>(seen + __popc(peers));
+      __syncwarp();
+      val_rank[r] = (in ? static_cast<uint32_t>(s_val[i]) << 16 : 0u) | (seen + before);
+    }
+    __syncthreads();
+    // per digit: the warps' counts become the warps' places within the digit, and their sum the digit's size
+    uint32_t size = 0;
+    if (threadIdx.x < digits) {
+      for (int w = 0; w < 32; ++w) {
+        const uint32_t c = count[w * digits + threadIdx.x];
+        count[w * digits + threadIdx.x] = static_cast<uint16_t>(size);
+        size += c;
+      }
+    }
+    uint32_t incl = size;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t up = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= static_cast<uint32_t>(o)) incl += up;
+    }
+    if (lane == 31) s_sum[warp] = incl;
+    __syncthreads();
+    uint32_t below = 0;
+    for (uint32_t w = 0; w < warp; ++w) below += s_sum[w];
+    if (threadIdx.x < digits) base[threadIdx.x] = below + incl - size;
+    __syncthreads();
+    const bool last = pass == passes - 1;
+#pragma unroll
+    for (int r = 0; r < kItems; ++r) {
+      if (r >= static_cast<int>(rounds)) break;
+      if (first + r * 32 < n) {
+        const uint32_t digit = (key[r] >> shift) & mask;
+        const uint32_t at = base[digit] + mine[digit] + (val_rank[r] & 0xffffu), val = val_rank[r] >> 16;
+        if (last) {
+          keys[at] = static_cast<int32_t>(key[r]);
+          rows[at] = val == 0xffffu ? -1 : static_cast<int32_t>(val);
+        } else {
+          s_key[at] = key[r];
+          s_val[at] = static_cast<uint16_t>(val);
+        }
+      }
+    }
+    __syncthreads();
+  }
+}
+
+/*!
  * \brief sums of the runs of a sorted list, and zeros for the rows that are not in it.
  *  grid: chunks * slabs CTAs that sum, then (when assigning) CTAs that write zeros.
+ *  A thread walks its chunk's entries eight at a time whatever runs they belong to, with the eight source
+ *  rows (and, when adding, the table rows of the runs that end among them) in flight together: with one run
+ *  after the other, 600 tokens of mostly different rows took 48 us.
  */
-template <typename T, bool kVec>
+template <typename T, bool kVec, bool kAdd>
 __global__ void __launch_bounds__(256) EmbedSumKernel(const GradArgs<T> a) {
   gpu_rt::GridDependencySync();
   typedef Group<T, kVec> G;
-  __shared__ int32_t s_keys[3 * kChunk], s_rows[3 * kChunk];
   if (blockIdx.x >= a.chunks * a.slabs) {
     __shared__ uint8_t named[kZeroRows];
     const uint32_t first = (blockIdx.x - a.chunks * a.slabs) * kZeroRows;
@@ -343,67 +441,108 @@ __global__ void __launch_bounds__(256) EmbedSumKernel(const GradArgs<T> a) {
     WriteZeros<T, kVec>(a, first, last, named);
     return;
   }
+  static_assert(kChunk == 64, "the ends of runs are kept in 64-bit words");
+  __shared__ int32_t s_keys[3 * kChunk + 1], s_rows[3 * kChunk];
+  __shared__ uint32_t s_ends[3 * kChunk / 32];
   const uint32_t chunk = blockIdx.x / a.slabs, slab = blockIdx.x - chunk * a.slabs;
   const int64_t begin = static_cast<int64_t>(chunk) * kChunk;
-  // entries [begin - kChunk, begin + 2 kChunk); keys outside the list differ from all others
-  for (uint32_t i = threadIdx.x; i < 3 * kChunk; i += blockDim.x) {
+  // entries [begin - kChunk, begin + 2 kChunk] of the list; keys outside the list differ from all others
+  for (uint32_t i = threadIdx.x; i < 3 * kChunk + 1; i += blockDim.x) {
     const int64_t e = begin - kChunk + i;
     const bool in = e >= 0 && e < a.n;
     s_keys[i] = in ? a.keys[e] : -1;
-    s_rows[i] = in ? a.rows[e] : -1;
+    if (i < 3 * kChunk) s_rows[i] = in ? a.rows[e] : -1;
   }
   __syncthreads();
+  for (uint32_t i = threadIdx.x; i < 3 * kChunk; i += blockDim.x) {
+    const uint32_t ends = __ballot_sync(0xffffffffu, s_keys[i] != s_keys[i + 1]);  // (blocks are whole warps, 192 too)
+    if ((i & 31) == 0) s_ends[i / 32] = ends;
+  }
+  __syncthreads();
+  // bit p of `ends` of chunk c of the window: a run ends with entry p
+  uint64_t ends[3];
+#pragma unroll
+  for (int c = 0; c < 3; ++c) ends[c] = s_ends[2 * c] | static_cast<uint64_t>(s_ends[2 * c + 1]) << 32;
+  // (all below in positions of the chunk: entry 0 is list entry `begin`)
+  const int count = static_cast<int>(min(static_cast<int64_t>(kChunk), a.n - begin));
+  auto end_of = [&](int p) -> int {  // one past the end of the run of entry p, 0 <= p; kChunk * 2 if further
+    const uint64_t here = p < 64 ? ends[1] >> p : 0;
+    if (here != 0) return p + __ffsll(static_cast<long long>(here));
+    return ends[2] != 0 ? 64 + __ffsll(static_cast<long long>(ends[2])) : 128;
+  };
+  int from = 0, head = 0;  // entries before `head` belong to a split run that began in an earlier chunk
+  if (!(ends[0] >> 63)) {
+    // the first run began in an earlier chunk: that chunk adds it up, unless it is longer than a chunk
+    const int start = ends[0] == 0 ? -64 : -static_cast<int>(__clzll(static_cast<long long>(ends[0])));
+    const int stop = end_of(0);
+    if (ends[0] == 0 || stop - start > kChunk) head = min(stop, count);
+    else from = min(stop, count);
+  }
+  // the last run, if it is not the first one: followed past the chunk's end, unless it is longer than a chunk
+  int to = count;
+  bool tail = false;
+  const int begun = from > head ? from : head;  // runs from here on begin in this chunk
+  if (begun < count) {
+    const uint64_t before = count >= 2 ? ends[1] & ((uint64_t(1) << (count - 1)) - 1) : 0;  // ends before the last entry
+    int last = before == 0 ? 0 : 64 - __clzll(static_cast<long long>(before));
+    if (last < begun) last = begun;
+    const int stop = end_of(count - 1);
+    tail = stop - last > kChunk;
+    if (!tail) to = stop;
+  }
   const uint32_t col = (slab * blockDim.x + threadIdx.x) * G::kLanes;
-  const bool active = col < a.width;
-  const bool lead = slab == 0 && threadIdx.x == 0;
-  const uint32_t lo = kChunk;
-  const uint32_t hi = kChunk + static_cast<uint32_t>(min(static_cast<int64_t>(kChunk), a.n - begin));
-  uint32_t at = lo;
-  const int32_t before = s_keys[lo - 1];
-  if (before == s_keys[lo]) {
-    // the first run began in an earlier chunk
-    uint32_t start = lo, stop = lo;
-    while (start > 0 && s_keys[start - 1] == before) --start;
-    while (stop < hi && s_keys[stop] == before) ++stop;
-    const bool split = start == 0 || s_keys[start + kChunk] == before;
-    if (split && active) {
-      float acc[G::kLanes];
+  if (tail && slab == 0 && threadIdx.x < 32) {
+    const uint32_t last = (WarpLowerBound(a.keys, a.n, s_keys[kChunk + count - 1] + 1) - 1) / kChunk;  // key < rows <= 2^31 - 1
+    if (threadIdx.x == 0) {
+      const bool many = last - chunk >= kManyParts;
+      const uint32_t place = static_cast<uint32_t>(atomicAdd(a.spans + (many ? 1 : 0), 1));
+      int2 *list = reinterpret_cast<int2 *>(a.spans + 2);
+      list[many ? a.chunks - 1 - place : place] = make_int2(static_cast<int>(chunk), static_cast<int>(last));
+    }
+  }
+  if (col >= a.width) return;
+  float acc[G::kLanes];
+#pragma unroll
+  for (int l = 0; l < G::kLanes; ++l) acc[l] = -0.0f;  // the sum of nothing: adding it changes no value
+  for (int i = from; i < to; i += kDepth) {
+    Bits<T, kVec> b[kDepth], d[kAdd ? kDepth : 1];
+    int32_t r[kDepth];
+    uint32_t stops = 0;  // bit u: a run ends with entry i + u
+#pragma unroll
+    for (int u = 0; u < kDepth; ++u) {
+      const int p = i + u;
+      r[u] = p < to ? s_rows[kChunk + p] : -1;
+      if (r[u] >= 0) LoadStream(a.g + r[u] * a.ld_g + col, &b[u]);
+      const bool stop = p < to && (p == to - 1 || ((p < 64 ? ends[1] >> p : ends[2] >> (p - 64)) & 1u));
+      if (stop) stops |= 1u << u;
+      if (kAdd && stop && p >= head && !(tail && p == to - 1)) {
+        Load(a.grad + s_keys[kChunk + p] * a.ld_grad + col, &d[kAdd ? u : 0]);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kDepth; ++u) {
+      const int p = i + u;
+      float v[G::kLanes];
+      if (r[u] >= 0) {
+        Unpack<T, kVec>(b[u], v);
+#pragma unroll
+        for (int l = 0; l < G::kLanes; ++l) acc[l] = __fadd_rn(acc[l], v[l]);
+      }
+      if (!(stops >> u & 1u)) continue;
+      if (p < head || (tail && p == to - 1)) {
+        float *part = a.parts + (2 * static_cast<int64_t>(chunk) + (p < head ? 0 : 1)) * a.ld_parts + col;
+#pragma unroll
+        for (int l = 0; l < G::kLanes; ++l) part[l] = acc[l];
+      } else {
+        if (kAdd) Unpack<T, kVec>(d[kAdd ? u : 0], v);
+#pragma unroll
+        for (int l = 0; l < G::kLanes; ++l) v[l] = __fadd_rn(__fmul_rn(a.scale, acc[l]), kAdd ? v[l] : 0.0f);
+        Pack<T, kVec>(v, &b[u]);
+        Store(a.grad + s_keys[kChunk + p] * a.ld_grad + col, b[u]);
+      }
 #pragma unroll
       for (int l = 0; l < G::kLanes; ++l) acc[l] = -0.0f;
-      AddRows<T, kVec>(a, s_rows, lo, stop, col, acc);
-#pragma unroll
-      for (int l = 0; l < G::kLanes; ++l) a.parts[2 * chunk * a.ld_parts + col + l] = acc[l];
     }
-    at = stop;
-  }
-  while (at < hi) {
-    const int32_t key = s_keys[at];
-    uint32_t stop = at + 1;
-    while (stop < 3 * kChunk && s_keys[stop] == key) ++stop;
-    const bool split = stop - at > kChunk;
-    if (split) stop = hi;  // a longer run leaves this chunk's part only
-    if (active) {
-      float acc[G::kLanes];
-#pragma unroll
-      for (int l = 0; l < G::kLanes; ++l) acc[l] = -0.0f;  // the sum of nothing: adding it changes no value
-      AddRows<T, kVec>(a, s_rows, at, stop, col, acc);
-      if (split) {
-#pragma unroll
-        for (int l = 0; l < G::kLanes; ++l) a.parts[(2 * chunk + 1) * a.ld_parts + col + l] = acc[l];
-      } else {
-        WriteRow<T, kVec>(a, key, col, acc);
-      }
-    }
-    if (split && slab == 0 && threadIdx.x < 32) {
-      const uint32_t last = (WarpLowerBound(a.keys, a.n, key + 1) - 1) / kChunk;  // key < rows <= 2^31 - 1
-      if (lead) {
-        const bool many = last - chunk >= kManyParts;
-        const uint32_t place = static_cast<uint32_t>(atomicAdd(a.spans + (many ? 1 : 0), 1));
-        int2 *list = reinterpret_cast<int2 *>(a.spans + 2);
-        list[many ? a.chunks - 1 - place : place] = make_int2(static_cast<int>(chunk), static_cast<int>(last));
-      }
-    }
-    at = stop;
   }
 }
 
@@ -651,16 +790,30 @@ inline void GradGo(GradArgs<T> a, const GradPlan &p, char *ws, cudaStream_t stre
   int bits = 1;
   while (bits < 31 && (int64_t(1) << bits) < a.table_rows) ++bits;
   a.spans = reinterpret_cast<int32_t *>(ws + p.spans);
-  MSHADOW_CUDA_CALL(cudaMemsetAsync(a.spans, 0, 8, stream));
-  const sortdetail::Source named = {static_cast<int>(a.table_rows), 1};
-  // (Writing the zeros by further CTAs of the sort's launches instead was slower: 186 against 165 us for 16384 indices
-  // into 131072 x 2048 bf16 -- writes alone run at 3.9 TB/s however they are issued, and each of the six launches
-  // drained its share of them before the next began.)
-  sortdetail::SortPairs<int32_t, int32_t>(keys, rows, a.index, a.n, bits, true, named, ws + p.sort, stream);
+  if (a.n <= static_cast<uint32_t>(kOneCta)) {
+    const int passes = (bits + 8) / 9, digit_bits = (bits + passes - 1) / passes;
+    const size_t pairs = (a.n + 1023) / 1024 * 1024, digits = size_t(1) << digit_bits;
+    const size_t smem = pairs * 6 + digits * (32 * 2 + 4), most = size_t(kOneCta) * 6 + 512 * (32 * 2 + 4);
+    gpu_rt::AllowSharedMemory(EmbedSortKernel<0>, most);
+    gpu_rt::LaunchAfterDrain(EmbedSortKernel<0>, dim3(1), dim3(1024), smem, stream, keys, rows, a.index, a.n, a.table_rows, passes,
+                             digit_bits, a.spans);
+    MSHADOW_CUDA_POST_KERNEL_CHECK(EmbedSortKernel);
+  } else {
+    // (Writing the zeros by further CTAs of the sort's launches instead was slower: 186 against 165 us for 16384 indices
+    // into 131072 x 2048 bf16 -- writes alone run at 3.9 TB/s however they are issued, and each of the six launches
+    // drained its share of them before the next began.)
+    MSHADOW_CUDA_CALL(cudaMemsetAsync(a.spans, 0, 8, stream));
+    const sortdetail::Source named = {static_cast<int>(a.table_rows), 1};
+    sortdetail::SortPairs<int32_t, int32_t>(keys, rows, a.index, a.n, bits, true, named, ws + p.sort, stream);
+  }
   a.keys = keys, a.rows = rows;
   a.chunks = p.chunks;
   a.parts = reinterpret_cast<float *>(ws + p.parts), a.ld_parts = p.ld_parts;
-  gpu_rt::LaunchAfterDrain(EmbedSumKernel<T, kVec>, dim3(a.chunks * a.slabs + zero), dim3(threads), 0, stream, a);
+  if (a.add) {
+    gpu_rt::LaunchAfterDrain(EmbedSumKernel<T, kVec, true>, dim3(a.chunks * a.slabs), dim3(threads), 0, stream, a);
+  } else {
+    gpu_rt::LaunchAfterDrain(EmbedSumKernel<T, kVec, false>, dim3(a.chunks * a.slabs + zero), dim3(threads), 0, stream, a);
+  }
   MSHADOW_CUDA_POST_KERNEL_CHECK(EmbedSumKernel);
   const int64_t most = static_cast<int64_t>(p.chunks) * ((a.width + 127) / 128);
   const int64_t cap = static_cast<int64_t>(gpu_rt::CurrentDevice().sm_count) * 4;

@@ -52,7 +52,7 @@ const int kTileN = 256;       // columns of a tile
 const int kStepK = 64;        // contraction elements per stage (one 128-byte swizzle row)
 const int kThreads = 384;     // warp 0: copies, warp 1: products, warp 2: tensor memory, warps 4-11: epilogue
 const int kHalfN = kTileN / 2;  // columns of a tile that one epilogue group (four warps, a thread per row) takes
-const int kChunkSteps = 16;   // kStat: stages per run of accumulation in tensor memory (1024 contraction elements)
+const int kChunkSteps = 8;    // kStat: stages per run of accumulation in tensor memory (512 contraction elements)
 const uint32_t kBoxOut = 128 * 128;  // a box of 128 rows by 128 bytes, on its way out through shared memory
 const int kPadRows = 256;     // token rows of the scratch matrices are padded to this
 const float kLog2e = 1.4426950408889634f;
@@ -414,9 +414,10 @@ __device__ __forceinline__ void WeightColumns(const uint32_t (&r)[32], int64_t r
  *
  *  Tensor memory holds two sets of accumulators; the products of one run into them while the epilogue empties the
  *  other.  A set is a whole tile, except in kStat: there the contraction is cut into runs of at most
- *  1024 elements, which the epilogue adds up in registers.  The tensor cores cut off, rather than
+ *  512 elements, which the epilogue adds up in registers.  The tensor cores cut off, rather than
  *  round, each time they add to an accumulator, always towards zero: over 4096 elements that moved
- *  the loss by 1.8e-6 of its value, against 6e-7 for a product in plain binary32.
+ *  the loss by 1.8e-6 of its value, against 6e-7 for a product in plain binary32 and for the runs (whose
+ *  additions cost 1 to 2 % of the time where power is the limit).
  *
  *  kWide: both sets belong to one tile.  A step's rows of A then serve 512 columns, a quarter less is read from the L2
  *  and, where A is d', from memory; in return the products wait while a tile is emptied.  For the gradients

@@ -257,6 +257,23 @@ def test_embed_take_grad(lib, dtype, add, n, rows, width, pad, offset, kind):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n", [1023, 1025, 16383, 16384, 16385])
+@pytest.mark.parametrize("rows", [2, 500, 70000, 1500000])
+def test_embed_take_grad_list_lengths(lib, n, rows):
+    """Around the lengths where the way of sorting changes, with one to three digits per row number."""
+    g = gen(n + rows)
+    src = torch.randn(n, 8, device="cuda", generator=g)
+    index = zipf(n, rows, g)
+    index = torch.randperm(rows, device="cuda", generator=g).to(torch.int32)[index.long()]
+    index[::11] = -1
+    index[5::13] = rows
+    dst = torch.empty(rows, 8, device="cuda")
+    want, bound = grad_oracle(dst, src, index, 1.0, False)
+    lib.embed_take_grad(dst, src, index)
+    within(dst, want, bound, "take_grad")
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_embed_take_grad_no_indices(lib, dtype):
     dst = torch.ones(300, 24, dtype=dtype, device="cuda")
