@@ -37,7 +37,7 @@ namespace embtake {
 
 const int kChunk = 64;        // sorted entries per CTA; also the longest run that is not split
 const int kFewTokens = 512;   // lists up to this are not sorted
-const int kOneCta = 16384;    // lists up to this are sorted by one CTA
+const int kOneCta = 8192;     // lists up to this are sorted by one CTA
 const int kDepth = 8;         // source rows in flight per thread
 const uint32_t kManyParts = 32;  // a split run of more chunks than this is shared by a CTA's warps
 const int kZeroRows = 32;     // table rows per CTA that writes zeros
@@ -315,8 +315,9 @@ __device__ __forceinline__ void AddRows(const GradArgs<T> &a, const int32_t *row
  *  significant digit first, and the start values of the list of split runs: one launch instead of six and a
  *  memory set.  The pairs live in shared memory (4 + 2 bytes each); in a pass every warp takes a
  *  contiguous part of them into registers, counts its digits (ranks within a round of 32 from a
- *  warp-wide match), and after a scan over warps and digits scatters them back.  Bound by latency: 16384
- *  pairs in two passes of nine bits MEASURED.
+ *  warp-wide match), and after a scan over warps and digits scatters them back.  Bound by latency: two passes
+ *  of eight bits take 5 us for 1024 pairs and 22 us for 8192, where the many-CTA sort takes 25 us in six
+ *  launches, whose issue alone costs the host 15 us more.
  *  Dynamic shared memory: SortOneBytes(n, digit_bits).
  */
 template <int kUnused>
