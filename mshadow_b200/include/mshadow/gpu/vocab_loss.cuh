@@ -52,7 +52,7 @@ const int kTileN = 256;       // columns of a tile
 const int kStepK = 64;        // contraction elements per stage (one 128-byte swizzle row)
 const int kThreads = 384;     // warp 0: copies, warp 1: products, warp 2: tensor memory, warps 4-11: epilogue
 const int kHalfN = kTileN / 2;  // columns of a tile that one epilogue group (four warps, a thread per row) takes
-const int kChunkSteps = 8;    // kStat: stages per run of accumulation in tensor memory (512 contraction elements)
+const int kChunkSteps = 16;   // kStat: stages per run of accumulation in tensor memory (1024 contraction elements)
 const uint32_t kBoxOut = 128 * 128;  // a box of 128 rows by 128 bytes, on its way out through shared memory
 const int kPadRows = 256;     // token rows of the scratch matrices are padded to this
 const float kLog2e = 1.4426950408889634f;
@@ -92,8 +92,8 @@ struct GemmArgs {
   int32_t n_tiles;
   int32_t k_blocks;      // kWeightGrad: from the live rows
   int32_t k_plan;        // kDataGrad: k_blocks of the first piece, by which all pieces are cut into the same parts
-  int32_t acc_tiles;     // kDataGrad: row tiles that the partial gradients have room for
-  float step_cycles, tile_cycles;  // kDataGrad: what PartsOf counts
+  int32_t room;          // kDataGrad: tiles that there is room for beside the gradient itself, for parts of tiles
+  float step_cycles, tile_cycles;  // kDataGrad: what CutOf counts
   int32_t group;         // row tiles that are walked before the next column tile
   int32_t b_row0;        // first row of B (the piece's first vocabulary row)
   uint32_t instr;
@@ -143,45 +143,61 @@ __device__ __forceinline__ float Widen(uint16_t bits, int bf16) {
   return bf16 ? __uint_as_float(static_cast<uint32_t>(bits) << 16) : __half2float(__ushort_as_half(bits));
 }
 
-/*! \brief one tile of the walk */
+/*! \brief a piece of work: tile (m, n), part `slice` of `parts` of its contraction; `spare`: its place beside the gradient */
 struct Unit {
-  int m, n, slice;
+  int m, n, slice, parts, spare;
 };
 
 /*!
- * \brief parts into which the contraction of grad x is cut, the same in every thread of a warp that asks.  n x h has few
- *  tiles and a contraction as long as the vocabulary piece: the cheapest of 1 .. 16 parts by this count
- *  -- rounds of tiles over the `slots` of the GPU, step_cycles a step, some 4000 to begin and end a tile,
- *  and tile_cycles to write a part of a tile and read it again -- among those of at least eight steps
- *  for which there is room.  Decided on the device, by the tokens that count.
+ * \brief how the walk over `tiles` tiles is cut: the first `full` of them whole, whole rounds over the GPU, and the
+ *  `rest`, which would leave part of it idle for a round, in `parts` parts of their contraction each
  */
-__device__ __forceinline__ int PartsOf(int m_tiles, int n_tiles, int k_blocks, int room, int slots, float step_cycles,
-                                       float tile_cycles) {
-  const int parts = (threadIdx.x & 15) + 1;
+struct Cut {
+  int full, rest, parts;
+  __device__ __forceinline__ int Units() const { return full + rest * parts; }
+};
+
+/*!
+ * \brief the cut for grad x, the same in every thread of a warp that asks.  n x h has few tiles and a contraction as long
+ *  as the vocabulary piece.  Of 1 .. 16 parts, at least eight steps long and as many as there is room for,
+ *  the cheapest by this count: rounds over the `slots` of the GPU, step_cycles a step, some 4000 to begin and
+ *  end a part, and tile_cycles to write a part of a tile and read it again.  Decided on the device, by the
+ *  tokens that count.
+ */
+__device__ __forceinline__ Cut CutOf(int m_tiles, int n_tiles, int k_blocks, int room, int slots, float step_cycles,
+                                     float tile_cycles) {
+  Cut cut;
   const int tiles = m_tiles * n_tiles;
-  const bool fits = parts == 1 || (parts * 8 <= k_blocks && parts * m_tiles <= room);
-  const float rounds = static_cast<float>((tiles * parts + slots - 1) / slots);
+  cut.full = tiles / slots * slots;
+  cut.rest = tiles - cut.full;
+  const int parts = (threadIdx.x & 15) + 1;
+  const bool fits = parts == 1 || (parts * 8 <= k_blocks && parts * cut.rest <= room);
+  const float rounds = static_cast<float>((cut.rest * parts + slots - 1) / slots);
   const float steps = static_cast<float>((k_blocks + parts - 1) / parts);
   // (each operation rounded by itself: the two kernels that ask must not differ by how theirs is compiled)
   float cost = __fadd_rn(__fmul_rn(rounds, __fadd_rn(__fmul_rn(steps, step_cycles), 4000.0f)),
-                         __fmul_rn(static_cast<float>(parts * tiles), tile_cycles));
+                         __fmul_rn(static_cast<float>(parts * cut.rest), tile_cycles));
   if (!fits) cost = INFINITY;
-  int best = parts;
+  cut.parts = parts;
 #pragma unroll
   for (int o = 8; o > 0; o >>= 1) {
     const float other = __shfl_xor_sync(0xffffffffu, cost, o);
-    const int which = __shfl_xor_sync(0xffffffffu, best, o);
-    if (other < cost || (other == cost && which < best)) cost = other, best = which;
+    const int which = __shfl_xor_sync(0xffffffffu, cut.parts, o);
+    if (other < cost || (other == cost && which < cut.parts)) cost = other, cut.parts = which;
   }
-  return best;
+  return cut;
 }
 
-/*! \brief unit u of the walk: `group` row tiles by all column tiles, then the next group; slices outermost */
-__device__ __forceinline__ Unit UnitOf(int u, int m_tiles, int n_tiles, int group) {
-  Unit t;
-  const int plane = m_tiles * n_tiles;
-  t.slice = u / plane;
-  const int r = u - t.slice * plane;
+/*! \brief work w of the walk: `group` row tiles by all column tiles, then the next group; parts outermost */
+__device__ __forceinline__ Unit UnitOf(int w, const Cut &cut, int m_tiles, int n_tiles, int group) {
+  Unit t = {0, 0, 0, 1, 0};
+  int r = w;
+  if (w >= cut.full) {
+    t.parts = cut.parts;
+    t.slice = (w - cut.full) / cut.rest;
+    r = w - t.slice * cut.rest;
+    t.spare = (r - cut.full) * cut.parts + t.slice;
+  }
   const int band = group * n_tiles;
   const int g = r / band;
   const int first = g * group;
@@ -190,6 +206,11 @@ __device__ __forceinline__ Unit UnitOf(int u, int m_tiles, int n_tiles, int grou
   t.n = q / height;
   t.m = first + (q - t.n * height);
   return t;
+}
+/*! \brief place of tile (m, n) in that walk */
+__device__ __forceinline__ int PlaceOf(int m, int n, int m_tiles, int n_tiles, int group) {
+  const int first = m / group * group;
+  return first * n_tiles + n * min(group, m_tiles - first) + (m - first);
 }
 
 // ---- epilogues: one thread per row of the tile and half of its columns ----------------------------
@@ -308,7 +329,7 @@ __device__ __forceinline__ void DeltaHalf(const Half &t, int limit, int label, f
 
 /*! \brief the half tile as binary32, times `factor`, stored or added */
 template <bool kAdd>
-__device__ __forceinline__ void FloatHalf(const Half &t, float factor, const CUtensorMap *map, int row0, int row1) {
+__device__ __forceinline__ void FloatHalf(const Half &t, float factor, const CUtensorMap *map, int x, int y) {
 #pragma unroll 1
   for (int b = 0; b < kHalfN / 32; ++b) {
     uint32_t r[32];
@@ -319,7 +340,7 @@ __device__ __forceinline__ void FloatHalf(const Half &t, float factor, const CUt
     BoxFree(t);
 #pragma unroll
     for (int q = 0; q < 8; ++q) BoxPut(t, q, r[4 * q], r[4 * q + 1], r[4 * q + 2], r[4 * q + 3]);
-    BoxSend<kAdd>(t, map, t.col + b * 32, row0 + row1);
+    BoxSend<kAdd>(t, map, x + b * 32, y);
   }
 }
 
@@ -414,10 +435,10 @@ __device__ __forceinline__ void WeightColumns(const uint32_t (&r)[32], int64_t r
  *
  *  Tensor memory holds two sets of accumulators; the products of one run into them while the epilogue empties the
  *  other.  A set is a whole tile, except in kStat: there the contraction is cut into runs of at most
- *  512 elements, which the epilogue adds up in registers.  The tensor cores cut off, rather than
+ *  1024 elements, which the epilogue adds up in registers.  The tensor cores cut off, rather than
  *  round, each time they add to an accumulator, always towards zero: over 4096 elements that moved
- *  the loss by 1.8e-6 of its value, against 6e-7 for a product in plain binary32 and for the runs (whose
- *  additions cost 1 to 2 % of the time where power is the limit).
+ *  the loss by 1.8e-6 of its value, against 6e-7 for a product in plain binary32 and 4e-7 for these runs, which
+ *  cost 1 % of the time (runs of 512: 2.5e-7 and another 3 %; of 256: 17 %).
  *
  *  kWide: both sets belong to one tile.  A step's rows of A then serve 512 columns, a quarter less is read from the L2
  *  and, where A is d', from memory; in return the products wait while a tile is emptied.  For the gradients
@@ -427,6 +448,7 @@ template <int kMode, int kCtas, bool kWide>
 __global__ void __launch_bounds__(kThreads, 1)
 VocabGemmKernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                 const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_out, const GemmArgs a) {
+  // map_x: the rows of x where the caller has them; kDataGrad: the parts of tiles beside the gradient
   typedef StageShape<kCtas, kWide> S;
   typedef Layout<kMode> L;
   extern __shared__ uint8_t raw[];
@@ -447,7 +469,7 @@ VocabGemmKernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
     }
     tc5::PrefetchMap(&map_a);
     tc5::PrefetchMap(&map_b);
-    if (kMode != kDataGrad) tc5::PrefetchMap(&map_x);
+    tc5::PrefetchMap(&map_x);
     if (kMode != kStat) tc5::PrefetchMap(&map_out);
   }
   if (warp == 2) tc5::AllocTensorMemory<kCtas>(&tmem_slot);
@@ -471,11 +493,10 @@ VocabGemmKernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                       : kMode == kDelta    ? max(1, (live + tile_m - 1) / tile_m)
                                            : (live + tile_m - 1) / tile_m;
   const int k_blocks = kMode == kWeightGrad ? max(1, (live + kStepK - 1) / kStepK) : a.k_blocks;
-  const int slices = kMode != kDataGrad ? 1
-                                        : min(k_blocks, PartsOf(max(m_tiles, 1), a.n_tiles, a.k_plan, a.acc_tiles,
-                                                                gridDim.x / kCtas, a.step_cycles, a.tile_cycles));
+  Cut cut = {m_tiles * a.n_tiles, 0, 1};
+  if (kMode == kDataGrad) cut = CutOf(m_tiles, a.n_tiles, a.k_plan, a.room, gridDim.x / kCtas, a.step_cycles, a.tile_cycles);
   const int runs = kMode == kStat ? (k_blocks + kChunkSteps - 1) / kChunkSteps : 1;
-  const int units = m_tiles * a.n_tiles * slices;
+  const int units = cut.Units();
   const int first = blockIdx.x / kCtas, step = gridDim.x / kCtas;
 
   if (warp < 4) {
@@ -483,8 +504,8 @@ VocabGemmKernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
       uint32_t fill = 0;  // stages filled so far
       bool ok = true;
       for (int w = first; ok && w < units; w += step) {
-        const Unit u = UnitOf(w, m_tiles, a.n_tiles, a.group);
-        const int k_begin = u.slice * k_blocks / slices, k_end = (u.slice + 1) * k_blocks / slices;
+        const Unit u = UnitOf(w, cut, m_tiles, a.n_tiles, a.group);
+        const int k_begin = u.slice * k_blocks / u.parts, k_end = (u.slice + 1) * k_blocks / u.parts;
         const int m0 = u.m * tile_m + static_cast<int>(rank) * 128;
         const int n0 = u.n * tile_n + static_cast<int>(rank) * rows_n;
         for (int kb = k_begin; kb < k_end; ++kb, ++fill) {
@@ -525,8 +546,9 @@ VocabGemmKernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
       uint32_t fill = 0, turn = 0;
       bool ok = true;
       for (int w = first; ok && w < units; w += step) {
-        const int slice = w / (m_tiles * a.n_tiles);
-        const int k_first = slice * k_blocks / slices, k_count = (slice + 1) * k_blocks / slices - k_first;
+        const Unit u = UnitOf(w, cut, m_tiles, a.n_tiles, a.group);
+        const int k_first = u.slice * k_blocks / u.parts, k_count = (u.slice + 1) * k_blocks / u.parts - k_first;
+        if (k_count == 0) continue;  // the last piece of the vocabulary may have fewer steps than there are parts
         for (int run = 0; ok && run < runs; ++run, turn += S::kSets) {
           const int k_begin = k_first + run * k_count / runs, k_end = k_first + (run + 1) * k_count / runs;
           for (int kb = k_begin; ok && kb < k_end; ++kb, ++fill) {
@@ -582,7 +604,8 @@ VocabGemmKernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
       ++turn;
     };
     for (int w = first; w < units; w += step) {
-      const Unit u = UnitOf(w, m_tiles, a.n_tiles, a.group);
+      const Unit u = UnitOf(w, cut, m_tiles, a.n_tiles, a.group);
+      if (kMode == kDataGrad && u.slice * k_blocks / u.parts == (u.slice + 1) * k_blocks / u.parts) continue;
       const int row0 = u.m * tile_m + static_cast<int>(rank) * 128;
       t.row = row0 + t.thread;
       t.col = u.n * tile_n + t.group * kHalfN;
@@ -618,13 +641,17 @@ VocabGemmKernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
       for (int set = 0; set < S::kSets; ++set, t.col += kTileN) {
         if (!ready()) break;
         if (kMode == kDataGrad) {
-          const int part = u.slice * m_tiles * tile_m;
-          if (a.accumulate) FloatHalf<true>(t, 1.0f, &map_out, row0, part);
-          else FloatHalf<false>(t, 1.0f, &map_out, row0, part);
+          // a whole tile goes to its place in the gradient, a part of one to a tile of its own beside it
+          const bool whole = u.parts == 1;
+          const CUtensorMap *to = whole ? &map_out : &map_x;
+          const int x = whole ? t.col : t.group * kHalfN + set * kTileN;
+          const int y = whole ? row0 : u.spare * tile_m + static_cast<int>(rank) * 128;
+          if (a.accumulate) FloatHalf<true>(t, 1.0f, to, x, y);
+          else FloatHalf<false>(t, 1.0f, to, x, y);
         } else {
           const float inv = a.inv_scale[0];
           if (a.out_tiled) {
-            if (a.out_type == kFloat32) FloatHalf<false>(t, inv, &map_out, row0, 0);
+            if (a.out_type == kFloat32) FloatHalf<false>(t, inv, &map_out, t.col, row0);
             else PackedHalf(t, inv, a.out_type == kBfloat16, &map_out, row0);
           } else {
 #pragma unroll 1
@@ -895,10 +922,10 @@ __global__ void __launch_bounds__(512) JoinTilesKernel(const JoinArgs a) {
 }
 
 struct FinishArgs {
-  const float *acc;
+  const float *acc, *spare;
   int64_t ld_acc;
   const int32_t *live;
-  int n_tiles, k_plan, acc_tiles, slots, ctas;  // of the kernel that wrote the parts
+  int n_tiles, tile_n, group, k_plan, room, slots, ctas;  // of the kernel that wrote the parts
   float step_cycles, tile_cycles;
   const int32_t *pos_of;
   const float *inv_scale;
@@ -915,16 +942,24 @@ __global__ void __launch_bounds__(256) DataGradFinishKernel(const FinishArgs a) 
   const float inv = a.inv_scale[0];
   const int groups = (a.h + 7) / 8;
   const int tile_m = 128 * a.ctas, m_tiles = (a.live[0] + tile_m - 1) / tile_m;
-  const int slices = PartsOf(max(m_tiles, 1), a.n_tiles, a.k_plan, a.acc_tiles, a.slots, a.step_cycles, a.tile_cycles);
-  const int64_t stride = static_cast<int64_t>(m_tiles) * tile_m * a.ld_acc;
+  const Cut cut = CutOf(m_tiles, a.n_tiles, a.k_plan, a.room, a.slots, a.step_cycles, a.tile_cycles);
   for (int64_t i = blockIdx.x; i < a.n; i += gridDim.x) {
     const int pos = a.pos_of[i];
     uint16_t *out = a.out + i * a.ld_out;
     for (int g = threadIdx.x; g < groups; g += 256) {
       float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
       if (pos >= 0) {
-        for (int s = 0; s < slices; ++s) {
-          const float4 *p = reinterpret_cast<const float4 *>(a.acc + s * stride + pos * a.ld_acc) + 2 * g;
+        const int m = pos / tile_m, n = 8 * g / a.tile_n;
+        const int place = PlaceOf(m, n, m_tiles, a.n_tiles, a.group) - cut.full;
+        const bool whole = place < 0 || cut.parts == 1;
+        const float *from = a.acc + pos * a.ld_acc + 8 * g;
+        int64_t stride = 0;
+        if (!whole) {
+          stride = static_cast<int64_t>(tile_m) * a.tile_n;
+          from = a.spare + place * cut.parts * stride + static_cast<int64_t>(pos - m * tile_m) * a.tile_n + (8 * g - n * a.tile_n);
+        }
+        for (int s = 0; s < (whole ? 1 : cut.parts); ++s) {
+          const float4 *p = reinterpret_cast<const float4 *>(from + s * stride);
           const float4 lo = __ldcs(p), hi = __ldcs(p + 1);
           v[0] += lo.x, v[1] += lo.y, v[2] += lo.z, v[3] += lo.w;
           v[4] += hi.x, v[5] += hi.y, v[6] += hi.z, v[7] += hi.w;
@@ -999,9 +1034,9 @@ inline bool WideFor(int64_t tiles, int64_t h_tiles, int64_t steps, int sms) {
 struct Plan {
   bool pack, copy_w;
   int64_t pad_rows, ld_x, ld_w, piece, ld_acc, tile_n, tiles;
-  int acc_tiles, ctas, ctas_gx;
+  int room, ctas, ctas_gx;
   bool wide_gx;
-  int64_t counts, words, row_of, pos_of, label_of, lse2, row_scale, x, w, part, part_sum, label_logit, delta, acc, bytes;
+  int64_t counts, words, row_of, pos_of, label_of, lse2, row_scale, x, w, part, part_sum, label_logit, delta, acc, spare, bytes;
 };
 
 /*! \brief layout of a call; sms = multiprocessors of the device */
@@ -1031,9 +1066,7 @@ inline Plan MakePlan(int64_t n, int64_t v, int64_t h, bool gradient, bool want_g
   p.ctas_gx = CtasFor(n, h_tiles, sms);
   const int64_t x_tiles = Ceil(n, 128 * p.ctas_gx);
   p.wide_gx = p.ctas_gx == 2 && WideFor(x_tiles * h_tiles, h_tiles, Ceil(p.piece, kStepK), sms);
-  // room for as many parts of the gradient of x as give every SM two tiles when all tokens count (PartsOf cuts it)
-  const int64_t parts = std::min<int64_t>(16, Ceil(2 * sms / p.ctas_gx, x_tiles * h_tiles / (p.wide_gx ? 2 : 1)));
-  p.acc_tiles = static_cast<int>(x_tiles * std::max<int64_t>(1, std::min<int64_t>(parts, p.piece / kStepK / 8)));
+  p.room = 4 * (sms / p.ctas_gx);  // parts of tiles: four rounds over the GPU
   int64_t at = 0;
   auto take = [&at](int64_t bytes) {
     const int64_t was = at;
@@ -1051,7 +1084,8 @@ inline Plan MakePlan(int64_t n, int64_t v, int64_t h, bool gradient, bool want_g
     p.lse2 = take(p.pad_rows * 4);
     p.row_scale = take(p.pad_rows * 4);
     p.delta = take(p.pad_rows * p.piece * 2);
-    p.acc = take(want_gx ? static_cast<int64_t>(p.acc_tiles) * 128 * p.ctas_gx * p.ld_acc * 4 : 0);
+    p.acc = take(want_gx ? p.pad_rows * p.ld_acc * 4 : 0);
+    p.spare = take(want_gx ? static_cast<int64_t>(p.room) * 128 * p.ctas_gx * kTileN * (p.wide_gx ? 2 : 1) * 4 : 0);
   } else {
     p.part = take(2 * p.tiles * p.pad_rows * 8);
     p.part_sum = take(smooth ? 2 * p.tiles * p.pad_rows * 4 : 0);
@@ -1266,19 +1300,22 @@ inline void BackwardLaunch(const GradOut &g, const Problem &q, const Plan &p, ch
     Gemm<kDelta>(x_along, w_along, x_along_in_place, d_along, a, m_tiles * a.n_tiles, p.ctas, sms, stream);
     if (g.gx != nullptr) {
       const CUtensorMap w_across = WeightMap(q, p, ws, p0, cols, 64, stream, false, &a.b_row0);
-      const CUtensorMap out = tc5::MatrixMap(acc, kFloat32, static_cast<int64_t>(p.acc_tiles) * 128 * p.ctas_gx, p.ld_acc, p.ld_acc, 128);
+      const CUtensorMap out = tc5::MatrixMap(acc, kFloat32, p.pad_rows, p.ld_acc, p.ld_acc, 128);
+      const int64_t tile_n = kTileN * (p.wide_gx ? 2 : 1);
+      const CUtensorMap spare =
+          tc5::MatrixMap(ws + p.spare, kFloat32, static_cast<int64_t>(p.room) * 128 * p.ctas_gx, tile_n, tile_n, 128);
       const int64_t x_tiles = Ceil(q.n, 128 * p.ctas_gx);
       a.n_tiles = p.wide_gx ? h_tiles / 2 : h_tiles;
       a.step_cycles = p.wide_gx ? 1024.0f : p.ctas_gx == 1 ? 560.0f : 512.0f;
       a.tile_cycles = static_cast<float>(128 * p.ctas_gx * kTileN * (p.wide_gx ? 2 : 1) * 8) / 2400.0f;
       a.k_blocks = static_cast<int32_t>(Ceil(cols, kStepK));
       a.k_plan = static_cast<int32_t>(Ceil(std::min(p.piece, q.v), kStepK));
-      a.acc_tiles = p.acc_tiles;
+      a.room = p.room;
       a.accumulate = p0 > 0;
       a.group = GroupOf(x_tiles, 8);
       a.instr = tc5::InstrDesc(q.bf16, false, true, 128 * p.ctas_gx, kTileN);
-      if (p.wide_gx) LaunchGemm<kDataGrad, 2, true>(d_along, w_across, d_along, out, a, x_tiles * a.n_tiles, sms, stream);
-      else Gemm<kDataGrad>(d_along, w_across, d_along, out, a, x_tiles * a.n_tiles, p.ctas_gx, sms, stream);
+      if (p.wide_gx) LaunchGemm<kDataGrad, 2, true>(d_along, w_across, spare, out, a, x_tiles * a.n_tiles, sms, stream);
+      else Gemm<kDataGrad>(d_along, w_across, spare, out, a, x_tiles * a.n_tiles, p.ctas_gx, sms, stream);
     }
     if (g.gw != nullptr) {
       const int64_t elem = g.gw_type == kFloat32 ? 4 : 2;
@@ -1310,9 +1347,11 @@ inline void BackwardLaunch(const GradOut &g, const Problem &q, const Plan &p, ch
   }
   if (g.gx != nullptr) {
     FinishArgs f = {};
-    f.acc = acc, f.ld_acc = p.ld_acc, f.live = a.live;
+    f.acc = acc, f.spare = reinterpret_cast<const float *>(ws + p.spare), f.ld_acc = p.ld_acc, f.live = a.live;
     f.n_tiles = p.wide_gx ? h_tiles / 2 : h_tiles;
-    f.k_plan = a.k_plan, f.acc_tiles = p.acc_tiles, f.slots = sms / p.ctas_gx, f.ctas = p.ctas_gx;
+    f.tile_n = p.wide_gx ? 2 * kTileN : kTileN;
+    f.group = GroupOf(Ceil(q.n, 128 * p.ctas_gx), 8);
+    f.k_plan = a.k_plan, f.room = p.room, f.slots = sms / p.ctas_gx, f.ctas = p.ctas_gx;
     f.step_cycles = a.step_cycles, f.tile_cycles = a.tile_cycles;
     f.pos_of = k.pos_of, f.inv_scale = a.inv_scale;
     f.out = g.gx, f.ld_out = g.ld_gx, f.n = static_cast<int32_t>(q.n), f.h = static_cast<int32_t>(q.h);
