@@ -10,7 +10,7 @@
  *
  * The products run on the tensor cores: 16-bit operands, binary32 accumulators in tensor memory,
  * one persistent CTA (or pair of CTAs) per SM (or pair of SMs) whose warps have fixed roles -- one
- * thread issues the tiled copies of the operands, one the products, four warps (a thread per
+ * thread issues the tiled copies of the operands, one the products, eight warps (two threads per
  * tile row) take the finished accumulators while the next tile's products run into the other
  * half of the tensor memory.  All waits are bounded.
  *
@@ -54,6 +54,7 @@ const int kThreads = 384;     // warp 0: copies, warp 1: products, warp 2: tenso
 const int kHalfN = kTileN / 2;  // columns of a tile that one epilogue group (four warps, a thread per row) takes
 const int kChunkSteps = 16;   // kStat: stages per run of accumulation in tensor memory (1024 contraction elements)
 const uint32_t kBoxOut = 128 * 128;  // a box of 128 rows by 128 bytes, on its way out through shared memory
+const int kWideSteps = 96;    // stages from which a gradient is computed in tiles of 512 columns
 const int kPadRows = 256;     // token rows of the scratch matrices are padded to this
 const float kLog2e = 1.4426950408889634f;
 
@@ -249,12 +250,12 @@ __device__ __forceinline__ void BoxSend(const Half &t, const CUtensorMap *map, i
  *  largest logit is log(sum) with nothing cancelled, never negative.  The exponentials' rate (16 a
  *  cycle and SM) leaves room for the addition.
  */
-__device__ __forceinline__ void StatHalf(float (&v)[kHalfN], const Half &t, int limit, int label, int64_t at, const GemmArgs &a) {
+__device__ __forceinline__ void StatHalf(float (&v)[kHalfN], const Half &own, int limit, int label, int64_t at, const GemmArgs &a) {
   if (a.part_sum != nullptr) {
-    float total = 0.0f;
+    float t[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int i = 0; i < kHalfN; ++i) total += i < limit ? v[i] : 0.0f;
-    a.part_sum[at] = total;
+    for (int i = 0; i < kHalfN; ++i) t[i & 7] += i < limit ? v[i] : 0.0f;
+    a.part_sum[at] = ((t[0] + t[1]) + (t[2] + t[3])) + ((t[4] + t[5]) + (t[6] + t[7]));
   }
   if (limit < kHalfN) {  // columns past the vocabulary weigh nothing
 #pragma unroll
@@ -273,7 +274,7 @@ __device__ __forceinline__ void StatHalf(float (&v)[kHalfN], const Half &t, int 
     float z = v[0];
 #pragma unroll
     for (int i = 1; i < kHalfN; ++i) z = i == label ? v[i] : z;
-    a.label_logit[t.row] = z;
+    a.label_logit[own.row] = z;
   }
   float s[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -651,7 +652,8 @@ VocabGemmKernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         } else {
           const float inv = a.inv_scale[0];
           if (a.out_tiled) {
-            if (a.out_type == kFloat32) FloatHalf<false>(t, inv, &map_out, t.col, row0);
+            if (a.out_type == kFloat32 && a.out_add) FloatHalf<true>(t, inv, &map_out, t.col, row0);
+            else if (a.out_type == kFloat32) FloatHalf<false>(t, inv, &map_out, t.col, row0);
             else PackedHalf(t, inv, a.out_type == kBfloat16, &map_out, row0);
           } else {
 #pragma unroll 1
@@ -1007,9 +1009,6 @@ inline bool Aligned16(const void *p, int64_t ld, int64_t elem) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * elem % 16 == 0;
 }
 
-#ifndef MSHADOW_B200_VLOSS_WIDE
-#define MSHADOW_B200_VLOSS_WIDE 96
-#endif
 /*!
  * \brief one CTA or a pair per tile.  A pair reads each operand half as often and runs a long grid of tiles
  *  about 6 % faster (8192 x 131072 x 4096: 6.06 against 6.50 ms), but its tiles are twice as high: where that
@@ -1027,7 +1026,7 @@ inline int CtasFor(int64_t rows, int64_t other_tiles, int sms) {
  *  while nothing multiplies (some 8000 cycles) costs less than the quarter of the loads that is saved
  */
 inline bool WideFor(int64_t tiles, int64_t h_tiles, int64_t steps, int sms) {
-  return h_tiles % 2 == 0 && tiles / 2 >= sms && steps >= MSHADOW_B200_VLOSS_WIDE;
+  return h_tiles % 2 == 0 && tiles / 2 >= sms && steps >= kWideSteps;
 }
 
 /*! \brief how a call is cut, and where its scratch matrices lie (offsets in bytes) */
@@ -1099,7 +1098,7 @@ inline Plan MakePlan(int64_t n, int64_t v, int64_t h, bool gradient, bool want_g
 inline void CheckExtents(const Problem &q) {
   CHECK(q.n <= (int64_t(1) << 30) && Ceil(q.n, 128) * Ceil(q.v, 16) < (int64_t(1) << 31) &&
         Ceil(q.v, 128) * Ceil(q.h, 256) < (int64_t(1) << 31))
-      << "LinearSoftmaxLoss: more tokens times classes than one call covers";
+      << "LinearSoftmaxLoss: more tokens, classes or features than one call covers";
 }
 inline Plan PlanForward(const Problem &q, int sms) {
   CheckExtents(q);
@@ -1333,8 +1332,9 @@ inline void BackwardLaunch(const GradOut &g, const Problem &q, const Plan &p, ch
       a.out_add = g.gw_add;
       a.out_vec = Aligned16(a.out, g.ld_gw, elem);
       // (a tiled copy leaves out columns past the matrix in units of 16 bytes: rows that do not end on such a
-      // boundary would lose up to 14 bytes behind them to zeros)
-      a.out_tiled = a.out_vec && !a.out_add && q.h * elem % 16 == 0;
+      // boundary would lose up to 14 bytes behind them to zeros.  It also adds, binary32 to binary32 (numbers below
+      // 2^-126 count as zero); a 16-bit sum would be rounded twice, so those additions are plain accesses.)
+      a.out_tiled = a.out_vec && (!a.out_add || a.out_type == kFloat32) && q.h * elem % 16 == 0;
       const CUtensorMap out = a.out_tiled ? tc5::MatrixMap(a.out, g.gw_type, cols, q.h, g.ld_gw, 128) : x_across;
       const int64_t tiles = static_cast<int64_t>(a.m_tiles) * h_tiles;
       if (ctas == 2 && WideFor(tiles, h_tiles, Ceil(q.n, kStepK), sms)) {
