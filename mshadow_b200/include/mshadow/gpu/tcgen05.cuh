@@ -148,8 +148,11 @@ __device__ __forceinline__ void StoreBox(const CUtensorMap *map, int x, int y, u
   }
   asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
-/*! \brief this thread's stores have read their shared memory */
-__device__ __forceinline__ void WaitStoresRead() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+/*! \brief all but the last kPending of this thread's stores have read their shared memory */
+template <int kPending>
+__device__ __forceinline__ void WaitStoresRead() {
+  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kPending) : "memory");
+}
 /*! \brief this thread's stores have been written */
 __device__ __forceinline__ void WaitStores() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 

@@ -55,6 +55,7 @@ const int kHalfN = kTileN / 2;  // columns of a tile that one epilogue group (fo
 const int kChunkSteps = 16;   // kStat: stages per run of accumulation in tensor memory (1024 contraction elements)
 const uint32_t kBoxOut = 128 * 128;  // a box of 128 rows by 128 bytes, on its way out through shared memory
 const int kWideSteps = 96;    // stages from which a gradient is computed in tiles of 512 columns
+const int kWideDeltaSteps = 48;  // the same for d, whose columns stay at least two rounds of tiles (64 steps: 7 % faster, 32: even, 16: 15 % slower)
 const int kPadRows = 256;     // token rows of the scratch matrices are padded to this
 const float kLog2e = 1.4426950408889634f;
 
@@ -73,16 +74,20 @@ struct Layout {
 };
 
 /*! \brief kWide: a pair's tile is 512 columns wide, two sets of 256, and fills the tensor memory */
-template <int kCtas, bool kWide>
+template <int kMode, int kCtas, bool kWide>
 struct StageShape {
   static const int kRowsN = kTileN / kCtas;                          // rows of B that a CTA holds, of a set
   static const int kSets = kWide ? 2 : 1;                            // sets of accumulators per tile
   static const uint32_t kBytesA = 128 * kStepK * 2;
   static const uint32_t kBytesB = kRowsN * kStepK * 2;
   static const uint32_t kStage = kBytesA + kSets * kBytesB;
-  static const int kStages = kCtas == 2 && !kWide ? 6 : 4;
-  static const uint32_t kOut = kStage * kStages;                     // a box per epilogue group
-  static const size_t kSmem = kOut + 2 * kBoxOut + 1024;  // + alignment to the swizzle's 1024 bytes
+  // Five stages of 32 KB are enough where there is something to send: the sixth's place is worth more as a second
+  // outgoing box for each epilogue group (d of 8192 x 32768 x 512: 3 %).  kStat sends nothing (and is 2 % faster with
+  // six than with five; seven are no better).
+  static const int kStages = kCtas != 2 || kWide ? 4 : kMode == kStat ? 6 : 5;
+  static const int kBoxes = kMode == kStat ? 0 : kCtas == 2 && !kWide ? 2 : 1;  // outgoing boxes of an epilogue group
+  static const uint32_t kOut = kStage * kStages;
+  static const size_t kSmem = kOut + 2 * kBoxes * kBoxOut + 1024;    // + alignment to the swizzle's 1024 bytes
 };
 
 struct GemmArgs {
@@ -221,18 +226,21 @@ struct Half {
   uint32_t acc;      // tensor memory of this thread's row, first column of the half
   int64_t row;       // row of the matrix
   int col;           // first column of the half, within the piece
-  uint32_t box;      // shared memory of the group's outgoing box
+  uint32_t boxes, box;  // shared memory of the group's first outgoing box; which one is filled next
   int group, thread; // 0 / 1; thread of the group: 0 .. 127
+  __device__ __forceinline__ uint32_t Box() const { return boxes + box * 2 * kBoxOut; }
 };
 
-/*! \brief the group's outgoing box is free again */
-__device__ __forceinline__ void BoxFree(const Half &t) {
-  if (t.thread == 0) tc5::WaitStoresRead();
-  tc5::NamedBarrier(1 + t.group, 128);
+/*! \brief the group's next outgoing box is free */
+template <int kBoxes>
+__device__ __forceinline__ void BoxFree(Half *t) {
+  if (kBoxes == 2) t->box ^= 1u;
+  if (t->thread == 0) tc5::WaitStoresRead<kBoxes == 2 ? 1 : 0>();
+  tc5::NamedBarrier(1 + t->group, 128);
 }
 /*! \brief 16 bytes of this thread's row of the box, in the place the 128-byte swizzle gives them */
 __device__ __forceinline__ void BoxPut(const Half &t, int chunk, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-  const uint32_t at = t.box + t.thread * 128 + ((chunk ^ (t.thread & 7)) << 4);
+  const uint32_t at = t.Box() + t.thread * 128 + ((chunk ^ (t.thread & 7)) << 4);
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 /*! \brief the box is full: one thread sends it to column x, row y of the output */
@@ -240,7 +248,7 @@ template <bool kAdd>
 __device__ __forceinline__ void BoxSend(const Half &t, const CUtensorMap *map, int x, int y) {
   tma::FenceAsyncShared();
   tc5::NamedBarrier(1 + t.group, 128);
-  if (t.thread == 0) tc5::StoreBox<kAdd>(map, x, y, t.box);
+  if (t.thread == 0) tc5::StoreBox<kAdd>(map, x, y, t.Box());
 }
 
 /*!
@@ -290,9 +298,10 @@ __device__ __forceinline__ void StatHalf(float (&v)[kHalfN], const Half &own, in
 /*! \brief d' of 32 columns */
 __device__ __forceinline__ void DeltaColumns(const uint32_t (&r)[32], int limit, int label, float lse2, float scale,
                                              const GemmArgs &a, uint32_t (&out)[16]) {
+  const float other = a.q_other * scale;
   float d[32];
 #pragma unroll
-  for (int i = 0; i < 32; ++i) d[i] = (Exp2(__fmaf_rn(__uint_as_float(r[i]), kLog2e, -lse2)) - a.q_other) * scale;
+  for (int i = 0; i < 32; ++i) d[i] = __fmaf_rn(Exp2(__fmaf_rn(__uint_as_float(r[i]), kLog2e, -lse2)), scale, -other);
   if (static_cast<unsigned>(label) < 32u) {
 #pragma unroll
     for (int i = 0; i < 32; ++i) {
@@ -307,7 +316,8 @@ __device__ __forceinline__ void DeltaColumns(const uint32_t (&r)[32], int limit,
   for (int i = 0; i < 16; ++i) out[i] = PackPair(d[2 * i], d[2 * i + 1], a.bf16);
 }
 
-__device__ __forceinline__ void DeltaHalf(const Half &t, int limit, int label, float lse2, float scale, const CUtensorMap *map,
+template <int kBoxes>
+__device__ __forceinline__ void DeltaHalf(Half &t, int limit, int label, float lse2, float scale, const CUtensorMap *map,
                                           int row0, const GemmArgs &a) {
 #pragma unroll 1
   for (int b = 0; b < kHalfN / 64; ++b) {
@@ -318,7 +328,7 @@ __device__ __forceinline__ void DeltaHalf(const Half &t, int limit, int label, f
     tc5::WaitColumns(r1);
     DeltaColumns(r0, limit - b * 64, label - b * 64, lse2, scale, a, p0);
     DeltaColumns(r1, limit - b * 64 - 32, label - b * 64 - 32, lse2, scale, a, p1);
-    BoxFree(t);
+    BoxFree<kBoxes>(&t);
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       BoxPut(t, q, p0[4 * q], p0[4 * q + 1], p0[4 * q + 2], p0[4 * q + 3]);
@@ -329,8 +339,8 @@ __device__ __forceinline__ void DeltaHalf(const Half &t, int limit, int label, f
 }
 
 /*! \brief the half tile as binary32, times `factor`, stored or added */
-template <bool kAdd>
-__device__ __forceinline__ void FloatHalf(const Half &t, float factor, const CUtensorMap *map, int x, int y) {
+template <int kBoxes, bool kAdd>
+__device__ __forceinline__ void FloatHalf(Half &t, float factor, const CUtensorMap *map, int x, int y) {
 #pragma unroll 1
   for (int b = 0; b < kHalfN / 32; ++b) {
     uint32_t r[32];
@@ -338,7 +348,7 @@ __device__ __forceinline__ void FloatHalf(const Half &t, float factor, const CUt
     tc5::WaitColumns(r);
 #pragma unroll
     for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * factor);
-    BoxFree(t);
+    BoxFree<kBoxes>(&t);
 #pragma unroll
     for (int q = 0; q < 8; ++q) BoxPut(t, q, r[4 * q], r[4 * q + 1], r[4 * q + 2], r[4 * q + 3]);
     BoxSend<kAdd>(t, map, x + b * 32, y);
@@ -346,7 +356,8 @@ __device__ __forceinline__ void FloatHalf(const Half &t, float factor, const CUt
 }
 
 /*! \brief the half tile in the operands' type, times `factor` */
-__device__ __forceinline__ void PackedHalf(const Half &t, float factor, int bf16, const CUtensorMap *map, int row0) {
+template <int kBoxes>
+__device__ __forceinline__ void PackedHalf(Half &t, float factor, int bf16, const CUtensorMap *map, int row0) {
 #pragma unroll 1
   for (int b = 0; b < kHalfN / 64; ++b) {
     uint32_t r0[32], r1[32];
@@ -359,7 +370,7 @@ __device__ __forceinline__ void PackedHalf(const Half &t, float factor, int bf16
       r0[i] = PackPair(__uint_as_float(r0[2 * i]) * factor, __uint_as_float(r0[2 * i + 1]) * factor, bf16);
       r1[i] = PackPair(__uint_as_float(r1[2 * i]) * factor, __uint_as_float(r1[2 * i + 1]) * factor, bf16);
     }
-    BoxFree(t);
+    BoxFree<kBoxes>(&t);
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       BoxPut(t, q, r0[4 * q], r0[4 * q + 1], r0[4 * q + 2], r0[4 * q + 3]);
@@ -442,15 +453,15 @@ __device__ __forceinline__ void WeightColumns(const uint32_t (&r)[32], int64_t r
  *  cost 1 % of the time (runs of 512: 2.5e-7 and another 3 %; of 256: 17 %).
  *
  *  kWide: both sets belong to one tile.  A step's rows of A then serve 512 columns, a quarter less is read from the L2
- *  and, where A is d', from memory; in return the products wait while a tile is emptied.  For the gradients
- *  with long contractions.
+ *  and, where A is d', from memory; in return the products wait while a tile is emptied.  For long contractions (not
+ *  in kStat, whose runs would be emptied too often).
  */
 template <int kMode, int kCtas, bool kWide>
 __global__ void __launch_bounds__(kThreads, 1)
 VocabGemmKernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                 const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_out, const GemmArgs a) {
   // map_x: the rows of x where the caller has them; kDataGrad: the parts of tiles beside the gradient
-  typedef StageShape<kCtas, kWide> S;
+  typedef StageShape<kMode, kCtas, kWide> S;
   typedef Layout<kMode> L;
   extern __shared__ uint8_t raw[];
   __shared__ uint64_t full[S::kStages], empty[S::kStages], acc_full[2], acc_empty[2];
@@ -533,7 +544,10 @@ VocabGemmKernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
               tc5::LoadBox<kCtas>(sb + j * tc5::kBoxBytes, from_b, x, a.b_row0 + k0, bar);
             }
           } else {
-            tc5::LoadBox<kCtas>(sb, from_b, k0, a.b_row0 + n0, bar);
+#pragma unroll
+            for (int set = 0; set < S::kSets; ++set) {
+              tc5::LoadBox<kCtas>(sb + set * S::kBytesB, from_b, k0, a.b_row0 + n0 + set * kTileN, bar);
+            }
           }
         }
       }
@@ -583,7 +597,8 @@ VocabGemmKernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
     Half t;
     t.group = (warp - 4) >> 2;
     t.thread = threadIdx.x - 128 - t.group * 128;
-    t.box = smem + S::kOut + t.group * kBoxOut;
+    t.box = 0u;
+    t.boxes = smem + S::kOut + t.group * kBoxOut;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     uint32_t turn = 0;
     bool ok = true;
@@ -610,7 +625,6 @@ VocabGemmKernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
       const int row0 = u.m * tile_m + static_cast<int>(rank) * 128;
       t.row = row0 + t.thread;
       t.col = u.n * tile_n + t.group * kHalfN;
-      const int limit = min(a.cols - t.col, tile_n - t.group * kHalfN);  // columns of this half that exist
       const int label = (kMode == kStat || kMode == kDelta) && t.row < live ? a.label[t.row] : -1;
       if (kMode == kStat) {
         float v[kHalfN];
@@ -629,32 +643,30 @@ VocabGemmKernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         if (!ok) break;
         if (row0 + (warp & 3) * 32 >= live) continue;  // no row of this warp's exists
         const int64_t at = (static_cast<int64_t>(a.tile0 + u.n) * 2 + t.group) * a.pad_rows + t.row;
+        const int limit = min(a.cols - t.col, tile_n - t.group * kHalfN);  // columns of this half that exist
         StatHalf(v, t, limit, label < 0 ? -1 : label - a.col0 - t.col, at, a);
-        continue;
-      }
-      if (kMode == kDelta) {
-        if (!ready()) break;
-        // rows past the live ones: lse and scale are 0, the data row is zero, and so is d'
-        DeltaHalf(t, limit, label < 0 ? -1 : label - a.col0 - t.col, a.lse2[t.row], a.row_scale[t.row], &map_out, row0, a);
-        release();
         continue;
       }
       for (int set = 0; set < S::kSets; ++set, t.col += kTileN) {
         if (!ready()) break;
-        if (kMode == kDataGrad) {
+        if (kMode == kDelta) {
+          // rows past the live ones: lse and scale are 0, the data row is zero, and so is d'
+          DeltaHalf<S::kBoxes>(t, a.cols - t.col, label < 0 ? -1 : label - a.col0 - t.col, a.lse2[t.row], a.row_scale[t.row],
+                               &map_out, row0, a);
+        } else if (kMode == kDataGrad) {
           // a whole tile goes to its place in the gradient, a part of one to a tile of its own beside it
           const bool whole = u.parts == 1;
           const CUtensorMap *to = whole ? &map_out : &map_x;
           const int x = whole ? t.col : t.group * kHalfN + set * kTileN;
           const int y = whole ? row0 : u.spare * tile_m + static_cast<int>(rank) * 128;
-          if (a.accumulate) FloatHalf<true>(t, 1.0f, to, x, y);
-          else FloatHalf<false>(t, 1.0f, to, x, y);
+          if (a.accumulate) FloatHalf<S::kBoxes, true>(t, 1.0f, to, x, y);
+          else FloatHalf<S::kBoxes, false>(t, 1.0f, to, x, y);
         } else {
           const float inv = a.inv_scale[0];
           if (a.out_tiled) {
-            if (a.out_type == kFloat32 && a.out_add) FloatHalf<true>(t, inv, &map_out, t.col, row0);
-            else if (a.out_type == kFloat32) FloatHalf<false>(t, inv, &map_out, t.col, row0);
-            else PackedHalf(t, inv, a.out_type == kBfloat16, &map_out, row0);
+            if (a.out_type == kFloat32 && a.out_add) FloatHalf<S::kBoxes, true>(t, inv, &map_out, t.col, row0);
+            else if (a.out_type == kFloat32) FloatHalf<S::kBoxes, false>(t, inv, &map_out, t.col, row0);
+            else PackedHalf<S::kBoxes>(t, inv, a.out_type == kBfloat16, &map_out, row0);
           } else {
 #pragma unroll 1
             for (int c = 0; c < kHalfN / 32; ++c) {
@@ -1123,7 +1135,7 @@ template <int kMode, int kCtas, bool kWide>
 inline void LaunchGemm(const CUtensorMap &ma, const CUtensorMap &mb, const CUtensorMap &mx, const CUtensorMap &mo, const GemmArgs &args, int64_t units,
                        int sms, cudaStream_t stream) {
   auto kernel = VocabGemmKernel<kMode, kCtas, kWide>;
-  const size_t smem = StageShape<kCtas, kWide>::kSmem;
+  const size_t smem = StageShape<kMode, kCtas, kWide>::kSmem;
   gpu_rt::AllowSharedMemory(kernel, smem);
   cudaLaunchConfig_t cfg = {};
   // (the parts of kDataGrad are counted by the kernel: it gets every slot)
@@ -1296,7 +1308,12 @@ inline void BackwardLaunch(const GradOut &g, const Problem &q, const Plan &p, ch
     a.group = GroupOf(m_tiles, 16);
     a.instr = tc5::InstrDesc(q.bf16, false, false, 128 * p.ctas, kTileN);
     const CUtensorMap w_along = WeightMap(q, p, ws, p0, cols, kTileN / p.ctas, stream, true, &a.b_row0);
-    Gemm<kDelta>(x_along, w_along, x_along_in_place, d_along, a, m_tiles * a.n_tiles, p.ctas, sms, stream);
+    if (p.ctas == 2 && a.n_tiles % 2 == 0 && m_tiles * a.n_tiles >= 4 * sms && a.k_blocks >= kWideDeltaSteps) {
+      a.n_tiles /= 2;
+      LaunchGemm<kDelta, 2, true>(x_along, w_along, x_along_in_place, d_along, a, m_tiles * a.n_tiles, sms, stream);
+    } else {
+      Gemm<kDelta>(x_along, w_along, x_along_in_place, d_along, a, m_tiles * a.n_tiles, p.ctas, sms, stream);
+    }
     if (g.gx != nullptr) {
       const CUtensorMap w_across = WeightMap(q, p, ws, p0, cols, 64, stream, false, &a.b_row0);
       const CUtensorMap out = tc5::MatrixMap(acc, kFloat32, p.pad_rows, p.ld_acc, p.ld_acc, 128);
