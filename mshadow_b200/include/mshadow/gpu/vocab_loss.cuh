@@ -628,6 +628,8 @@ VocabGemmKernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
       const int label = (kMode == kStat || kMode == kDelta) && t.row < live ? a.label[t.row] : -1;
       if (kMode == kStat) {
         float v[kHalfN];
+#pragma unroll
+        for (int i = 0; i < kHalfN; ++i) v[i] = 0.0f;
         for (int run = 0; run < runs; ++run) {
           if (!ready()) break;
 #pragma unroll
@@ -636,14 +638,14 @@ VocabGemmKernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
             tc5::LoadColumns(t.acc + c * 16, r);
             tc5::WaitColumns(r);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) v[c * 16 + i] = run == 0 ? __uint_as_float(r[i]) : v[c * 16 + i] + __uint_as_float(r[i]);
+            for (int i = 0; i < 16; ++i) v[c * 16 + i] += __uint_as_float(r[i]);
           }
           release();
         }
         if (!ok) break;
         if (row0 + (warp & 3) * 32 >= live) continue;  // no row of this warp's exists
-        const int64_t at = (static_cast<int64_t>(a.tile0 + u.n) * 2 + t.group) * a.pad_rows + t.row;
         const int limit = min(a.cols - t.col, tile_n - t.group * kHalfN);  // columns of this half that exist
+        const int64_t at = (static_cast<int64_t>(a.tile0 + u.n) * 2 + t.group) * a.pad_rows + t.row;
         StatHalf(v, t, limit, label < 0 ? -1 : label - a.col0 - t.col, at, a);
         continue;
       }
