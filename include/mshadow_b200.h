@@ -421,8 +421,12 @@ int msb_softmax_grad3d_f32(float *dst, const float *src, const float *label, int
    `workspace` of the entries below: device memory of at least the size that the matching
    ..._workspace() call reports, used by the call until it completes on its stream; NULL takes the
    stream's scratch memory (see the conventions above).  A call that is captured into a graph must
-   bring its own workspace (MSB_ERR_ARGUMENT otherwise), and graphs whose replays may overlap must
-   not share one. */
+   bring its own workspace (MSB_ERR_ARGUMENT otherwise), graphs whose replays may overlap must not
+   share one, and the first call on a device (or a msb_stream_wait) precedes the first capture.
+
+   All operands, the workspace too, are memory of the current device (or managed memory): other
+   pointers are refused with MSB_ERR_ARGUMENT.  Rows may have any pitch and start at any element;
+   rows on 16-byte boundaries are the fast case.  Labels and indices are int32. */
 enum { MSB_FLOAT32 = 0, MSB_FLOAT16 = 2, MSB_BFLOAT16 = 12 };
 
 /* dst[i] = scale * table[index[i]], a row of zeros where index[i] is outside [0, rows): the

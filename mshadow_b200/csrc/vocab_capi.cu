@@ -18,7 +18,24 @@ using namespace mshadow;  // NOLINT(*)
 typedef mshadow::half::half_t half_t;
 typedef mshadow::bfloat::bf16_t bf16_t;
 
+// every entry that launches work runs inside an NVTX range named after it (-DMSHADOW_B200_NVTX=0: none)
+#ifndef MSHADOW_B200_NVTX
+#define MSHADOW_B200_NVTX 1
+#endif
+#if MSHADOW_B200_NVTX
+#include <nvtx3/nvToolsExt.h>
+#endif
+
 namespace {
+
+struct TraceRange {
+#if MSHADOW_B200_NVTX
+  explicit TraceRange(const char *name) { nvtxRangePushA(name); }
+  ~TraceRange() { nvtxRangePop(); }
+#else
+  explicit TraceRange(const char *) {}
+#endif
+};
 
 int Refuse(const char *name, int code, const std::string &msg) {
   msb_internal::SetLastError((std::string(name) + ": " + msg).c_str());
@@ -31,6 +48,7 @@ int Refuse(const char *name, int code, const std::string &msg) {
 /*! \brief runs `body`, turning whatever it throws into a status; nothing leaves through the C boundary */
 template <typename Body>
 int Guarded(const char *name, Body body) {
+  TraceRange range(name);
   try {
     body();
   } catch (const dmlc::Error &e) {
