@@ -7,3 +7,15 @@ sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 
 def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a CUDA device (run with -m gpu)")
+
+
+def pytest_collection_modifyitems(items):
+    """test_oracle_pin.py is skipped where the reference build (oracle/_ref) is absent; the one case there that
+    compares with it without carrying the mark gets it here."""
+    import pytest
+    built = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "oracle", "_ref", "libmshadow_ref.so")
+    if os.path.exists(built):
+        return
+    for item in items:
+        if item.name == "test_addtakegrad_matches_reference":
+            item.add_marker(pytest.mark.skip(reason="reference build (oracle/_ref) not present"))
