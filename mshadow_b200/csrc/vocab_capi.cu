@@ -65,6 +65,11 @@ int Guarded(const char *name, Body body) {
 inline bool ElementAligned(const void *p, int dtype) {
   return reinterpret_cast<uintptr_t>(p) % (dtype == kFloat32 ? 4 : 2) == 0;
 }
+/*! \brief addresses of int32 / float arrays */
+template <typename... Pointers>
+inline bool WordAligned(Pointers... p) {
+  return ((reinterpret_cast<uintptr_t>(p) % 4 == 0) && ...);
+}
 inline bool FitsIndex(int64_t v) { return v >= 0 && v <= 0x7fffffffLL; }
 inline bool LdOk(int64_t ld, int64_t width) { return ld >= width && FitsIndex(ld); }
 
@@ -138,7 +143,7 @@ int msb_embed_take(void *dst, const void *table, const int32_t *index, int64_t n
   VOCAB_REQUIRE(LdOk(ld_dst, width) && LdOk(ld_table, width), MSB_ERR_SHAPE, "stride < width");
   if (n == 0 || width == 0) return MSB_OK;
   VOCAB_REQUIRE(dst && index && (table || rows == 0), MSB_ERR_ARGUMENT, "null pointer");
-  VOCAB_REQUIRE(ElementAligned(dst, dtype) && ElementAligned(table, dtype), MSB_ERR_LAYOUT,
+  VOCAB_REQUIRE(ElementAligned(dst, dtype) && ElementAligned(table, dtype) && WordAligned(index), MSB_ERR_LAYOUT,
                 "operands must be aligned to their elements");
   const int rc = PlaceCheck(__func__, dst, table, index);
   if (rc != MSB_OK) return rc;
@@ -175,7 +180,7 @@ int msb_embed_take_grad(void *dst, const void *src, const int32_t *index, int64_
   VOCAB_REQUIRE(LdOk(ld_dst, width) && LdOk(ld_src, width), MSB_ERR_SHAPE, "stride < width");
   if (rows == 0 || width == 0 || (n == 0 && saver == 1)) return MSB_OK;
   VOCAB_REQUIRE(dst && (n == 0 || (src && index)), MSB_ERR_ARGUMENT, "null pointer");
-  VOCAB_REQUIRE(ElementAligned(dst, dtype) && ElementAligned(src, dtype), MSB_ERR_LAYOUT,
+  VOCAB_REQUIRE(ElementAligned(dst, dtype) && ElementAligned(src, dtype) && WordAligned(index), MSB_ERR_LAYOUT,
                 "operands must be aligned to their elements");
   int64_t need = 0;
   int rc = msb_embed_take_grad_workspace(n, width, &need);
@@ -224,7 +229,7 @@ int msb_linear_softmax_loss(float *loss, float *lse, const void *data, const voi
                 "smoothing must lie in [0, 1) and needs two classes");
   if (n == 0) return MSB_OK;
   VOCAB_REQUIRE(loss && lse && data && weight && label, MSB_ERR_ARGUMENT, "null pointer");
-  VOCAB_REQUIRE(ElementAligned(data, dtype) && ElementAligned(weight, dtype), MSB_ERR_LAYOUT,
+  VOCAB_REQUIRE(ElementAligned(data, dtype) && ElementAligned(weight, dtype) && WordAligned(loss, lse, label), MSB_ERR_LAYOUT,
                 "operands must be aligned to their elements");
   int rc = PlaceCheck(__func__, loss, lse, data, weight, label, workspace);
   if (rc == MSB_OK) rc = CaptureCheck(__func__, workspace, true, stream);
@@ -262,7 +267,7 @@ int msb_linear_softmax_loss_grad(void *gdata, void *gweight, const void *data, c
   if (gdata == nullptr && gweight == nullptr) return MSB_OK;
   VOCAB_REQUIRE(n == 0 || (data && weight && label && lse), MSB_ERR_ARGUMENT, "null pointer");
   VOCAB_REQUIRE(ElementAligned(data, dtype) && ElementAligned(weight, dtype) && ElementAligned(gdata, dtype) &&
-                    ElementAligned(gweight, gweight_dtype),
+                    ElementAligned(gweight, gweight_dtype) && WordAligned(label, lse, gloss),
                 MSB_ERR_LAYOUT, "operands must be aligned to their elements");
   int rc = PlaceCheck(__func__, gdata, gweight, data, weight, label, lse, gloss, workspace);
   if (rc == MSB_OK) rc = CaptureCheck(__func__, workspace, n > 0, stream);

@@ -237,6 +237,11 @@ struct GradArgs {
                                // the runs of few parts from the front, of many parts from the back
 };
 
+/*! \brief scale * sum; the sum of nothing (a run of entries that name no row) stays it, whatever the scale: adding it changes no value */
+__device__ __forceinline__ float Scaled(float scale, float sum) {
+  return __float_as_uint(sum) == 0x80000000u ? sum : __fmul_rn(scale, sum);
+}
+
 template <typename T, bool kVec>
 __device__ __forceinline__ void WriteRow(const GradArgs<T> &a, int32_t row, uint32_t col,
                                          const float (&acc)[Group<T, kVec>::kLanes]) {
@@ -247,10 +252,10 @@ __device__ __forceinline__ void WriteRow(const GradArgs<T> &a, int32_t row, uint
     Load(p, &b);
     Unpack<T, kVec>(b, v);
 #pragma unroll
-    for (int l = 0; l < Group<T, kVec>::kLanes; ++l) v[l] = __fadd_rn(v[l], __fmul_rn(a.scale, acc[l]));
+    for (int l = 0; l < Group<T, kVec>::kLanes; ++l) v[l] = __fadd_rn(v[l], Scaled(a.scale, acc[l]));
   } else {
 #pragma unroll
-    for (int l = 0; l < Group<T, kVec>::kLanes; ++l) v[l] = __fadd_rn(__fmul_rn(a.scale, acc[l]), 0.0f);
+    for (int l = 0; l < Group<T, kVec>::kLanes; ++l) v[l] = __fadd_rn(Scaled(a.scale, acc[l]), 0.0f);
   }
   Pack<T, kVec>(v, &b);
   Store(p, b);
@@ -504,7 +509,7 @@ __global__ void __launch_bounds__(256) EmbedSumKernel(const GradArgs<T> a) {
   if (col >= a.width) return;
   float acc[G::kLanes];
 #pragma unroll
-  for (int l = 0; l < G::kLanes; ++l) acc[l] = -0.0f;  // the sum of nothing: adding it changes no value
+  for (int l = 0; l < G::kLanes; ++l) acc[l] = -0.0f;  // the sum of nothing
   for (int i = from; i < to; i += kDepth) {
     Bits<T, kVec> b[kDepth], d[kAdd ? kDepth : 1];
     int32_t r[kDepth];
@@ -537,7 +542,7 @@ __global__ void __launch_bounds__(256) EmbedSumKernel(const GradArgs<T> a) {
       } else {
         if (kAdd) Unpack<T, kVec>(d[kAdd ? u : 0], v);
 #pragma unroll
-        for (int l = 0; l < G::kLanes; ++l) v[l] = __fadd_rn(__fmul_rn(a.scale, acc[l]), kAdd ? v[l] : 0.0f);
+        for (int l = 0; l < G::kLanes; ++l) v[l] = __fadd_rn(Scaled(a.scale, acc[l]), kAdd ? v[l] : 0.0f);
         Pack<T, kVec>(v, &b[u]);
         Store(a.grad + s_keys[kChunk + p] * a.ld_grad + col, b[u]);
       }

@@ -64,6 +64,8 @@ def test_embed_refusals(lib):
     assert take(ld_dst=7) == 2 and take(ld_table=4) == 2
     assert take(dst=None) == 1 and take(table=None) == 1 and take(index=None) == 1
     assert take(n=0, dst=None, table=None, index=None) == 0
+    odd, two = C.c_void_p((1 << 20) + 1), C.c_void_p((1 << 20) + 2)
+    assert take(dst=two) == 3 and take(table=two) == 3 and take(index=two) == 3 and take(dtype=2, dst=odd) == 3
 
     def grad(n=4, rows=10, width=8, ld_dst=8, ld_src=8, dtype=0, saver=0, dst=p, src=p, index=p, ws=None, size=0):
         return lib.status("msb_embed_take_grad", dst, src, index, n, rows, width, ld_dst, ld_src, dtype, 1.0, saver, ws,
@@ -73,6 +75,7 @@ def test_embed_refusals(lib):
     assert grad(n=-1) == 2 and grad(ld_dst=7) == 2 and grad(ld_src=7) == 2
     assert grad(dst=None) == 1 and grad(src=None) == 1 and grad(index=None) == 1
     assert grad(n=100000, ws=p, size=1000) == 1  # workspace too small
+    assert grad(dst=two) == 3 and grad(src=two) == 3 and grad(index=two) == 3
     assert grad(rows=0, dst=None, src=None, index=None) == 0
     assert grad(n=0, saver=1, dst=None, src=None, index=None) == 0
     assert lib.embed_take_grad_workspace(0, 64, 8) == 0
@@ -108,6 +111,10 @@ def test_loss_refusals(lib):
     for name in ("x", "w", "label", "lse"):
         assert grad(**{name: None}) == 1
     assert grad(gw_dtype=0, gw=C.c_void_p((1 << 20) + 2)) == 3
+    odd = C.c_void_p((1 << 20) + 2)  # 2-byte aligned: not an int32 or a float
+    assert grad(label=odd) == 3 and grad(lse=odd) == 3
+    for name in ("out", "lse", "label"):
+        assert loss(**{name: odd}) == 3
     assert grad(gx=None, gw=None) == 0
 
 
@@ -890,3 +897,117 @@ def test_gradient_in_place(lib):
         lib.linear_softmax_loss_grad(gx, gw, x, w, label, lse)
         lib.linear_softmax_loss_grad(x, gw2, x, w, label, lse)
         assert torch.equal(x, gx) and torch.equal(gw, gw2)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [100, 3000])
+@pytest.mark.parametrize("scale", [-2.0, float("inf"), float("nan")])
+def test_dropped_indices_touch_no_row(lib, n, scale):
+    """Indices that name no row leave every row's bits alone, whatever the scale (they are sorted among those of row 0)."""
+    index = torch.full((n,), -1, dtype=torch.int32, device="cuda")
+    index[1::2] = 50
+    src = torch.randn(n, 24, device="cuda")
+    dst = torch.full((50, 24), -0.0, device="cuda")
+    lib.embed_take_grad(dst, src, index, scale=scale, saver=1)
+    assert (dst.view(torch.int32) == -(1 << 31)).all()
+    lib.embed_take_grad(dst, src, index, scale=scale)
+    assert (dst.view(torch.int32) == 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,v,h", [(5, 300, 40), (300, 700, 72), (700, 3000, 520), (3000, 20000, 264)])
+def test_what_the_workspace_held_does_not_matter(lib, n, v, h):
+    """NaN everywhere in the workspace gives the same bits as zeros."""
+    table, tokens, label, gtable, bufs, ws = tied(lib, n, v, h, BF16, 21)
+    label[::3] = -1
+    seen = []
+    for fill in (0, 0xff):
+        ws.fill_(fill)
+        lib.embed_take(bufs[0], table, tokens)
+        lib.linear_softmax_loss(bufs[2], bufs[3], bufs[0], table, label, smooth=0.1, workspace=ws)
+        ws.fill_(fill)
+        lib.linear_softmax_loss_grad(bufs[1], gtable, bufs[0], table, label, bufs[3], smooth=0.1, workspace=ws)
+        ws.fill_(fill)
+        head = gtable.clone()
+        lib.embed_take_grad(gtable, bufs[1], tokens, saver=1, workspace=ws)
+        seen.append([t.clone() for t in (*bufs, head, gtable)])
+    assert all(torch.equal(a, b) for a, b in zip(*seen))
+    assert all(torch.isfinite(t).all() for t in seen[0])
+
+
+@pytest.mark.gpu
+def test_graph_of_kernels_not_used_before(lib):
+    """A capture may use sizes, and with them kernels, that no earlier call used; two graphs with a workspace each."""
+    x, w, label = problem(3, 40, 8, F16, 1)
+    lib.linear_softmax_loss(torch.empty(3, device="cuda"), torch.empty(3, device="cuda"), x, w, label)
+    torch.cuda.synchronize()
+    runs = []
+    for n, v, h in ((900, 9000, 1304), (77, 1300, 24)):
+        q = tied(lib, n, v, h, F16, n)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            model_step(lib, *q, torch.cuda.current_stream().cuda_stream)
+        runs.append((q, graph))
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    for _ in range(3):
+        for (q, graph), s in zip(runs, (a, b)):
+            with torch.cuda.stream(s):
+                graph.replay()
+    torch.cuda.synchronize()
+    for q, _ in runs:
+        got = q[3].clone()
+        model_step(lib, *q, None)
+        torch.cuda.synchronize()
+        assert torch.equal(got, q[3])
+
+
+@pytest.mark.gpu
+def test_offsets_beyond_32_bits(lib):
+    """Tables and token matrices of more than 2^31 elements: rows at the far end."""
+    v, h, n = 530000, 4104, 40
+    g = gen(1)
+    w = torch.empty(v, h, dtype=BF16, device="cuda")
+    for at in range(0, v, 50000):
+        w[at:at + 50000] = torch.randn(min(50000, v - at), h, device="cuda", generator=g) * (2.0 / h ** 0.5)
+    index = torch.tensor([v - 1, 0, v - 2, v // 2] * (n // 4), dtype=torch.int32, device="cuda")
+    x = torch.empty(n, h, dtype=BF16, device="cuda")
+    lib.embed_take(x, w, index)
+    assert torch.equal(x, w[index.long()])
+    label = index.flip(0).contiguous()
+    loss, lse = torch.empty(n, device="cuda"), torch.empty(n, device="cuda")
+    lib.linear_softmax_loss(loss, lse, x, w, label)
+    z = torch.cat([x.double() @ w[at:at + 50000].double().t() for at in range(0, v, 50000)], 1)
+    want = torch.logsumexp(z, 1)
+    e_z = (h + 8) * ADD * max((x.abs().double() @ w[at:at + 50000].abs().double().t()).max().item() for at in range(0, v, 50000))
+    assert ((lse.double() - want).abs() <= e_z + 2.0 ** -15 + 2 * ADD * want.abs()).all()
+    gw, gx = torch.empty_like(w), torch.empty_like(x)
+    lib.linear_softmax_loss_grad(gx, gw, x, w, label, lse, scale=1.0 / n)
+    far = torch.arange(v - 5, v, device="cuda")
+    d = (z[:, far] - want[:, None]).exp() - (label[:, None] == far[None]).double()
+    ref = d.t() @ x.double() / n
+    assert ((gw[far].double() - ref).abs() <= (U[BF16] * 4) * (d.abs().t() @ x.abs().double()) / n + 1e-7).all()
+    lib.embed_take_grad(gw, gx, index)
+    ref = torch.zeros(5, h, dtype=torch.float64, device="cuda")
+    for i in range(n):
+        if int(index[i]) >= v - 5:
+            ref[int(index[i]) - (v - 5)] += gx[i].double()
+    assert ((gw[far].double() - ref).abs() <= U[BF16] * 2 * ref.abs() + 1e-9).all()
+    del w, gw, z
+    torch.cuda.empty_cache()
+    n, v, h = 530000, 48, 4104
+    x = torch.empty(n, h, dtype=F16, device="cuda")
+    for at in range(0, n, 50000):
+        x[at:at + 50000] = torch.randn(min(50000, n - at), h, device="cuda", generator=g)
+    w = (torch.randn(v, h, device="cuda", generator=g) * (2.0 / h ** 0.5)).to(F16)
+    label = torch.randint(0, v, (n,), device="cuda", generator=g).to(torch.int32)
+    label[7] = -1
+    loss, lse = torch.empty(n, device="cuda"), torch.empty(n, device="cuda")
+    lib.linear_softmax_loss(loss, lse, x, w, label)
+    gx = torch.empty_like(x)
+    lib.linear_softmax_loss_grad(gx, None, x, w, label, lse)
+    far = slice(n - 300, n)
+    want, wlse, e_loss, e_lse, q = loss_oracle(x[far], w, label[far], -1, 0.0)
+    within(loss[far], want, e_loss, "loss")
+    wx, bx, _, _ = grad_bounds(q, None, 1.0, F16, F16)
+    within(gx[far], wx, bx, "gdata")
+    assert (gx[7] == 0).all()
