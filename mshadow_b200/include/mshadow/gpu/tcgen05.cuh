@@ -106,9 +106,12 @@ __device__ __forceinline__ uint32_t MapToRank(uint32_t saddr, uint32_t rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(saddr), "r"(rank));
   return r;
 }
-/*! \brief one arrival on a barrier of any CTA of the cluster */
+/*!
+ * \brief one arrival on a barrier of any CTA of the cluster, without ordering memory: for handing back accumulators whose
+ *  loads have completed (a releasing arrival waits for the warp's stores to global memory first)
+ */
 __device__ __forceinline__ void ArriveCluster(uint32_t cluster_addr) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 
 // ---- tiled copies ----------------------------------------------------------------------------
@@ -148,27 +151,14 @@ __device__ __forceinline__ void StoreBox(const CUtensorMap *map, int x, int y, u
   }
   asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
-/*! \brief all but the last kPending of this thread's stores have read their shared memory */
-template <int kPending>
-__device__ __forceinline__ void WaitStoresRead() {
-  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kPending) : "memory");
-}
+/*! \brief this thread's stores have read their shared memory */
+__device__ __forceinline__ void WaitStoresRead() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
 /*! \brief this thread's stores have been written */
 __device__ __forceinline__ void WaitStores() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 
 /*! \brief barrier of `threads` threads (whole warps), number `id` of 1 .. 15 */
 __device__ __forceinline__ void NamedBarrier(int id, int threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
-}
-/*! \brief the same, true if `ok` holds for all of them */
-__device__ __forceinline__ bool NamedBarrierAnd(int id, int threads, bool ok) {
-  uint32_t r;
-  asm volatile(
-      "{\n.reg .pred p, q;\nsetp.ne.u32 p, %3, 0;\nbar.red.and.pred q, %1, %2, p;\nselp.u32 %0, 1, 0, q;\n}\n"
-      : "=r"(r)
-      : "r"(id), "r"(threads), "r"(ok ? 1u : 0u)
-      : "memory");
-  return r != 0;
 }
 // ---- tensor memory and products ---------------------------------------------------------------
 
@@ -264,6 +254,28 @@ __device__ __forceinline__ void WaitColumns(uint32_t (&r)[16]) {
                  "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
                :
                : "memory");
+}
+
+// ---- two binary32 at a time --------------------------------------------------------------------
+
+__device__ __forceinline__ uint64_t Pair(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void Unpair(uint64_t p, float *lo, float *hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(*lo), "=f"(*hi) : "l"(p));
+}
+/*! \brief both sums, both products plus a third: each rounded as __fadd_rn and __fmaf_rn do, at twice their rate */
+__device__ __forceinline__ uint64_t AddPair(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t FmaPair(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
 }
 
 }  // namespace tc5
