@@ -54,8 +54,7 @@ const int kThreads = 384;     // warp 0: copies, warp 1: products, warp 2: tenso
 const int kHalfN = kTileN / 2;  // columns of a tile that one epilogue group (four warps, a thread per row) takes
 const int kChunkSteps = 16;   // kStat: stages per run of accumulation in tensor memory (1024 contraction elements)
 const uint32_t kBoxOut = 128 * 128;  // a box of 128 rows by 128 bytes, on its way out through shared memory
-const int kWideSteps = 96;    // stages from which a gradient is computed in tiles of 512 columns
-const int kWideDeltaSteps = 48;  // the same for d, whose columns stay at least two rounds of tiles (64 steps: 7 % faster, 32: even, 16: 15 % slower)
+const int kWideSteps = 24;    // steps from which d and grad W are computed in tiles of 512 columns (below)
 const int kPadRows = 256;     // token rows of the scratch matrices are padded to this
 const float kLog2e = 1.4426950408889634f;
 
@@ -1104,19 +1103,50 @@ inline int CtasFor(int64_t rows, int64_t other_tiles, int sms) {
 }
 
 /*!
- * \brief tiles of 512 columns (kWide) for a gradient with `tiles` tiles of 256, `h_tiles` side by side, and a contraction
- *  of `steps`: enough of them that whole rounds over the SMs lose little, and steps enough that emptying a tile
- *  while nothing multiplies (some 8000 cycles) costs less than the quarter of the loads that is saved
+ * \brief tiles of 512 columns (kWide) for a product with `tiles` tiles of 256, `across` of them side by side, and a
+ *  contraction of `steps`: steps enough that emptying a tile while nothing multiplies costs less than the quarter
+ *  of the copies that is saved (grad W: 14 % less time at 128 steps, 13 % at 64, 7 % at 32; d: 7 % at 64, 5 % at 32, 4 %
+ *  more at 16), and tiles enough that whole rounds over the SMs lose little
  */
-inline bool WideFor(int64_t tiles, int64_t h_tiles, int64_t steps, int sms) {
-  return h_tiles % 2 == 0 && tiles / 2 >= sms && steps >= kWideSteps;
+inline bool WideFor(int64_t tiles, int64_t across, int64_t steps, int sms) {
+  return across % 2 == 0 && tiles / 2 >= sms && steps >= kWideSteps;
+}
+/*!
+ * \brief cycles that CutOf counts for a step of a tile: as measured with all SMs busy (the operand copies, not the
+ *  products, set them).  Tiles of grad x: 0 = one CTA, 128 x 256; 1 = a pair, 256 x 256; 2 = a pair, 256 x 512
+ */
+inline double StepCycles(int shape) { return shape == 0 ? 850.0 : shape == 1 ? 810.0 : 1250.0; }
+/*! \brief cycles to write a part of a tile and read it again, at about 2400 bytes a cycle */
+inline double TileCycles(int shape) { return (shape == 0 ? 128.0 : 256.0) * (shape == 2 ? 512.0 : 256.0) * 8.0 / 2400.0; }
+/*!
+ * \brief the tile shape of grad x for n tokens, h_tiles blocks of 256 features and a contraction of `steps` (the vocabulary
+ *  piece): the one whose best cut (CutOf) costs least when all tokens count.  Wide tiles where there are enough
+ *  rows (8192 x 4096: 10 % less time than 256 x 256, 2048 x 4096: 14 %, 4096 x 1024: 12 %), single CTAs for 257 rows
+ */
+inline int DataShape(int64_t n, int64_t h_tiles, int64_t steps, int sms) {
+  int best = 0;
+  double least = 0.0;
+  for (int shape = 0; shape < 3; ++shape) {
+    if (shape == 2 && (h_tiles % 2 != 0 || steps < 4 * kWideSteps)) continue;
+    const int64_t slots = shape == 0 ? sms : sms / 2;
+    const int64_t tiles = Ceil(n, shape == 0 ? 128 : 256) * (shape == 2 ? h_tiles / 2 : h_tiles);
+    const int64_t full = tiles / slots, rest = tiles % slots;
+    double cut = 0.0;
+    for (int64_t parts = 1; parts <= 16 && rest > 0 && (parts == 1 || (parts * 8 <= steps && parts * rest <= 4 * slots)); ++parts) {
+      const double cost = Ceil(rest * parts, slots) * (Ceil(steps, parts) * StepCycles(shape) + 4000.0) + parts * rest * TileCycles(shape);
+      if (parts == 1 || cost < cut) cut = cost;
+    }
+    const double cost = full * (steps * StepCycles(shape) + 4000.0) + cut;
+    if (shape == 0 || cost < least) least = cost, best = shape;
+  }
+  return best;
 }
 
 /*! \brief how a call is cut, and where its scratch matrices lie (offsets in bytes) */
 struct Plan {
   bool pack, copy_w;
   int64_t pad_rows, ld_x, ld_w, piece, ld_acc, tile_n, tiles;
-  int room, ctas, ctas_gx;
+  int room, ctas, ctas_gx, shape_gx;
   bool wide_gx;
   int64_t counts, words, row_of, pos_of, label_of, lse2, row_scale, x, w, part, part_sum, label_logit, delta, acc, spare, bytes;
 };
@@ -1145,9 +1175,9 @@ inline Plan MakePlan(int64_t n, int64_t v, int64_t h, bool gradient, bool want_g
   }
   p.tiles = Ceil(v, p.tile_n);
   const int64_t h_tiles = p.ld_acc / kTileN;
-  p.ctas_gx = CtasFor(n, h_tiles, sms);
-  const int64_t x_tiles = Ceil(n, 128 * p.ctas_gx);
-  p.wide_gx = p.ctas_gx == 2 && WideFor(x_tiles * h_tiles, h_tiles, Ceil(p.piece, kStepK), sms);
+  p.shape_gx = DataShape(n, h_tiles, Ceil(std::min(p.piece, v), kStepK), sms);
+  p.ctas_gx = p.shape_gx == 0 ? 1 : 2;
+  p.wide_gx = p.shape_gx == 2;
   p.room = 4 * (sms / p.ctas_gx);  // parts of tiles: four rounds over the GPU
   int64_t at = 0;
   auto take = [&at](int64_t bytes) {
@@ -1379,7 +1409,7 @@ inline void BackwardLaunch(const GradOut &g, const Problem &q, const Plan &p, ch
     a.group = GroupOf(m_tiles, 16);
     a.instr = tc5::InstrDesc(q.bf16, false, false, 128 * p.ctas, kTileN);
     const CUtensorMap w_along = WeightMap(q, p, ws, p0, cols, kTileN / p.ctas, stream, true, &a.b_row0);
-    if (p.ctas == 2 && a.n_tiles % 2 == 0 && m_tiles * a.n_tiles >= 4 * sms && a.k_blocks >= kWideDeltaSteps) {
+    if (p.ctas == 2 && WideFor(m_tiles * a.n_tiles, a.n_tiles, a.k_blocks, sms)) {
       a.n_tiles /= 2;
       LaunchGemm<kDelta, 2, true>(x_along, w_along, x_along_in_place, d_along, a, m_tiles * a.n_tiles, sms, stream);
     } else {
@@ -1393,8 +1423,8 @@ inline void BackwardLaunch(const GradOut &g, const Problem &q, const Plan &p, ch
           tc5::MatrixMap(ws + p.spare, kFloat32, static_cast<int64_t>(p.room) * 128 * p.ctas_gx, tile_n, tile_n, 128);
       const int64_t x_tiles = Ceil(q.n, 128 * p.ctas_gx);
       a.n_tiles = p.wide_gx ? h_tiles / 2 : h_tiles;
-      a.step_cycles = p.wide_gx ? 1024.0f : p.ctas_gx == 1 ? 560.0f : 512.0f;
-      a.tile_cycles = static_cast<float>(128 * p.ctas_gx * kTileN * (p.wide_gx ? 2 : 1) * 8) / 2400.0f;
+      a.step_cycles = static_cast<float>(StepCycles(p.shape_gx));
+      a.tile_cycles = static_cast<float>(TileCycles(p.shape_gx));
       a.k_blocks = static_cast<int32_t>(Ceil(cols, kStepK));
       a.k_plan = static_cast<int32_t>(Ceil(std::min(p.piece, q.v), kStepK));
       a.room = p.room;
