@@ -479,6 +479,40 @@ __device__ __forceinline__ void WeightColumns(const uint32_t (&r)[32], int64_t r
 }
 
 /*!
+ * \brief 32 columns of grad W of the warp's 32 rows, for rows that start at any element: the accumulators change places
+ *  in shared memory (the warp's own part of the outgoing box), so that a warp writes a row's 32 columns at
+ *  once instead of every thread its own row, element by element (60000 x 300 bf16: 202 us, now 72)
+ */
+__device__ __forceinline__ void WeightRows(const uint32_t (&r)[32], const Half &t, int64_t row0, int col, float inv,
+                                           const GemmArgs &a) {
+  const int lane = t.thread & 31;
+  __syncwarp();
+#pragma unroll
+  for (int q = 0; q < 8; ++q) BoxPut(t, q, r[4 * q], r[4 * q + 1], r[4 * q + 2], r[4 * q + 3]);
+  __syncwarp();
+  const bool in = col + lane < a.out_cols;
+  const uint32_t box = t.Box() + (t.thread & ~31) * 128;
+  const int64_t first = (row0 + (t.thread & ~31)) * a.ld_out + col + lane;
+  const int rows = static_cast<int>(min(static_cast<int64_t>(32), a.out_rows - (row0 + (t.thread & ~31))));
+#pragma unroll 8
+  for (int i = 0; i < rows; ++i) {
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(box + i * 128 + (((lane >> 2) ^ (i & 7)) << 4) + (lane & 3) * 4) : "memory");
+    v *= inv;
+    if (!in) continue;
+    if (a.out_type == kFloat32) {
+      float *out = static_cast<float *>(a.out) + first + i * a.ld_out;
+      *out = a.out_add ? *out + v : v;
+    } else {
+      const int bf16 = a.out_type == kBfloat16;
+      uint16_t *out = static_cast<uint16_t *>(a.out) + first + i * a.ld_out;
+      if (a.out_add) v += Widen(*out, bf16);
+      *out = static_cast<uint16_t>(PackPair(v, 0.0f, bf16) & 0xffffu);
+    }
+  }
+}
+
+/*!
  * \brief persistent product kernel of all four modes.  kCtas CTAs (a cluster) share a tile of
  *  128 * kCtas rows by 256 columns (kStat: a.tile_n; kWide: 512).  Dynamic shared memory StageShape::kSmem.
  *
@@ -712,7 +746,8 @@ VocabGemmKernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
               uint32_t r[32];
               tc5::LoadColumns(t.acc + c * 32, r);
               tc5::WaitColumns(r);
-              if (t.row < a.out_rows) WeightColumns(r, t.row, t.col + c * 32, inv, a);
+              if (!a.out_vec) WeightRows(r, t, row0, t.col + c * 32, inv, a);
+              else if (t.row < a.out_rows) WeightColumns(r, t.row, t.col + c * 32, inv, a);
             }
           }
         }
@@ -885,13 +920,24 @@ __global__ void __launch_bounds__(256) PackRowsKernel(const PackArgs a) {
   }
 }
 
-/*! \brief copies rows of 16-bit elements to rows that start on 16-byte boundaries */
+/*!
+ * \brief copies rows of 16-bit elements to rows that start on 16-byte boundaries: a thread assembles eight elements (the
+ *  groups of all rows dealt out to threads; a CTA per row and an element per thread took three times as long)
+ */
 template <int kUnused>
 __global__ void __launch_bounds__(256)
-AlignRowsKernel(uint16_t *dst, int64_t ld_dst, const uint16_t *src, int64_t ld_src, int rows, int cols) {
+AlignRowsKernel(uint16_t *dst, int64_t ld_dst, const uint16_t *src, int64_t ld_src, int64_t total, gpu_rt::FastDiv groups,
+                int cols) {
   gpu_rt::GridDependencySync();
-  for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
-    for (int c = threadIdx.x; c < cols; c += 256) dst[r * ld_dst + c] = src[r * ld_src + c];
+  for (int64_t e = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; e < total; e += static_cast<int64_t>(gridDim.x) * 256) {
+    uint32_t row;
+    const int col = static_cast<int>(groups.DivMod(static_cast<uint32_t>(e), &row)) * 8;
+    const uint16_t *from = src + row * ld_src + col;
+    uint32_t w[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w[j] = col + j < cols ? from[j] : 0u;
+    *reinterpret_cast<uint4 *>(dst + row * ld_dst + col) =
+        make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16);
   }
 }
 
@@ -1209,7 +1255,7 @@ inline Plan MakePlan(int64_t n, int64_t v, int64_t h, bool gradient, bool want_g
 
 /*! \brief the kernels count tiles in 32 bits */
 inline void CheckExtents(const Problem &q) {
-  CHECK(q.n <= (int64_t(1) << 30) && Ceil(q.n, 4) * Ceil(q.h, 8) < (int64_t(1) << 30) && Ceil(q.n, 128) * Ceil(q.v, 16) < (int64_t(1) << 31) &&
+  CHECK(q.n <= (int64_t(1) << 30) && q.h < (int64_t(1) << 22) && Ceil(q.n, 4) * Ceil(q.h, 8) < (int64_t(1) << 30) && Ceil(q.n, 128) * Ceil(q.v, 16) < (int64_t(1) << 31) &&
         Ceil(q.v, 128) * Ceil(q.h, 256) < (int64_t(1) << 31))
       << "LinearSoftmaxLoss: more tokens, classes or features than one call covers";
 }
@@ -1283,8 +1329,10 @@ inline CUtensorMap WeightMap(const Problem &q, const Plan &p, char *ws, int64_t 
   }
   uint16_t *w = reinterpret_cast<uint16_t *>(ws + p.w);
   if (copy_now) {
-    gpu_rt::LaunchAfterDrain(AlignRowsKernel<0>, dim3(static_cast<unsigned>(std::min<int64_t>(rows, 4096))), dim3(256), 0,
-                             stream, w, p.ld_w, q.w + p0 * q.ld_w, q.ld_w, static_cast<int>(rows), static_cast<int>(q.h));
+    const int64_t groups = Ceil(q.h, 8), total = rows * groups;  // below 2^31: a piece holds at most 2^30 elements
+    gpu_rt::LaunchAfterDrain(AlignRowsKernel<0>, dim3(static_cast<unsigned>(std::min<int64_t>(Ceil(total, 256), 4096))), dim3(256),
+                             0, stream, w, p.ld_w, q.w + p0 * q.ld_w, q.ld_w, total, gpu_rt::FastDiv(static_cast<uint32_t>(groups)),
+                             static_cast<int>(q.h));
     MSHADOW_CUDA_POST_KERNEL_CHECK(AlignRowsKernel);
   }
   *row0 = 0;
