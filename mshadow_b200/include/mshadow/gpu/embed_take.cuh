@@ -44,9 +44,17 @@ const int kZeroRows = 32;     // table rows per CTA that writes zeros
 
 // ---- element types: groups of 16 bytes (or single elements) as binary32 ----------------------------
 
-template <typename T, bool kVec>
+/*!
+ * \brief how rows are accessed: kOne element at a time; kAligned, 16-byte groups; kAnywhere, rows that start at any
+ *  element: two 32-bit elements or one 16-bit element per thread.  16-bit elements in fours spread each store of
+ *  a warp over four times the sectors: 16384 gradient rows of 2047 into 131072, assigned, took 414 us instead
+ *  of 198; 32-bit elements in twos take 246 us there, one at a time 264.
+ */
+enum Form { kOne = 0, kAligned = 1, kAnywhere = 2 };
+
+template <typename T, int kVec>
 struct Group {
-  static const int kLanes = kVec ? 16 / static_cast<int>(sizeof(T)) : 1;
+  static const int kLanes = (kVec == kAligned ? 16 / static_cast<int>(sizeof(T)) : kVec == kAnywhere && sizeof(T) == 4 ? 2 : 1);
 };
 
 __device__ __forceinline__ float ToFloat(float v) { return v; }
@@ -59,47 +67,55 @@ __device__ __forceinline__ void FromFloat(float v, bfloat::bf16_t *out) {
 }
 
 /*! \brief raw bits of one group */
-template <typename T, bool kVec>
+template <typename T, int kVec>
 struct Bits {
+  T raw[Group<T, kVec>::kLanes];
+};
+template <typename T>
+struct Bits<T, kAligned> {
   uint4 raw;
 };
-template <typename T>
-struct Bits<T, false> {
-  T raw;
-};
 
+/*! \brief `left`: elements of the row from p on; an aligned group is whole */
 template <typename T>
-__device__ __forceinline__ void LoadStream(const T *p, Bits<T, true> *b) {
+__device__ __forceinline__ void LoadStream(const T *p, uint32_t, Bits<T, kAligned> *b) {
   b->raw = __ldcs(reinterpret_cast<const uint4 *>(p));
 }
 template <typename T>
-__device__ __forceinline__ void LoadStream(const T *p, Bits<T, false> *b) {
-  b->raw = *p;
-}
-template <typename T>
-__device__ __forceinline__ void Load(const T *p, Bits<T, true> *b) {
+__device__ __forceinline__ void Load(const T *p, uint32_t, Bits<T, kAligned> *b) {
   b->raw = *reinterpret_cast<const uint4 *>(p);
 }
 template <typename T>
-__device__ __forceinline__ void Load(const T *p, Bits<T, false> *b) {
-  b->raw = *p;
-}
-template <typename T>
-__device__ __forceinline__ void Store(T *p, const Bits<T, true> &b) {
+__device__ __forceinline__ void Store(T *p, uint32_t, const Bits<T, kAligned> &b) {
   *reinterpret_cast<uint4 *>(p) = b.raw;
 }
-template <typename T>
-__device__ __forceinline__ void Store(T *p, const Bits<T, false> &b) {
-  *p = b.raw;
+template <typename T, int kVec>
+__device__ __forceinline__ void Load(const T *p, uint32_t left, Bits<T, kVec> *b) {
+#pragma unroll
+  for (int l = 0; l < Group<T, kVec>::kLanes; ++l) {
+    if (l < static_cast<int>(left)) b->raw[l] = p[l];
+    else memset(&b->raw[l], 0, sizeof(T));
+  }
 }
-template <typename T, bool kVec>
+template <typename T, int kVec>
+__device__ __forceinline__ void LoadStream(const T *p, uint32_t left, Bits<T, kVec> *b) {
+  Load(p, left, b);
+}
+template <typename T, int kVec>
+__device__ __forceinline__ void Store(T *p, uint32_t left, const Bits<T, kVec> &b) {
+#pragma unroll
+  for (int l = 0; l < Group<T, kVec>::kLanes; ++l) {
+    if (l < static_cast<int>(left)) p[l] = b.raw[l];
+  }
+}
+template <typename T, int kVec>
 __device__ __forceinline__ void Unpack(const Bits<T, kVec> &b, float (&v)[Group<T, kVec>::kLanes]) {
   T e[Group<T, kVec>::kLanes];
   memcpy(e, &b.raw, sizeof(e));
 #pragma unroll
   for (int l = 0; l < Group<T, kVec>::kLanes; ++l) v[l] = ToFloat(e[l]);
 }
-template <typename T, bool kVec>
+template <typename T, int kVec>
 __device__ __forceinline__ void Pack(const float (&v)[Group<T, kVec>::kLanes], Bits<T, kVec> *b) {
   T e[Group<T, kVec>::kLanes];
 #pragma unroll
@@ -110,18 +126,18 @@ __device__ __forceinline__ void Pack(const float (&v)[Group<T, kVec>::kLanes], B
 // ---- look-up -------------------------------------------------------------------------------------------
 
 /*!
- * \brief grid-stride over (token, group) pairs, four per thread and sweep: the look-ups of the four row numbers and
- *  then the four groups are in flight together
+ * \brief rows on 16-byte boundaries: grid-stride over (token, group) pairs, four per thread and sweep: the look-ups of the
+ *  four row numbers and then the four groups are in flight together
  */
-template <typename T, bool kVec>
+template <typename T>
 __global__ void __launch_bounds__(256)
 EmbedTakeKernel(T *out, int64_t ld_out, const int32_t *index, const T *table, int64_t ld_table, uint32_t total,
                 gpu_rt::FastDiv groups, int32_t rows, float scale) {
   gpu_rt::GridDependencySync();
-  typedef Group<T, kVec> G;
+  typedef Group<T, kAligned> G;
   const uint32_t step = gridDim.x * 256;
   for (uint32_t e0 = blockIdx.x * 256 + threadIdx.x; e0 < total; e0 += 4 * step) {
-    Bits<T, kVec> b[4];
+    Bits<T, kAligned> b[4];
     uint32_t token[4], col[4];
     int32_t r[4];
 #pragma unroll
@@ -136,82 +152,86 @@ EmbedTakeKernel(T *out, int64_t ld_out, const int32_t *index, const T *table, in
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       memset(&b[u], 0, sizeof(b[u]));
-      if (r[u] >= 0 && r[u] < rows) Load(table + r[u] * ld_table + col[u], &b[u]);
+      if (r[u] >= 0 && r[u] < rows) Load(table + r[u] * ld_table + col[u], G::kLanes, &b[u]);
     }
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       if (e0 + u * step >= total) continue;
       float v[G::kLanes];
-      Unpack<T, kVec>(b[u], v);
+      Unpack<T, kAligned>(b[u], v);
       const bool named = r[u] >= 0 && r[u] < rows;
 #pragma unroll
       for (int l = 0; l < G::kLanes; ++l) v[l] = named ? v[l] * scale : 0.0f;
-      Pack<T, kVec>(v, &b[u]);
-      Store(out + token[u] * ld_out + col[u], b[u]);
+      Pack<T, kAligned>(v, &b[u]);
+      Store(out + token[u] * ld_out + col[u], G::kLanes, b[u]);
     }
   }
 }
 
+const int kTakeDeep = 8;            // loads of a lane in flight
+const uint32_t kTakeSegment = 512;  // elements of a row taken at a time where rows start anywhere
+
 /*!
- * \brief 16-bit elements whose rows start at any 2-byte address: two elements at a time, stored as the 4-byte words
- *  of the output row; the first and last element of a row that fill no word go to one more slot
+ * \brief rows that start at any element: a segment of a row goes to 4 to 32 lanes, so that what depends on the row is found once,
+ *  and 16-bit elements go in pairs, as the 4-byte words of the output row (its first and last element may be
+ *  left over).  16384 x 2047 bf16: 50 us; with row and column found for each pair of elements 79 us.
  */
 template <typename T>
 __global__ void __launch_bounds__(256)
-EmbedTakeOddKernel(T *out, int64_t ld_out, const int32_t *index, const T *table, int64_t ld_table, uint32_t total,
-                   gpu_rt::FastDiv slots, uint32_t width, int32_t rows, float scale) {
+EmbedTakeAnywhereKernel(T *out, int64_t ld_out, const int32_t *index, const T *table, int64_t ld_table, uint32_t total,
+                        gpu_rt::FastDiv segments, uint32_t width, int32_t rows, float scale, int lanes_log2) {
   gpu_rt::GridDependencySync();
-  const uint32_t step = gridDim.x * 256;
-  for (uint32_t e0 = blockIdx.x * 256 + threadIdx.x; e0 < total; e0 += 4 * step) {
-    uint32_t token[4], slot[4];
-    int32_t r[4];
-    T v[4][2];
+  constexpr int kDeep = kTakeDeep;
+  const uint32_t lanes = 1u << lanes_log2, lane = threadIdx.x & (lanes - 1);
+  const uint32_t teams = gridDim.x * (256u >> lanes_log2);
+  for (uint32_t e = blockIdx.x * (256u >> lanes_log2) + (threadIdx.x >> lanes_log2); e < total; e += teams) {
+    uint32_t token;
+    const uint32_t begin = segments.DivMod(e, &token) * kTakeSegment, end = min(width, begin + kTakeSegment);
+    const int32_t r = index[token];
+    const bool named = r >= 0 && r < rows;
+    T *dst = out + token * ld_out;
+    const T *src = table + (named ? r : 0) * ld_table;
+    if (sizeof(T) == 2) {
+      const uint32_t head = begin + (static_cast<uint32_t>(reinterpret_cast<uintptr_t>(dst + begin) >> 1) & 1u);
+      const uint32_t words = end > head ? (end - head) / 2 : 0;
+      const bool even = reinterpret_cast<uintptr_t>(src + head) % 4 == 0;
+      for (uint32_t w0 = lane; w0 < words; w0 += lanes * kDeep) {
+        T v[kDeep][2];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const uint32_t e = e0 + u * step;
-      r[u] = -1;
-      if (e < total) {
-        slot[u] = slots.DivMod(e, &token[u]);
-        r[u] = index[token[u]];
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      if (e0 + u * step >= total) continue;
-      memset(v[u], 0, sizeof(v[u]));
-      if (r[u] < 0 || r[u] >= rows) continue;
-      const uint32_t head = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(out + token[u] * ld_out) >> 1) & 1u;
-      const uint32_t words = (width - head) / 2;
-      const T *src = table + r[u] * ld_table;
-      if (slot[u] < words) {
-        src += head + 2 * slot[u];
-        if (reinterpret_cast<uintptr_t>(src) % 4 == 0) {
-          const uint32_t w = *reinterpret_cast<const uint32_t *>(src);
-          memcpy(v[u], &w, 4);
-        } else {
-          v[u][0] = src[0], v[u][1] = src[1];
+        for (int u = 0; u < kDeep; ++u) {
+          const T *from = src + head + 2 * (w0 + lanes * u);
+          if (w0 + lanes * u >= words || !named) {
+            memset(v[u], 0, sizeof(v[u]));
+          } else if (even) {
+            memcpy(v[u], reinterpret_cast<const uint32_t *>(from), 4);
+          } else {
+            v[u][0] = from[0], v[u][1] = from[1];
+          }
         }
-      } else {
-        v[u][0] = src[0];
-        if (head + 2 * words < width) v[u][1] = src[width - 1];
-      }
-    }
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      if (e0 + u * step >= total) continue;
-      const bool named = r[u] >= 0 && r[u] < rows;
-      T *row = out + token[u] * ld_out;
-      const uint32_t head = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(row) >> 1) & 1u;
-      const uint32_t words = (width - head) / 2;
-      FromFloat(named ? ToFloat(v[u][0]) * scale : 0.0f, &v[u][0]);
-      FromFloat(named ? ToFloat(v[u][1]) * scale : 0.0f, &v[u][1]);
-      if (slot[u] < words) {
-        uint32_t w;
-        memcpy(&w, v[u], 4);
-        *reinterpret_cast<uint32_t *>(row + head + 2 * slot[u]) = w;
-      } else if (slot[u] == words) {
-        if (head) row[0] = v[u][0];
-        if (head + 2 * words < width) row[width - 1] = v[u][1];
+        for (int u = 0; u < kDeep; ++u) {
+          if (w0 + lanes * u >= words) continue;
+          T o[2];
+          FromFloat(named ? ToFloat(v[u][0]) * scale : 0.0f, &o[0]);
+          FromFloat(named ? ToFloat(v[u][1]) * scale : 0.0f, &o[1]);
+          uint32_t bits;
+          memcpy(&bits, o, 4);
+          *reinterpret_cast<uint32_t *>(dst + head + 2 * (w0 + lanes * u)) = bits;
+        }
+      }
+      const uint32_t rest = lane == 0 ? begin : head + 2 * words;  // the elements before the first and behind the last word
+      if ((lane == 0 && head > begin && begin < end) || (lane == 1 && rest < end)) {
+        FromFloat(named ? ToFloat(src[rest]) * scale : 0.0f, &dst[rest]);
+      }
+    } else {
+      for (uint32_t c0 = begin + lane; c0 < end; c0 += lanes * kDeep) {
+        float v[kDeep];
+#pragma unroll
+        for (int u = 0; u < kDeep; ++u) v[u] = c0 + lanes * u < end && named ? ToFloat(src[c0 + lanes * u]) : 0.0f;
+#pragma unroll
+        for (int u = 0; u < kDeep; ++u) {
+          if (c0 + lanes * u < end) FromFloat(named ? v[u] * scale : 0.0f, &dst[c0 + lanes * u]);
+        }
       }
     }
   }
@@ -242,14 +262,14 @@ __device__ __forceinline__ float Scaled(float scale, float sum) {
   return __float_as_uint(sum) == 0x80000000u ? sum : __fmul_rn(scale, sum);
 }
 
-template <typename T, bool kVec>
+template <typename T, int kVec>
 __device__ __forceinline__ void WriteRow(const GradArgs<T> &a, int32_t row, uint32_t col,
                                          const float (&acc)[Group<T, kVec>::kLanes]) {
   T *p = a.grad + row * a.ld_grad + col;
   Bits<T, kVec> b;
   float v[Group<T, kVec>::kLanes];
   if (a.add) {
-    Load(p, &b);
+    Load(p, a.width - col, &b);
     Unpack<T, kVec>(b, v);
 #pragma unroll
     for (int l = 0; l < Group<T, kVec>::kLanes; ++l) v[l] = __fadd_rn(v[l], Scaled(a.scale, acc[l]));
@@ -258,11 +278,11 @@ __device__ __forceinline__ void WriteRow(const GradArgs<T> &a, int32_t row, uint
     for (int l = 0; l < Group<T, kVec>::kLanes; ++l) v[l] = __fadd_rn(Scaled(a.scale, acc[l]), 0.0f);
   }
   Pack<T, kVec>(v, &b);
-  Store(p, b);
+  Store(p, a.width - col, b);
 }
 
 /*! \brief zeros for the rows [first, last) whose flag is not set */
-template <typename T, bool kVec>
+template <typename T, int kVec>
 __device__ __forceinline__ void WriteZeros(const GradArgs<T> &a, uint32_t first, uint32_t last, const uint8_t *named) {
   Bits<T, kVec> zero;
   memset(&zero, 0, sizeof(zero));
@@ -270,7 +290,7 @@ __device__ __forceinline__ void WriteZeros(const GradArgs<T> &a, uint32_t first,
   for (uint32_t r = first + warp; r < last; r += warps) {
     if (named[r - first]) continue;
     for (uint32_t c = lane * Group<T, kVec>::kLanes; c < a.width; c += 32 * Group<T, kVec>::kLanes) {
-      Store(a.grad + r * a.ld_grad + c, zero);
+      Store(a.grad + r * a.ld_grad + c, a.width - c, zero);
     }
   }
 }
@@ -292,7 +312,7 @@ __device__ __forceinline__ uint32_t WarpLowerBound(const int32_t *keys, uint32_t
 }
 
 /*! \brief adds the source rows of window entries [from, to) to acc, kDepth of them in flight */
-template <typename T, bool kVec>
+template <typename T, int kVec>
 __device__ __forceinline__ void AddRows(const GradArgs<T> &a, const int32_t *rows, uint32_t from, uint32_t to, uint32_t col,
                                         float (&acc)[Group<T, kVec>::kLanes]) {
   for (uint32_t i = from; i < to; i += kDepth) {
@@ -301,7 +321,7 @@ __device__ __forceinline__ void AddRows(const GradArgs<T> &a, const int32_t *row
 #pragma unroll
     for (int u = 0; u < kDepth; ++u) {
       r[u] = i + u < to ? rows[i + u] : -1;
-      if (r[u] >= 0) LoadStream(a.g + r[u] * a.ld_g + col, &b[u]);
+      if (r[u] >= 0) LoadStream(a.g + r[u] * a.ld_g + col, a.width - col, &b[u]);
     }
 #pragma unroll
     for (int u = 0; u < kDepth; ++u) {
@@ -418,7 +438,7 @@ EmbedSortKernel(int32_t *keys, int32_t *rows, const int32_t *index, uint32_t n, 
  *  rows (and, when adding, the table rows of the runs that end among them) in flight together: with one run
  *  after the other, 600 tokens of mostly different rows took 48 us.
  */
-template <typename T, bool kVec, bool kAdd>
+template <typename T, int kVec, bool kAdd>
 __global__ void __launch_bounds__(256) EmbedSumKernel(const GradArgs<T> a) {
   gpu_rt::GridDependencySync();
   typedef Group<T, kVec> G;
@@ -518,11 +538,11 @@ __global__ void __launch_bounds__(256) EmbedSumKernel(const GradArgs<T> a) {
     for (int u = 0; u < kDepth; ++u) {
       const int p = i + u;
       r[u] = p < to ? s_rows[kChunk + p] : -1;
-      if (r[u] >= 0) LoadStream(a.g + r[u] * a.ld_g + col, &b[u]);
+      if (r[u] >= 0) LoadStream(a.g + r[u] * a.ld_g + col, a.width - col, &b[u]);
       const bool stop = p < to && (p == to - 1 || ((p < 64 ? ends[1] >> p : ends[2] >> (p - 64)) & 1u));
       if (stop) stops |= 1u << u;
       if (kAdd && stop && p >= head && !(tail && p == to - 1)) {
-        Load(a.grad + s_keys[kChunk + p] * a.ld_grad + col, &d[kAdd ? u : 0]);
+        Load(a.grad + s_keys[kChunk + p] * a.ld_grad + col, a.width - col, &d[kAdd ? u : 0]);
       }
     }
 #pragma unroll
@@ -544,7 +564,7 @@ __global__ void __launch_bounds__(256) EmbedSumKernel(const GradArgs<T> a) {
 #pragma unroll
         for (int l = 0; l < G::kLanes; ++l) v[l] = __fadd_rn(Scaled(a.scale, acc[l]), kAdd ? v[l] : 0.0f);
         Pack<T, kVec>(v, &b[u]);
-        Store(a.grad + s_keys[kChunk + p] * a.ld_grad + col, b[u]);
+        Store(a.grad + s_keys[kChunk + p] * a.ld_grad + col, a.width - col, b[u]);
       }
 #pragma unroll
       for (int l = 0; l < G::kLanes; ++l) acc[l] = -0.0f;
@@ -581,7 +601,7 @@ __device__ __forceinline__ void WriteFour(const GradArgs<T> &a, int32_t key, uin
 #pragma unroll
   for (int l = 0; l < 4; ++l) {
     const float one[1] = {acc[l]};
-    if (col + l < a.width) WriteRow<T, false>(a, key, col + l, one);
+    if (col + l < a.width) WriteRow<T, kOne>(a, key, col + l, one);
   }
 }
 
@@ -618,7 +638,7 @@ __global__ void __launch_bounds__(512) EmbedSpanKernel(const GradArgs<T> a) {
       float sum[1] = {s_sum[0][threadIdx.x]};
 #pragma unroll
       for (int q = 1; q < 16; ++q) sum[0] = __fadd_rn(sum[0], s_sum[q][threadIdx.x]);
-      WriteRow<T, false>(a, key, strip + threadIdx.x, sum);
+      WriteRow<T, kOne>(a, key, strip + threadIdx.x, sum);
     }
     __syncthreads();
   }
@@ -637,7 +657,7 @@ __global__ void __launch_bounds__(512) EmbedSpanKernel(const GradArgs<T> a) {
  * \brief short lists, in one launch and without a sort.  grid: n * slabs CTAs, then (when assigning) CTAs that
  *  write zeros.  The CTA of an entry whose index occurred before does nothing.
  */
-template <typename T, bool kVec>
+template <typename T, int kVec>
 __global__ void __launch_bounds__(256) EmbedFewKernel(const GradArgs<T> a) {
   gpu_rt::GridDependencySync();
   typedef Group<T, kVec> G;
@@ -703,35 +723,9 @@ inline bool Aligned(const T *p, int64_t ld, int64_t width) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % lanes == 0 && width % lanes == 0;
 }
 
-inline unsigned TakeGrid(uint32_t total) {
+inline unsigned TakeGrid(uint32_t items, uint32_t per_cta) {
   const int64_t cap = static_cast<int64_t>(gpu_rt::CurrentDevice().sm_count) * 8;
-  return static_cast<unsigned>(std::min<int64_t>((static_cast<int64_t>(total) + 255) / 256, cap));
-}
-
-template <typename T, bool kVec>
-inline void TakeGo(T *out, int64_t ld_out, const int32_t *index, const T *table, int64_t ld_table, int64_t n, int64_t rows,
-                   int64_t width, float scale, cudaStream_t stream) {
-  const uint32_t groups = static_cast<uint32_t>(width / Group<T, kVec>::kLanes);
-  const uint32_t total = static_cast<uint32_t>(n) * groups;
-  gpu_rt::LaunchAfterDrain(EmbedTakeKernel<T, kVec>, dim3(TakeGrid(total)), dim3(256), 0, stream, out, ld_out, index, table,
-                           ld_table, total, gpu_rt::FastDiv(groups), static_cast<int32_t>(rows), scale);
-  MSHADOW_CUDA_POST_KERNEL_CHECK(EmbedTakeKernel);
-}
-
-template <typename T>
-inline void TakeOdd(T *out, int64_t ld_out, const int32_t *index, const T *table, int64_t ld_table, int64_t n, int64_t rows,
-                    int64_t width, float scale, cudaStream_t stream, std::integral_constant<int, 2>) {
-  const uint32_t slots = static_cast<uint32_t>(width / 2 + 1);
-  const uint32_t total = static_cast<uint32_t>(n) * slots;
-  gpu_rt::LaunchAfterDrain(EmbedTakeOddKernel<T>, dim3(TakeGrid(total)), dim3(256), 0, stream, out, ld_out, index, table,
-                           ld_table, total, gpu_rt::FastDiv(slots), static_cast<uint32_t>(width), static_cast<int32_t>(rows),
-                           scale);
-  MSHADOW_CUDA_POST_KERNEL_CHECK(EmbedTakeOddKernel);
-}
-template <typename T>
-inline void TakeOdd(T *out, int64_t ld_out, const int32_t *index, const T *table, int64_t ld_table, int64_t n, int64_t rows,
-                    int64_t width, float scale, cudaStream_t stream, std::integral_constant<int, 4>) {
-  TakeGo<T, false>(out, ld_out, index, table, ld_table, n, rows, width, scale, stream);
+  return static_cast<unsigned>(std::min<int64_t>((static_cast<int64_t>(items) + per_cta - 1) / per_cta, cap));
 }
 
 /*! \brief out[i] = scale * table[index[i]]; rows and columns of the tensors as given by n, rows, width */
@@ -739,13 +733,26 @@ template <typename T>
 inline void TakeLaunch(T *out, int64_t ld_out, const int32_t *index, const T *table, int64_t ld_table, int64_t n,
                        int64_t rows, int64_t width, float scale, cudaStream_t stream) {
   if (n == 0 || width == 0) return;
-  const bool vec = Aligned(out, ld_out, width) && Aligned(table, ld_table, width);
-  // the kernels count (token, group) pairs in 32 bits, with room for a last sweep past the end
-  const int64_t block = std::max<int64_t>(1, (int64_t(1) << 30) / width);
+  const bool aligned = Aligned(out, ld_out, width) && Aligned(table, ld_table, width);
+  const uint32_t pieces = static_cast<uint32_t>(aligned ? width / Group<T, kAligned>::kLanes
+                                                        : (width + kTakeSegment - 1) / kTakeSegment);
+  // the kernels count (token, piece) pairs in 32 bits, with room for a last sweep past the end
+  const int64_t block = std::max<int64_t>(1, (int64_t(1) << 30) / pieces);
   for (int64_t i = 0; i < n; i += block) {
-    const int64_t m = std::min(block, n - i);
-    if (vec) TakeGo<T, true>(out + i * ld_out, ld_out, index + i, table, ld_table, m, rows, width, scale, stream);
-    else TakeOdd<T>(out + i * ld_out, ld_out, index + i, table, ld_table, m, rows, width, scale, stream, std::integral_constant<int, sizeof(T)>());
+    const uint32_t total = static_cast<uint32_t>(std::min(block, n - i)) * pieces;
+    if (aligned) {
+      gpu_rt::LaunchAfterDrain(EmbedTakeKernel<T>, dim3(TakeGrid(total, 256)), dim3(256), 0, stream, out + i * ld_out, ld_out,
+                               index + i, table, ld_table, total, gpu_rt::FastDiv(pieces), static_cast<int32_t>(rows), scale);
+    } else {
+      // as few lanes as take a segment in one sweep of kTakeDeep loads: short rows share a warp
+      const int64_t units = std::min<int64_t>(width, kTakeSegment) * static_cast<int64_t>(sizeof(T)) / 4;
+      int lanes_log2 = 2;
+      while (lanes_log2 < 5 && (int64_t(kTakeDeep) << lanes_log2) < units) ++lanes_log2;
+      gpu_rt::LaunchAfterDrain(EmbedTakeAnywhereKernel<T>, dim3(TakeGrid(total, 256 >> lanes_log2)), dim3(256), 0, stream, out + i * ld_out,
+                               ld_out, index + i, table, ld_table, total, gpu_rt::FastDiv(pieces),
+                               static_cast<uint32_t>(width), static_cast<int32_t>(rows), scale, lanes_log2);
+    }
+    MSHADOW_CUDA_POST_KERNEL_CHECK(EmbedTakeKernel);
   }
 }
 
@@ -777,9 +784,9 @@ inline GradPlan MakeGradPlan(int64_t n, int64_t width) {
   return p;
 }
 
-template <typename T, bool kVec>
+template <typename T, int kVec>
 inline void GradGo(GradArgs<T> a, const GradPlan &p, char *ws, cudaStream_t stream) {
-  const uint32_t items = a.width / Group<T, kVec>::kLanes;
+  const uint32_t items = (a.width + Group<T, kVec>::kLanes - 1) / Group<T, kVec>::kLanes;
   const uint32_t threads = std::min(256u, (items + 31) / 32 * 32);
   a.slabs = (items + threads - 1) / threads;
   const uint32_t zero = a.add ? 0 : (a.table_rows + kZeroRows - 1) / kZeroRows;
@@ -836,8 +843,8 @@ inline void GradLaunch(T *grad, int64_t ld_grad, const T *g, int64_t ld_g, const
   a.grad = grad, a.ld_grad = ld_grad, a.g = g, a.ld_g = ld_g, a.index = index;
   a.n = static_cast<uint32_t>(n), a.width = static_cast<uint32_t>(width), a.table_rows = static_cast<uint32_t>(rows);
   a.scale = scale, a.add = add;
-  if (Aligned(grad, ld_grad, width) && (n == 0 || Aligned(g, ld_g, width))) GradGo<T, true>(a, p, ws, stream);
-  else GradGo<T, false>(a, p, ws, stream);
+  if (Aligned(grad, ld_grad, width) && (n == 0 || Aligned(g, ld_g, width))) GradGo<T, kAligned>(a, p, ws, stream);
+  else GradGo<T, kAnywhere>(a, p, ws, stream);
 }
 
 }  // namespace embtake

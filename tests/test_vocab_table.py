@@ -177,6 +177,27 @@ def test_embed_take(lib, dtype, n, rows, width, pad, offset):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("width", [1, 2, 3, 9, 31, 65, 127, 257, 511, 512, 513, 1025, 1537])
+@pytest.mark.parametrize("at_table,at_out", [(0, 1), (1, 0), (1, 1)])
+def test_embed_take_rows_anywhere(lib, dtype, width, at_table, at_out):
+    """Around the segments and words that rows are cut into, the two sides starting at different parities."""
+    g = gen(width + 2 * at_table + at_out)
+    n, rows = 301, 67
+    table, _ = pitched(rows, width, dtype, 0, at_table)
+    table.copy_(torch.randn(rows, width, device="cuda", generator=g))
+    index = torch.randint(-2, rows + 3, (n,), device="cuda", generator=g).to(torch.int32)
+    out, base = pitched(n, width, dtype, at_out, at_out)
+    before = base.clone()
+    lib.embed_take(out, table, index, scale=-2.0)
+    named = (index >= 0) & (index < rows)
+    want = table[torch.where(named, index, 0).long()].double() * -2.0 * named[:, None]
+    assert torch.equal(out.double(), want)
+    out.copy_(torch.full_like(out, 7.0))
+    assert torch.equal(base, before)
+
+
+@pytest.mark.gpu
 def test_embed_take_special_values(lib):
     """Infinities and NaN in rows that no index names reach nothing; in named rows they come out."""
     table = torch.randn(6, 40, device="cuda").to(BF16)
