@@ -48,7 +48,7 @@ const int kZeroRows = 32;     // table rows per CTA that writes zeros
  * \brief how rows are accessed: kOne element at a time; kAligned, 16-byte groups; kAnywhere, rows that start at any
  *  element: two 32-bit elements or one 16-bit element per thread.  16-bit elements in fours spread each store of
  *  a warp over four times the sectors: 16384 gradient rows of 2047 into 131072, assigned, took 414 us instead
- *  of 198; 32-bit elements in twos take 246 us there, one at a time 264.
+ *  of 198; 32-bit elements in twos: 262144 rows of 511 into 65536 in 212 us, one at a time 264.
  */
 enum Form { kOne = 0, kAligned = 1, kAnywhere = 2 };
 
