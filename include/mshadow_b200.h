@@ -426,7 +426,8 @@ int msb_softmax_grad3d_f32(float *dst, const float *src, const float *label, int
 
    All operands, the workspace too, are memory of the current device (or managed memory): other
    pointers are refused with MSB_ERR_ARGUMENT.  Rows may have any pitch and start at any element;
-   rows on 16-byte boundaries are the fast case.  Labels and indices are int32. */
+   rows on 16-byte boundaries are the fast case.  Labels and indices are int32.  An output shares no
+   element with another operand or the workspace (this is not checked). */
 enum { MSB_FLOAT32 = 0, MSB_FLOAT16 = 2, MSB_BFLOAT16 = 12 };
 
 /* dst[i] = scale * table[index[i]], a row of zeros where index[i] is outside [0, rows): the

@@ -17,8 +17,8 @@
  * data (n x h) and weight (v x h) are binary16 or bfloat16; loss and lse are binary32; gdata has the type of
  * data; gweight that type or float.  Sums are binary32.  A token whose label equals ignore_label, or lies
  * outside [0, v), contributes nothing: its loss and lse are 0, its gdata row is zero, and whatever
- * its data row holds reaches no result.  gdata or gweight may be empty (dptr_ == NULL): not computed.  Equal calls
- * give equal bits.
+ * its data row holds reaches no result.  gdata or gweight may be empty (dptr_ == NULL): not computed.  Outputs share
+ * no element with other operands.  Equal calls give equal bits.
  *
  * `workspace`: at least LinearSoftmaxLossWorkspace() bytes of device memory, or NULL for the stream's scratch memory.
  * A call that is captured into a graph must bring its own.
@@ -65,7 +65,7 @@ template <typename DType>
 inline void LinearSoftmaxLoss(Tensor<gpu, 1, float> loss, Tensor<gpu, 1, float> lse, const Tensor<gpu, 2, DType> &data,
                               const Tensor<gpu, 2, DType> &weight, const Tensor<gpu, 1, int32_t> &label,
                               int ignore_label = -1, float smooth = 0.0f, void *workspace = NULL,
-                          size_t workspace_bytes = 0) {
+                              size_t workspace_bytes = 0) {
   const cuda::vloss::Problem q = vlossdetail::MakeProblem(data, weight, label, ignore_label, smooth);
   CHECK(loss.size(0) == data.size(0) && lse.size(0) == data.size(0)) << "LinearSoftmaxLoss: shape mismatch";
   if (q.n == 0) return;
@@ -81,8 +81,7 @@ inline void LinearSoftmaxLossGrad(Tensor<gpu, 2, DType> gdata, Tensor<gpu, 2, GT
                                   const Tensor<gpu, 2, DType> &data, const Tensor<gpu, 2, DType> &weight,
                                   const Tensor<gpu, 1, int32_t> &label, const Tensor<gpu, 1, float> &lse,
                                   const Tensor<gpu, 1, float> &gloss, float scale, int ignore_label = -1,
-                                  float smooth = 0.0f, void *workspace = NULL,
-                          size_t workspace_bytes = 0) {
+                                  float smooth = 0.0f, void *workspace = NULL, size_t workspace_bytes = 0) {
   static_assert(std::is_same<Saver, sv::saveto>::value || std::is_same<Saver, sv::plusto>::value,
                 "LinearSoftmaxLossGrad assigns or adds the weight's gradient");
   static_assert(std::is_same<GType, DType>::value || std::is_same<GType, float>::value,

@@ -1255,8 +1255,8 @@ inline Plan MakePlan(int64_t n, int64_t v, int64_t h, bool gradient, bool want_g
 
 /*! \brief the kernels count tiles in 32 bits */
 inline void CheckExtents(const Problem &q) {
-  CHECK(q.n <= (int64_t(1) << 30) && q.h < (int64_t(1) << 22) && Ceil(q.n, 4) * Ceil(q.h, 8) < (int64_t(1) << 30) && Ceil(q.n, 128) * Ceil(q.v, 16) < (int64_t(1) << 31) &&
-        Ceil(q.v, 128) * Ceil(q.h, 256) < (int64_t(1) << 31))
+  CHECK(q.n <= (int64_t(1) << 30) && q.h < (int64_t(1) << 22) && Ceil(q.n, 4) * Ceil(q.h, 8) < (int64_t(1) << 30) &&
+        Ceil(q.n, 128) * Ceil(q.v, 16) < (int64_t(1) << 31) && Ceil(q.v, 128) * Ceil(q.h, 256) < (int64_t(1) << 31))
       << "LinearSoftmaxLoss: more tokens, classes or features than one call covers";
 }
 inline Plan PlanForward(const Problem &q, int sms) {
@@ -1452,7 +1452,7 @@ inline void BackwardLaunch(const GradOut &g, const Problem &q, const Plan &p, ch
     const int64_t m_tiles = Ceil(q.n, 128 * p.ctas);
     a.cols = static_cast<int32_t>(cols);
     a.col0 = static_cast<int32_t>(p0);
-      a.n_tiles = static_cast<int32_t>(Ceil(cols, kTileN));
+    a.n_tiles = static_cast<int32_t>(Ceil(cols, kTileN));
     a.k_blocks = static_cast<int32_t>(Ceil(q.h, kStepK));
     a.group = GroupOf(m_tiles, 16);
     a.instr = tc5::InstrDesc(q.bf16, false, false, 128 * p.ctas, kTileN);
@@ -1487,7 +1487,7 @@ inline void BackwardLaunch(const GradOut &g, const Problem &q, const Plan &p, ch
       const int ctas = CtasFor(cols, h_tiles, sms);
       a.m_tiles = static_cast<int32_t>(Ceil(cols, 128 * ctas));
       a.n_tiles = h_tiles;
-          a.b_row0 = 0;
+      a.b_row0 = 0;
       a.group = GroupOf(a.m_tiles, 8);
       a.instr = tc5::InstrDesc(q.bf16, true, true, 128 * ctas, kTileN);
       a.out = static_cast<char *>(g.gw) + p0 * g.ld_gw * elem;
