@@ -723,9 +723,10 @@ VocabGemmKernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
       for (int set = 0; set < S::kSets; ++set, t.col += kTileN) {
         ready();
         if (kMode == kDelta) {
-          // rows past the live ones: lse and scale are 0, the data row is zero, and so is d'
-          DeltaHalf<S::kBoxes>(t, a.cols - t.col, label < 0 ? -1 : label - a.col0 - t.col, a.lse2[t.row], a.row_scale[t.row],
-                               &map_out, row0, a);
+          // rows past the live ones: no column of theirs exists, so that d' is zero there whatever the logits of a zero data
+          // row are (NaN beside a class with an infinite weight); the product for grad W reads them up to a whole step
+          DeltaHalf<S::kBoxes>(t, t.row < live ? a.cols - t.col : 0, label < 0 ? -1 : label - a.col0 - t.col, a.lse2[t.row],
+                               a.row_scale[t.row], &map_out, row0, a);
         } else if (kMode == kDataGrad) {
           // a whole tile goes to its place in the gradient, a part of one to a tile of its own beside it
           const bool whole = u.parts == 1;

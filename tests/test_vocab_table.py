@@ -1032,3 +1032,27 @@ def test_offsets_beyond_32_bits(lib):
     wx, bx, _, _ = grad_bounds(q, None, 1.0, F16, F16)
     within(gx[far], wx, bx, "gdata")
     assert (gx[7] == 0).all()
+
+
+# ---- values that are not finite, and calls that nothing reaches -----------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("n,ignored", [(1, 0.0), (40, 0.0), (64, 0.0), (100, 0.0), (257, 0.0), (300, 0.3), (700, 0.5)])
+def test_loss_grad_infinite_weights(lib, dtype, n, ignored):
+    """Classes at -infinity (a weight that acts as a mask) have no gradient, and the other classes have theirs."""
+    x, w, label = problem(n, 600, 64, dtype, 3, ignored=ignored)
+    x[:, 0] = x[:, 0].abs() + 0.5
+    w[300:] = 0
+    w[300:, 0] = float("-inf")
+    label.clamp_(max=299)
+    loss, lse = torch.empty(n, device="cuda"), torch.empty(n, device="cuda")
+    for gw_dtype in (dtype, F32):
+        for lab in (label, torch.full_like(label, -1)):
+            lib.linear_softmax_loss(loss, lse, x, w, lab)
+            gw = torch.full((600, 64), 5.0, dtype=gw_dtype, device="cuda")
+            lib.linear_softmax_loss_grad(None, gw, x, w, lab, lse, scale=1.0 / n)
+            _, _, _, _, q = loss_oracle(x, w[:300], lab, -1, 0.0)
+            _, _, want, bound = grad_bounds(q, None, 1.0 / n, dtype, gw_dtype)
+            within(gw[:300], want, bound, "gweight beside classes at -infinity")
+            assert (gw[300:] == 0).all()
