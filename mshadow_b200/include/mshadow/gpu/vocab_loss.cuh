@@ -897,7 +897,8 @@ __global__ void __launch_bounds__(256) PackRowsKernel(const PackArgs a) {
   }
   if (blockIdx.x == 0 && tid == 0) {
     a.words[0] = total;
-    reinterpret_cast<float *>(a.words)[1] = a.scale * a.q_label * down;
+    // (with no token that counts the sums are empty, and zero whatever the scale: 1 / 0 tokens, say)
+    reinterpret_cast<float *>(a.words)[1] = total > 0 ? a.scale * a.q_label * down : 0.0f;
     a.words[2] = a.tiled && total == a.n;
   }
   if (a.tiled && total == a.n) return;
@@ -1097,7 +1098,7 @@ __global__ void __launch_bounds__(256) DataGradFinishKernel(const FinishArgs a) 
       if (i0 + r >= a.n) break;
       uint16_t *out = a.out + (i0 + r) * a.ld_out;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[r][j] *= inv;
+      for (int j = 0; j < 8; ++j) v[r][j] = pos[r] >= 0 ? v[r][j] * inv : 0.0f;  // (inv may be infinite)
       if (a.vec && 8 * g + 8 <= a.h) {
         uint4 w;
         w.x = PackPair(v[r][0], v[r][1], a.bf16);

@@ -1056,3 +1056,27 @@ def test_loss_grad_infinite_weights(lib, dtype, n, ignored):
             _, _, want, bound = grad_bounds(q, None, 1.0 / n, dtype, gw_dtype)
             within(gw[:300], want, bound, "gweight beside classes at -infinity")
             assert (gw[300:] == 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scale", [float("inf"), float("nan"), -1.0])
+@pytest.mark.parametrize("n,h", [(40, 64), (700, 72), (300, 33)])
+def test_loss_grad_of_nothing(lib, n, h, scale):
+    """No token counts, and the scale is one over their number: empty sums are zero whatever they are scaled by."""
+    x, w, label = problem(n, 500, h, BF16, 6)
+    dead = torch.full_like(label, -1)
+    loss, lse = torch.empty(n, device="cuda"), torch.empty(n, device="cuda")
+    lib.linear_softmax_loss(loss, lse, x, w, dead)
+    for gw_dtype in (BF16, F32):
+        gx, gw = torch.full_like(x, 5.0), torch.full((500, h), 5.0, dtype=gw_dtype, device="cuda")
+        lib.linear_softmax_loss_grad(gx, gw, x, w, dead, lse, scale=scale)
+        assert (gx == 0).all() and (gw == 0).all()
+        gw.fill_(5.0)
+        lib.linear_softmax_loss_grad(gx, gw, x, w, dead, lse, scale=scale, saver=1)
+        assert (gx == 0).all() and (gw == 5).all()
+    # beside tokens that count the others' rows are zero all the same
+    dead[3] = label[3]
+    lib.linear_softmax_loss(loss, lse, x, w, dead)
+    lib.linear_softmax_loss_grad(gx, gw, x, w, dead, lse, scale=scale)
+    others = torch.arange(n, device="cuda") != 3
+    assert (gx[others] == 0).all() and bool(torch.isfinite(gx[3]).all()) == (scale == -1.0)
