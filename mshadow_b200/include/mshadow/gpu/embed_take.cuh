@@ -257,7 +257,19 @@ struct GradArgs {
                                // the runs of few parts from the front, of many parts from the back
 };
 
-/*! \brief scale * sum; the sum of nothing (a run of entries that name no row) stays it, whatever the scale: adding it changes no value */
+/*!
+ * \brief -0, the sum of nothing: a run of entries that name no row (they are sorted among those of the first and the last row).
+ *  Adding it, or a sum of -0 alone, changes no value, so a row is not written then: another call may be adding to it at
+ *  the same time on another stream, and a NaN would not keep its bits.
+ */
+template <int kLanes>
+__device__ __forceinline__ bool AddsNothing(const float (&sum)[kLanes]) {
+  bool nothing = true;
+#pragma unroll
+  for (int l = 0; l < kLanes; ++l) nothing = nothing && __float_as_uint(sum[l]) == 0x80000000u;
+  return nothing;
+}
+/*! \brief scale * sum; the sum of nothing stays it, whatever the scale */
 __device__ __forceinline__ float Scaled(float scale, float sum) {
   return __float_as_uint(sum) == 0x80000000u ? sum : __fmul_rn(scale, sum);
 }
@@ -269,6 +281,7 @@ __device__ __forceinline__ void WriteRow(const GradArgs<T> &a, int32_t row, uint
   Bits<T, kVec> b;
   float v[Group<T, kVec>::kLanes];
   if (a.add) {
+    if (AddsNothing(acc)) return;
     Load(p, a.width - col, &b);
     Unpack<T, kVec>(b, v);
 #pragma unroll
@@ -559,7 +572,7 @@ __global__ void __launch_bounds__(256) EmbedSumKernel(const GradArgs<T> a) {
         float *part = a.parts + (2 * static_cast<int64_t>(chunk) + (p < head ? 0 : 1)) * a.ld_parts + col;
 #pragma unroll
         for (int l = 0; l < G::kLanes; ++l) part[l] = acc[l];
-      } else {
+      } else if (!kAdd || !AddsNothing(acc)) {
         if (kAdd) Unpack<T, kVec>(d[kAdd ? u : 0], v);
 #pragma unroll
         for (int l = 0; l < G::kLanes; ++l) v[l] = __fadd_rn(Scaled(a.scale, acc[l]), kAdd ? v[l] : 0.0f);

@@ -1080,3 +1080,59 @@ def test_loss_grad_of_nothing(lib, n, h, scale):
     lib.linear_softmax_loss_grad(gx, gw, x, w, dead, lse, scale=scale)
     others = torch.arange(n, device="cuda") != 3
     assert (gx[others] == 0).all() and bool(torch.isfinite(gx[3]).all()) == (scale == -1.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,word,nan", [(F32, torch.int32, 0x7fc12345), (F32, torch.int32, -0x3edcbb), (F16, torch.int16, 0x7e41),
+                                            (F16, torch.int16, -0x1bf), (BF16, torch.int16, 0x7fc1), (BF16, torch.int16, -0x3f)])
+@pytest.mark.parametrize("n", [100, 600, 3000, 9000, 20000])
+@pytest.mark.parametrize("width,at", [(24, 0), (33, 1), (300, 0)])
+def test_rows_not_named_keep_their_bits(lib, dtype, word, nan, n, width, at):
+    """Added gradients leave rows alone that no index names, NaN bits too: dropped indices in lists of every kind of
+    sort, with few and with many entries, beside named rows and by themselves."""
+    rows = 50
+    src, _ = pitched(n, width, dtype, 0, at)
+    src.copy_(torch.randn(n, width, device="cuda", generator=gen(n)))
+    for named, dropped in ((0, n), (n // 2, n // 2), (n - 40, 40), (n - 130, 130), (n - 3, 3)):
+        index = torch.randint(1, rows - 1, (n,), device="cuda", generator=gen(n)).to(torch.int32)
+        index[named:named + dropped] = -1
+        index[named + dropped // 3:named + dropped] = rows + 7
+        dst, _ = pitched(rows, width, dtype, 0, at)
+        bits = torch.full((rows, width), nan, dtype=word, device="cuda")
+        dst.copy_(bits.view(dtype))  # copies keep bits
+        assert torch.equal(dst.contiguous().view(word), bits)
+        lib.embed_take_grad(dst, src, index, scale=0.5, saver=1)
+        left = torch.ones(rows, dtype=torch.bool, device="cuda")
+        left[index[(index >= 0) & (index < rows)].long()] = False
+        assert left[0] and left[rows - 1]
+        assert (dst.contiguous().view(word)[left] == nan).all() and dst[~left].isnan().all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [600, 5000, 12000])
+def test_two_streams_add_into_one_table(lib, n):
+    """Two calls at once into the same table: the rows that they name are disjoint, and both lists hold dropped indices, which
+    are sorted among those of the first and the last row."""
+    rows, width = 40, 2048
+    dst = torch.zeros(rows, width, device="cuda")
+    halves = []
+    for k in range(2):
+        index = torch.randint(0, rows // 2, (n,), device="cuda", generator=gen(k)).to(torch.int32)
+        if k:
+            index += rows // 2  # the last row is named here, the first one there
+        index[::5] = -1 - k
+        index[1::5] = rows + k
+        src = torch.randint(-4, 5, (n, width), device="cuda", generator=gen(9 + k)).float()  # sums are exact
+        ws = torch.empty(lib.embed_take_grad_workspace(n, rows, width), dtype=torch.uint8, device="cuda")
+        halves.append((src, index, ws, torch.cuda.Stream()))
+    want = torch.zeros(rows, width, dtype=torch.float64, device="cuda")
+    for src, index, _, _ in halves:
+        named = (index >= 0) & (index < rows)
+        want.index_add_(0, index[named].long(), src[named].double())
+    torch.cuda.synchronize()
+    calls = 30
+    for _ in range(calls):
+        for src, index, ws, s in halves:
+            lib.embed_take_grad(dst, src, index, saver=1, workspace=ws, stream=s.cuda_stream)
+    torch.cuda.synchronize()
+    assert torch.equal(dst.double(), calls * want)
