@@ -51,6 +51,8 @@ int Guarded(const char *name, Body body) {
   TraceRange range(name);
   try {
     body();
+  } catch (const gpu_rt::WorkspaceError &e) {
+    return Refuse(name, MSB_ERR_ARGUMENT, e.what());
   } catch (const dmlc::Error &e) {
     const std::string what = e.what();
     const bool cuda = what.find("CUDA") != std::string::npos || what.find("ErrStr") != std::string::npos;

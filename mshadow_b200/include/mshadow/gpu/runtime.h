@@ -255,14 +255,25 @@ inline bool IsCapturing(cudaStream_t stream) {
  *  stream, so a call that is recorded into a graph must bring its own.
  */
 inline size_t WorkspaceBytes(size_t need) { return need == 0 ? 0 : need + 256; }
+/*! \brief what a too small workspace throws, where failed checks throw: the C entries tell it from operands that do not agree */
+struct WorkspaceError : public dmlc::Error {
+  explicit WorkspaceError(const std::string &what) : dmlc::Error(what) {}
+};
 inline char *Workspace(void *given, size_t given_bytes, size_t need, cudaStream_t stream, const char *name) {
   if (need == 0) return nullptr;
   if (given == nullptr) {
     CHECK(!IsCapturing(stream)) << name << ": a call captured into a graph needs a workspace of the caller's";
     return static_cast<char *>(Scratch::Get(stream, need));
   }
-  CHECK(given_bytes >= WorkspaceBytes(need)) << name << ": the workspace holds " << given_bytes << " bytes, "
-                                             << WorkspaceBytes(need) << " are needed";
+  if (given_bytes < WorkspaceBytes(need)) {
+    const std::string what = std::string(name) + ": the workspace holds " + std::to_string(given_bytes) + " bytes, " +
+                             std::to_string(WorkspaceBytes(need)) + " are needed";
+#if DMLC_LOG_FATAL_THROW
+    throw WorkspaceError(what);
+#else
+    LOG(FATAL) << what;
+#endif
+  }
   return reinterpret_cast<char *>((reinterpret_cast<uintptr_t>(given) + 255) / 256 * 256);
 }
 

@@ -1136,3 +1136,21 @@ def test_two_streams_add_into_one_table(lib, n):
             lib.embed_take_grad(dst, src, index, saver=1, workspace=ws, stream=s.cuda_stream)
     torch.cuda.synchronize()
     assert torch.equal(dst.double(), calls * want)
+
+
+@pytest.mark.gpu
+def test_small_workspace_is_an_argument(lib):
+    """A workspace that is too small is answered with the same status by all entries, and the call does nothing."""
+    x, w, label = problem(700, 900, 64, BF16, 1)
+    loss, lse = torch.full((700,), 9.0, device="cuda"), torch.full((700,), 9.0, device="cuda")
+    gx, gw = torch.full_like(x, 9.0), torch.full_like(w, 9.0)
+    for size in (1, 1000):
+        small = torch.empty(size, dtype=torch.uint8, device="cuda")
+        for call in (lambda: lib.linear_softmax_loss(loss, lse, x, w, label, workspace=small),
+                     lambda: lib.linear_softmax_loss_grad(gx, gw, x, w, label, lse, workspace=small),
+                     lambda: lib.embed_take_grad(gw, x, label, workspace=small)):
+            with pytest.raises(capi.MsbError) as e:
+                call()
+            assert e.value.status == 1 and "workspace" in str(e.value)
+    torch.cuda.synchronize()
+    assert all((t == 9).all() for t in (loss, lse, gx, gw))
