@@ -377,7 +377,7 @@ EmbedSortKernel(int32_t *keys, int32_t *rows, const int32_t *index, uint32_t n, 
     const int32_t k = index[i];
     const bool named = k >= 0 && static_cast<uint32_t>(k) < table_rows;
     s_key[i] = named ? static_cast<uint32_t>(k) : 0u;
-    s_val[i] = named ? static_cast<uint16_t>(i) : 0xffffu;  // i < 16384
+    s_val[i] = named ? static_cast<uint16_t>(i) : 0xffffu;  // i < kOneCta
   }
   for (int pass = 0; pass < passes; ++pass) {
     const int shift = pass * digit_bits;

@@ -1154,3 +1154,22 @@ def test_small_workspace_is_an_argument(lib):
             assert e.value.status == 1 and "workspace" in str(e.value)
     torch.cuda.synchronize()
     assert all((t == 9).all() for t in (loss, lse, gx, gw))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [5121, 7169, 8191, 8192, 8193])
+@pytest.mark.parametrize("rows", [2, 500, 70000, 1500000])
+def test_embed_take_grad_where_one_cta_stops_sorting(lib, n, rows):
+    """The longest lists that one CTA sorts, all its rounds and all its shared memory, and the first that it does not, with
+    one to three digits per row number."""
+    g = gen(n + rows)
+    src = torch.randn(n, 8, device="cuda", generator=g)
+    index = zipf(n, rows, g)
+    index = torch.randperm(rows, device="cuda", generator=g).to(torch.int32)[index.long()]
+    index[::11] = -1
+    index[5::13] = rows
+    for add in (False, True):
+        dst = torch.randn(rows, 8, device="cuda", generator=g)
+        want, bound = grad_oracle(dst, src, index, 1.0, add)
+        lib.embed_take_grad(dst, src, index, saver=int(add))
+        within(dst, want, bound, "take_grad")
