@@ -24,11 +24,14 @@
  * operands, and it is relative to each d (half a unit of its last place), so the gradients come
  * out about as exact as their own final rounding leaves them.  What is stored is not d itself but
  *     d' = (p - q) / (1 - a) * gloss * 2^k,     d = d' * scale * (1 - a) * 2^-k
- * with 2^k bringing the largest of gloss / (1 - a) to 2^14 .. 2^15, and the factor on the right applied to the
+ * with 2^k bringing the largest finite |gloss| / (1 - a) to 2^14 .. 2^15, and the factor on the right applied to the
  * finished sums: a mean over thousands of tokens would put most of d below the smallest binary16 number, and the
  * label's term, which carries most of the gradient while p is small, would be rounded by the same fraction in every
  * row -- as stored it is a power of two.  (With scale and 1 - a inside: gradients of 0.31 % instead of 0.17 %
  * relative error, bf16, smoothing 0.1; 0.21 instead of 0.17 % without smoothing.)
+ * binary16 has too few exponents for one k: a token whose |gloss| is less than 2^-6 of the largest gets a k of its own for the
+ * gradient of x, whose row it alone determines, and its row of d' is brought back to the common k before the gradient
+ * of W, where it stands beside the others.  There an entry of d below 2^-39 of the largest |gloss| / (1 - a) is lost.
  *
  * Live tokens are packed together first (PackRowsKernel): tiles of padding cost nothing, whatever
  * their hidden states hold -- an infinity in a padded row does not meet a zero of d -- and the
@@ -786,6 +789,7 @@ struct PackArgs {
   const float *gloss;    // backward, may be null
   float scale, q_label;
   float *lse2, *row_scale;  // [pad_rows], backward
+  float *row_down;       // [pad_rows] 2^-(a row's own k - the common one), or null: all rows have the common one
   int vec;               // 16-byte copies possible
   int tiled;             // the tiled copies can read x itself: nothing is packed if all its rows count
   int rows_per_cta;
@@ -796,7 +800,17 @@ __device__ __forceinline__ bool IsLive(int32_t label, int32_t ignore, int32_t v)
   return label != ignore && label >= 0 && label < v;
 }
 
-/*! \brief live rows, and the largest |gloss| among them, of every 256 tokens: for lists too long to be counted by each CTA below */
+/*! \brief |gloss| where it is a number that a scale can be chosen by: an infinite one must not leave the other rows without */
+__device__ __forceinline__ float FiniteSize(float gloss) {
+  const float size = fabsf(gloss);
+  return size < INFINITY ? size : 0.0f;
+}
+/*! \brief the power of two that brings `size` to [2^14, 2^15); 0 for one that has none */
+__device__ __forceinline__ int ScaleExponent(float size) {
+  return size > 0.0f && size < INFINITY ? min(100, max(-100, 14 - ilogbf(size))) : 0;
+}
+
+/*! \brief live rows, and the largest finite |gloss| among them, of every 256 tokens: for lists too long to be counted by each CTA below */
 template <int kUnused>
 __global__ void __launch_bounds__(256) CountRowsKernel(const PackArgs a) {
   gpu_rt::GridDependencySync();
@@ -804,7 +818,7 @@ __global__ void __launch_bounds__(256) CountRowsKernel(const PackArgs a) {
   __shared__ float s_top[8];
   const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   const bool on = i < a.n && IsLive(a.label[i], a.ignore, a.v);
-  float top = on && a.gloss != nullptr ? fabsf(a.gloss[i]) : 0.0f;
+  float top = on && a.gloss != nullptr ? FiniteSize(a.gloss[i]) : 0.0f;
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   const int count = __popc(__ballot_sync(0xffffffffu, on));
   if ((threadIdx.x & 31) == 0) s_count[threadIdx.x >> 5] = count, s_top[threadIdx.x >> 5] = top;
@@ -845,7 +859,7 @@ __global__ void __launch_bounds__(256) PackRowsKernel(const PackArgs a) {
       const int on = IsLive(a.label[i], a.ignore, a.v) ? 1 : 0;
       total += on;
       before += i < base ? on : 0;
-      if (a.gloss != nullptr && on) top = fmaxf(top, fabsf(a.gloss[i]));
+      if (a.gloss != nullptr && on) top = fmaxf(top, FiniteSize(a.gloss[i]));
     }
   }
   for (int o = 16; o > 0; o >>= 1) {
@@ -860,16 +874,7 @@ __global__ void __launch_bounds__(256) PackRowsKernel(const PackArgs a) {
   for (int w = 0; w < 8; ++w) before += s_before[w], total += s_total[w], top = fmaxf(top, s_top[w]);
   __syncthreads();
 
-  // the power of two that brings the largest row scale to [2^14, 2^15)
-  float up = 1.0f, down = 1.0f;
-  if (a.row_scale != nullptr) {
-    const float largest = (a.gloss != nullptr ? top : 1.0f) / a.q_label;
-    if (largest > 0.0f && largest < INFINITY) {
-      const int e = min(100, max(-100, 14 - ilogbf(largest)));
-      up = __int_as_float((127 + e) << 23);
-      down = __int_as_float((127 - e) << 23);
-    }
-  }
+  const int common = a.row_scale != nullptr ? ScaleExponent((a.gloss != nullptr ? top : 1.0f) / a.q_label) : 0;
   const int end = (total + kPadRows - 1) / kPadRows * kPadRows;  // rows up to here are read by the products
   const int i = base + tid;
   const bool mine = tid < a.rows_per_cta && i < a.n;
@@ -885,7 +890,14 @@ __global__ void __launch_bounds__(256) PackRowsKernel(const PackArgs a) {
     a.label_of[pos] = label;
     if (a.row_of != nullptr) a.row_of[pos] = i;
     if (a.row_scale != nullptr) {
-      a.row_scale[pos] = (a.gloss != nullptr ? a.gloss[i] : 1.0f) / a.q_label * up;
+      const float factor = (a.gloss != nullptr ? a.gloss[i] : 1.0f) / a.q_label;
+      int own = common;
+      if (a.row_down != nullptr) {
+        const int best = FiniteSize(factor) > 0.0f ? ScaleExponent(fabsf(factor)) : common;
+        if (best - common > 6) own = min(best, common + 100);
+        a.row_down[pos] = __int_as_float((127 + common - own) << 23);
+      }
+      a.row_scale[pos] = factor * __int_as_float((127 + own) << 23);
       a.lse2[pos] = a.lse[i] * kLog2e;
     }
   }
@@ -898,7 +910,7 @@ __global__ void __launch_bounds__(256) PackRowsKernel(const PackArgs a) {
   if (blockIdx.x == 0 && tid == 0) {
     a.words[0] = total;
     // (with no token that counts the sums are empty, and zero whatever the scale: 1 / 0 tokens, say)
-    reinterpret_cast<float *>(a.words)[1] = total > 0 ? a.scale * a.q_label * down : 0.0f;
+    reinterpret_cast<float *>(a.words)[1] = total > 0 ? a.scale * a.q_label * __int_as_float((127 - common) << 23) : 0.0f;
     a.words[2] = a.tiled && total == a.n;
   }
   if (a.tiled && total == a.n) return;
@@ -940,6 +952,29 @@ AlignRowsKernel(uint16_t *dst, int64_t ld_dst, const uint16_t *src, int64_t ld_s
     for (int j = 0; j < 8; ++j) w[j] = col + j < cols ? from[j] : 0u;
     *reinterpret_cast<uint4 *>(dst + row * ld_dst + col) =
         make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16);
+  }
+}
+
+/*! \brief rows of d' with a k of their own back to the common one, between the gradients of x and W: a warp per row */
+template <int kUnused>
+__global__ void __launch_bounds__(256)
+CommonScaleKernel(uint16_t *delta, int64_t ld, const int32_t *live, const float *row_down, int cols) {
+  gpu_rt::GridDependencySync();
+  const int lane = threadIdx.x & 31;
+  for (int row = blockIdx.x * 8 + (threadIdx.x >> 5); row < live[0]; row += gridDim.x * 8) {
+    const float down = row_down[row];
+    if (down == 1.0f) continue;
+    uint4 *p = reinterpret_cast<uint4 *>(delta + row * ld);
+    for (int c = lane; c < (cols + 7) / 8; c += 32) {
+      uint4 v = p[c];
+      uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        w[j] = PackPair(Widen(static_cast<uint16_t>(w[j] & 0xffffu), 0) * down, Widen(static_cast<uint16_t>(w[j] >> 16), 0) * down, 0);
+      }
+      v.x = w[0], v.y = w[1], v.z = w[2], v.w = w[3];
+      p[c] = v;
+    }
   }
 }
 
@@ -1028,7 +1063,7 @@ struct FinishArgs {
   int n_tiles, tile_n, group, k_plan, room, slots, ctas;  // of the kernel that wrote the parts
   float step_cycles, tile_cycles;
   const int32_t *pos_of;
-  const float *inv_scale;
+  const float *inv_scale, *row_down;  // (row_down may be null)
   uint16_t *out;
   int64_t ld_out;
   int32_t n, h;
@@ -1097,8 +1132,9 @@ __global__ void __launch_bounds__(256) DataGradFinishKernel(const FinishArgs a) 
     for (int r = 0; r < kRows; ++r) {
       if (i0 + r >= a.n) break;
       uint16_t *out = a.out + (i0 + r) * a.ld_out;
+      const float down = a.row_down != nullptr && pos[r] >= 0 ? a.row_down[pos[r]] : 1.0f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[r][j] = pos[r] >= 0 ? v[r][j] * inv : 0.0f;  // (inv may be infinite)
+      for (int j = 0; j < 8; ++j) v[r][j] = pos[r] >= 0 ? v[r][j] * down * inv : 0.0f;  // (inv may be infinite)
       if (a.vec && 8 * g + 8 <= a.h) {
         uint4 w;
         w.x = PackPair(v[r][0], v[r][1], a.bf16);
@@ -1196,7 +1232,7 @@ struct Plan {
   int64_t pad_rows, ld_x, ld_w, piece, ld_acc, tile_n, tiles;
   int room, ctas, ctas_gx, shape_gx;
   bool wide_gx;
-  int64_t counts, words, row_of, pos_of, label_of, lse2, row_scale, x, w, part, part_sum, label_logit, delta, acc, spare, bytes;
+  int64_t counts, words, row_of, pos_of, label_of, lse2, row_scale, row_down, x, w, part, part_sum, label_logit, delta, acc, spare, bytes;
 };
 
 /*! \brief layout of a call; sms = multiprocessors of the device */
@@ -1243,6 +1279,7 @@ inline Plan MakePlan(int64_t n, int64_t v, int64_t h, bool gradient, bool want_g
   if (gradient) {
     p.lse2 = take(p.pad_rows * 4);
     p.row_scale = take(p.pad_rows * 4);
+    p.row_down = take(want_gx ? p.pad_rows * 4 : 0);
     p.delta = take(p.pad_rows * p.piece * 2);
     p.acc = take(want_gx ? p.pad_rows * p.ld_acc * 4 : 0);
     p.spare = take(want_gx ? static_cast<int64_t>(p.room) * 128 * p.ctas_gx * kTileN * (p.wide_gx ? 2 : 1) * 4 : 0);
@@ -1425,6 +1462,8 @@ inline void BackwardLaunch(const GradOut &g, const Problem &q, const Plan &p, ch
   k.lse = g.lse, k.gloss = g.gloss, k.scale = g.scale, k.q_label = static_cast<float>(1.0 - q.smooth);
   k.lse2 = reinterpret_cast<float *>(ws + p.lse2);
   k.row_scale = reinterpret_cast<float *>(ws + p.row_scale);
+  // (bfloat16 has the exponents for a common scale; without the gradient of x there is no use for another)
+  if (!q.bf16 && g.gloss != nullptr && g.gx != nullptr) k.row_down = reinterpret_cast<float *>(ws + p.row_down);
   PackLaunch(q, p, ws, k, stream);
 
   const int32_t h_tiles = static_cast<int32_t>(p.ld_acc / kTileN);
@@ -1484,6 +1523,12 @@ inline void BackwardLaunch(const GradOut &g, const Problem &q, const Plan &p, ch
       if (p.wide_gx) LaunchGemm<kDataGrad, 2, true>(d_along, w_across, spare, out, a, x_tiles * a.n_tiles, sms, stream);
       else Gemm<kDataGrad>(d_along, w_across, spare, out, a, x_tiles * a.n_tiles, p.ctas_gx, sms, stream);
     }
+    if (g.gw != nullptr && k.row_down != nullptr) {
+      gpu_rt::LaunchAfterDrain(CommonScaleKernel<0>, dim3(static_cast<unsigned>(std::min<int64_t>(Ceil(q.n, 8), 8 * sms))), dim3(256),
+                               0, stream, reinterpret_cast<uint16_t *>(delta), p.piece, a.live,
+                               static_cast<const float *>(k.row_down), static_cast<int>(cols));
+      MSHADOW_CUDA_POST_KERNEL_CHECK(CommonScaleKernel);
+    }
     if (g.gw != nullptr) {
       const int64_t elem = g.gw_type == kFloat32 ? 4 : 2;
       const int ctas = CtasFor(cols, h_tiles, sms);
@@ -1521,7 +1566,7 @@ inline void BackwardLaunch(const GradOut &g, const Problem &q, const Plan &p, ch
     f.group = GroupOf(Ceil(q.n, 128 * p.ctas_gx), 8);
     f.k_plan = a.k_plan, f.room = p.room, f.slots = sms / p.ctas_gx, f.ctas = p.ctas_gx;
     f.step_cycles = a.step_cycles, f.tile_cycles = a.tile_cycles;
-    f.pos_of = k.pos_of, f.inv_scale = a.inv_scale;
+    f.pos_of = k.pos_of, f.inv_scale = a.inv_scale, f.row_down = k.row_down;
     f.out = g.gx, f.ld_out = g.ld_gx, f.n = static_cast<int32_t>(q.n), f.h = static_cast<int32_t>(q.h);
     f.bf16 = q.bf16, f.vec = Aligned16(g.gx, g.ld_gx, 2);
     f.groups = gpu_rt::FastDiv(static_cast<uint32_t>(Ceil(q.h, 8)));

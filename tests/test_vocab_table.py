@@ -1173,3 +1173,60 @@ def test_embed_take_grad_where_one_cta_stops_sorting(lib, n, rows):
         want, bound = grad_oracle(dst, src, index, 1.0, add)
         lib.embed_take_grad(dst, src, index, saver=int(add))
         within(dst, want, bound, "take_grad")
+
+
+def own_row_bounds(q, gloss, scale, dtype):
+    """gdata of tokens that count and its bound as in grad_bounds, but with what d loses below binary16's normal range counted in
+    the token's own |gloss|: its row of d is stored 2^8 times that / (1 - a) or larger, so half of the smallest
+    binary16 number is at most 2^-33 of it."""
+    s = float(np.float32(scale)) * gloss.double()
+    p = (q["z"] - q["lse"][:, None]).exp()
+    v = p.shape[1]
+    t = torch.full_like(p, q["a"] / (v - 1) if q["a"] else 0.0)
+    t.scatter_(1, q["at"], 1.0 - q["a"])
+    d = (p - t) * s[:, None]
+    rho = q["dz"] + q["e_lse"] + 4 * ADD * (q["lse"].abs() + q["z"].abs().amax(1)) + 2.0 ** -20
+    e = (p * rho.expm1()[:, None] + 3 * ADD * (p + t)) * s.abs()[:, None]
+    e = e + U[dtype] * (d.abs() + e) + TINY[dtype] * 2.0 ** -8 * s.abs()[:, None]
+    gx = d @ q["wd"]
+    bx = e @ q["wd"].abs() + (v + 16) * ADD * ((d.abs() + e) @ q["wd"].abs())
+    return gx, bx + U[dtype] * (gx.abs() + bx) + TINY[dtype]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,v,h,smooth", [(60, 40000, 64, 0.0), (300, 9000, 72, 0.1), (17000, 600, 40, 0.0)])
+@pytest.mark.parametrize("largest", [1.0, 4096.0, float("inf"), float("nan")])
+def test_loss_grad_of_unlike_tokens(lib, n, v, h, smooth, largest):
+    """Tokens whose gloss lie many binary16 ranges apart, over flat distributions: each token's gdata is as exact as if it were
+    alone; an infinite gloss spoils its own token and the weight's gradient, no other token's."""
+    x, w, label = problem(n, v, h, F16, 17, ignored=0.2, spread=0.25)
+    x.mul_(0.25)
+    gloss = torch.exp2(-24.0 * torch.rand(n, device="cuda", generator=gen(2)))
+    gloss[::4] = -gloss[::4]
+    gloss[1::9] = 0.0
+    label[n // 2] = 1
+    gloss[n // 2] = largest
+    usual = torch.isfinite(gloss)
+    loss, lse = torch.empty(n, device="cuda"), torch.empty(n, device="cuda")
+    lib.linear_softmax_loss(loss, lse, x, w, label, smooth=smooth)
+    _, _, _, _, q = loss_oracle(x, w, label, -1, smooth)
+    counts = (q["live"] & usual).nonzero()[:, 0]
+    for scale in (1.0, 2.0 ** 12):  # the largest leave binary16's range then, the others must not care
+        gx, gw = torch.full_like(x, 9.0), torch.full((v, h), 9.0, device="cuda")
+        lib.linear_softmax_loss_grad(gx, gw, x, w, label, lse, gloss, scale, smooth=smooth)
+        part = dict(q, **{k: q[k][counts] for k in ("z", "lse", "dz", "e_lse", "at")})
+        want, bound = own_row_bounds(part, gloss[counts], scale, F16)
+        inside = (want.abs() + bound).amax(1) < 60000
+        assert inside.sum() >= counts.numel() // 2
+        within(gx[counts][inside], want[inside], bound[inside], "gdata")
+        assert (gx[~q["live"]] == 0).all()
+        if np.isfinite(largest):
+            _, _, ww, bw = grad_bounds(q, gloss, scale, F16, F32)
+            within(gw, ww, bw, "gweight")
+        only = torch.full_like(x, 9.0)  # without the weight's gradient: the same
+        lib.linear_softmax_loss_grad(only, None, x, w, label, lse, gloss, scale, smooth=smooth)
+        assert torch.equal(only.view(torch.int16), gx.view(torch.int16))
+        alone = torch.empty_like(gw)
+        lib.linear_softmax_loss_grad(None, alone, x, w, label, lse, gloss, scale, smooth=smooth)
+        if np.isfinite(largest):
+            within(alone, ww, bw, "gweight alone")
