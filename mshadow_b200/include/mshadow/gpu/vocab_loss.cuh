@@ -55,7 +55,6 @@ const int kTileN = 256;       // columns of a tile
 const int kStepK = 64;        // contraction elements per stage (one 128-byte swizzle row)
 const int kThreads = 384;     // warp 0: copies, warp 1: products, warp 2: tensor memory, warps 4-11: epilogue
 const int kHalfN = kTileN / 2;  // columns of a tile that one epilogue group (four warps, a thread per row) takes
-const int kChunkSteps = 16;   // kStat: stages per run of accumulation in tensor memory (1024 contraction elements)
 const uint32_t kBoxOut = 128 * 128;  // a box of 128 rows by 128 bytes, on its way out through shared memory
 const int kWideSteps = 24;    // steps from which d and grad W are computed in tiles of 512 columns (below)
 const int kPadRows = 256;     // token rows of the scratch matrices are padded to this
@@ -74,6 +73,20 @@ struct Layout {
   static const bool kAAcross = kMode == kWeightGrad;
   static const bool kBAcross = kMode == kDataGrad || kMode == kWeightGrad;
 };
+
+/*!
+ * \brief stages per run of accumulation in tensor memory (VocabGemmKernel): 1024 contraction elements for the loss; 8192 for the
+ *  logits of the gradient, whose exponentials are rounded to 16 bits, and for sums that stay binary32; 16384 for
+ *  sums that are rounded to 16 bits themselves
+ */
+__host__ __device__ __forceinline__ int RunSteps(int mode, bool wide_out) {
+  return mode == kStat ? 16 : mode == kDelta || wide_out ? 128 : 256;
+}
+/*! \brief first stage of run `run` of a contraction of `steps` */
+template <int kMode>
+__device__ __forceinline__ int RunBegin(int run, int runs, int steps, int run_steps) {
+  return kMode == kStat ? run * steps / runs : run < runs ? run * run_steps : steps;
+}
 
 /*! \brief kWide: a pair's tile is 512 columns wide, two sets of 256, and fills the tensor memory */
 template <int kMode, int kCtas, bool kWide>
@@ -130,6 +143,8 @@ struct GemmArgs {
   int out_add;
   int out_vec;           // rows of `out` start on 16-byte boundaries
   int out_tiled;         // written by tiled copies (map_out)
+  int run_steps;         // RunSteps
+  float4 *earlier;       // sums of earlier runs (EarlierOf), or null: every contraction is one run
   int *status;
 };
 
@@ -230,8 +245,45 @@ struct Half {
   int col;           // first column of the half, within the piece
   uint32_t boxes, box;  // shared memory of the group's first outgoing box; which one is filled next
   int group, thread; // 0 / 1; thread of the group: 0 .. 127
+  float4 *earlier;   // this thread's sums of the tile's earlier runs, or null: there are none
   __device__ __forceinline__ uint32_t Box() const { return boxes + box * 2 * kBoxOut; }
 };
+
+// ---- sums of earlier runs: 128 columns of a row per thread and set of accumulators, read and written by that thread alone -----
+
+const int kEarlierStep = 256;  // groups of four columns of a thread are this far apart: a warp's lie side by side
+const int64_t kEarlierBytes = int64_t(2) * (kHalfN / 4) * kEarlierStep * 16;  // of a CTA: two sets
+__device__ __forceinline__ float4 *EarlierOf(float4 *all, int set) {
+  return all + (static_cast<int64_t>(blockIdx.x) * 2 + set) * (kHalfN / 4) * kEarlierStep + (threadIdx.x - 128);
+}
+/*! \brief accumulators of the columns from `col` on, plus those of the earlier runs */
+template <int kColumns>
+__device__ __forceinline__ void AddEarlier(const Half &t, int col, uint32_t (&r)[kColumns]) {
+  if (t.earlier == nullptr) return;
+#pragma unroll
+  for (int q = 0; q < kColumns / 4; ++q) {
+    const float4 e = t.earlier[(col / 4 + q) * kEarlierStep];
+    r[4 * q] = __float_as_uint(__fadd_rn(__uint_as_float(r[4 * q]), e.x));
+    r[4 * q + 1] = __float_as_uint(__fadd_rn(__uint_as_float(r[4 * q + 1]), e.y));
+    r[4 * q + 2] = __float_as_uint(__fadd_rn(__uint_as_float(r[4 * q + 2]), e.z));
+    r[4 * q + 3] = __float_as_uint(__fadd_rn(__uint_as_float(r[4 * q + 3]), e.w));
+  }
+}
+/*! \brief a run that is not its tile's last: its sums, and those of the runs before it, are kept */
+__device__ __forceinline__ void KeepHalf(const Half &t, float4 *keep) {
+#pragma unroll 1
+  for (int b = 0; b < kHalfN / 32; ++b) {
+    uint32_t r[32];
+    tc5::LoadColumns(t.acc + b * 32, r);
+    tc5::WaitColumns(r);
+    AddEarlier(t, b * 32, r);
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      keep[(b * 8 + q) * kEarlierStep] = make_float4(__uint_as_float(r[4 * q]), __uint_as_float(r[4 * q + 1]),
+                                                     __uint_as_float(r[4 * q + 2]), __uint_as_float(r[4 * q + 3]));
+    }
+  }
+}
 
 /*!
  * \brief before a box is filled.  With two boxes the next one is known to be free already (BoxSend); a single one is
@@ -366,6 +418,8 @@ __device__ __forceinline__ void DeltaHalf(Half &t, int limit, int label, float l
     tc5::LoadColumns(t.acc + b * 64 + 32, r1);
     tc5::WaitColumns(r0);
     tc5::WaitColumns(r1);
+    AddEarlier(t, b * 64, r0);
+    AddEarlier(t, b * 64 + 32, r1);
     DeltaColumns(r0, limit - b * 64, label - b * 64, lse2, scale, a, p0);
     DeltaColumns(r1, limit - b * 64 - 32, label - b * 64 - 32, lse2, scale, a, p1);
     BoxFree<kBoxes>(&t);
@@ -386,6 +440,7 @@ __device__ __forceinline__ void FloatHalf(Half &t, float factor, const CUtensorM
     uint32_t r[32];
     tc5::LoadColumns(t.acc + b * 32, r);
     tc5::WaitColumns(r);
+    AddEarlier(t, b * 32, r);
 #pragma unroll
     for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * factor);
     BoxFree<kBoxes>(&t);
@@ -405,6 +460,8 @@ __device__ __forceinline__ void PackedHalf(Half &t, float factor, int bf16, cons
     tc5::LoadColumns(t.acc + b * 64 + 32, r1);
     tc5::WaitColumns(r0);
     tc5::WaitColumns(r1);
+    AddEarlier(t, b * 64, r0);
+    AddEarlier(t, b * 64 + 32, r1);
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       r0[i] = PackPair(__uint_as_float(r0[2 * i]) * factor, __uint_as_float(r0[2 * i + 1]) * factor, bf16);
@@ -520,11 +577,15 @@ __device__ __forceinline__ void WeightRows(const uint32_t (&r)[32], const Half &
  *  128 * kCtas rows by 256 columns (kStat: a.tile_n; kWide: 512).  Dynamic shared memory StageShape::kSmem.
  *
  *  Tensor memory holds two sets of accumulators; the products of one run into them while the epilogue empties the
- *  other.  A set is a whole tile, except in kStat: there the contraction is cut into runs of at most
- *  1024 elements, which the epilogue adds up in registers.  The tensor cores cut off, rather than
- *  round, each time they add to an accumulator, always towards zero: over 4096 elements that moved
- *  the loss by 1.8e-6 of its value, against 6e-7 for a product in plain binary32 and 4e-7 for these runs, which
- *  cost 1 % of the time (runs of 512: 2.5e-7 and another 3 %; of 256: 17 %).
+ *  other.  The contraction is cut into runs (RunSteps) that are added up in binary32 outside of it, because the
+ *  tensor cores cut off, rather than round, each time they add to an accumulator, always towards zero.  kStat adds its runs
+ *  of 1024 elements up in registers: over 4096 elements the loss was off by 1.8e-6 of its value in one run, by 4e-7 in
+ *  these, which cost 1 % of the time (plain binary32: 6e-7 there, 3e-8 to 4e-8 at 1000 to 2000 features; runs of 512:
+ *  2.5e-7 and another 3 %; of 256: 17 %).  The other modes keep the sums of a tile's runs in memory (38 MB for all CTAs,
+ *  written and read once per run, some 20 000 cycles); most calls have one run there.  Without runs the gradient of W of a
+ *  class that 65536 tokens name was off by 4.2e-4 of its value, and by 1.7e-3 at 262144, however well the rounding of
+ *  d' averages out, now by 5e-5; 1 % of the time of 2048 x 32000 x 4096, 1.5 % of 32768 x 32000 x 2048 with the gradient of
+ *  W as binary32 (runs of 8192 for all: 3.5 % of 8192 x 131072 x 4096).
  *
  *  kWide: both sets belong to one tile.  A step's rows of A then serve 512 columns, a quarter less is read from the L2
  *  and, where A is d', from memory; in return the products wait while a tile is emptied.  For long contractions (not
@@ -581,7 +642,6 @@ VocabGemmKernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
   const int k_blocks = kMode == kWeightGrad ? max(1, (live + kStepK - 1) / kStepK) : a.k_blocks;
   Cut cut = {m_tiles * a.n_tiles, 0, 1};
   if (kMode == kDataGrad) cut = CutOf(m_tiles, a.n_tiles, a.k_plan, a.room, gridDim.x / kCtas, a.step_cycles, a.tile_cycles);
-  const int runs = kMode == kStat ? (k_blocks + kChunkSteps - 1) / kChunkSteps : 1;
   const int units = cut.Units();
   const int first = blockIdx.x / kCtas, step = gridDim.x / kCtas;
 
@@ -638,8 +698,10 @@ VocabGemmKernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         const Unit u = UnitOf(w, cut, m_tiles, a.n_tiles, a.group);
         const int k_first = u.slice * k_blocks / u.parts, k_count = (u.slice + 1) * k_blocks / u.parts - k_first;
         if (k_count == 0) continue;  // the last piece of the vocabulary may have fewer steps than there are parts
+        const int runs = (k_count + a.run_steps - 1) / a.run_steps;
         for (int run = 0; ok && run < runs; ++run, turn += S::kSets) {
-          const int k_begin = k_first + run * k_count / runs, k_end = k_first + (run + 1) * k_count / runs;
+          const int k_begin = k_first + RunBegin<kMode>(run, runs, k_count, a.run_steps);
+          const int k_end = k_first + RunBegin<kMode>(run + 1, runs, k_count, a.run_steps);
           for (int kb = k_begin; ok && kb < k_end; ++kb, ++fill) {
             const int s = fill % S::kStages;
             const uint32_t sa = smem + s * S::kStage;
@@ -694,7 +756,9 @@ VocabGemmKernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
     };
     for (int w = first; w < units; w += step) {
       const Unit u = UnitOf(w, cut, m_tiles, a.n_tiles, a.group);
-      if (kMode == kDataGrad && u.slice * k_blocks / u.parts == (u.slice + 1) * k_blocks / u.parts) continue;
+      const int k_count = (u.slice + 1) * k_blocks / u.parts - u.slice * k_blocks / u.parts;
+      if (kMode == kDataGrad && k_count == 0) continue;
+      const int runs = (k_count + a.run_steps - 1) / a.run_steps;
       const int row0 = u.m * tile_m + static_cast<int>(rank) * 128;
       t.row = row0 + t.thread;
       t.col = u.n * tile_n + t.group * kHalfN;
@@ -723,9 +787,14 @@ VocabGemmKernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         StatHalf(v, t, limit, label < 0 ? -1 : label - a.col0 - t.col, at, a);
         continue;
       }
-      for (int set = 0; set < S::kSets; ++set, t.col += kTileN) {
+      for (int i = 0; i < runs * S::kSets; ++i) {
+        const int run = i / S::kSets, set = i - run * S::kSets;
+        t.col = u.n * tile_n + t.group * kHalfN + set * kTileN;
+        t.earlier = run > 0 ? EarlierOf(a.earlier, set) : nullptr;
         ready();
-        if (kMode == kDelta) {
+        if (run < runs - 1) {
+          KeepHalf(t, EarlierOf(a.earlier, set));
+        } else if (kMode == kDelta) {
           // rows past the live ones: no column of theirs exists, so that d' is zero there whatever the logits of a zero data
           // row are (NaN beside a class with an infinite weight); the product for grad W reads them up to a whole step
           DeltaHalf<S::kBoxes>(t, t.row < live ? a.cols - t.col : 0, label < 0 ? -1 : label - a.col0 - t.col, a.lse2[t.row],
@@ -750,6 +819,7 @@ VocabGemmKernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
               uint32_t r[32];
               tc5::LoadColumns(t.acc + c * 32, r);
               tc5::WaitColumns(r);
+              AddEarlier(t, c * 32, r);
               if (!a.out_vec) WeightRows(r, t, row0, t.col + c * 32, inv, a);
               else if (t.row < a.out_rows) WeightColumns(r, t.row, t.col + c * 32, inv, a);
             }
@@ -1231,8 +1301,8 @@ struct Plan {
   bool pack, copy_w;
   int64_t pad_rows, ld_x, ld_w, piece, ld_acc, tile_n, tiles;
   int room, ctas, ctas_gx, shape_gx;
-  bool wide_gx;
-  int64_t counts, words, row_of, pos_of, label_of, lse2, row_scale, row_down, x, w, part, part_sum, label_logit, delta, acc, spare, bytes;
+  bool wide_gx, runs;
+  int64_t counts, words, row_of, pos_of, label_of, lse2, row_scale, row_down, x, w, part, part_sum, label_logit, delta, acc, spare, earlier, bytes;
 };
 
 /*! \brief layout of a call; sms = multiprocessors of the device */
@@ -1282,6 +1352,10 @@ inline Plan MakePlan(int64_t n, int64_t v, int64_t h, bool gradient, bool want_g
     p.row_down = take(want_gx ? p.pad_rows * 4 : 0);
     p.delta = take(p.pad_rows * p.piece * 2);
     p.acc = take(want_gx ? p.pad_rows * p.ld_acc * 4 : 0);
+    // (whether a contraction is longer than a run)
+    p.runs = Ceil(h, kStepK) > RunSteps(kDelta, false) || Ceil(n, kStepK) > RunSteps(kWeightGrad, true) ||
+             Ceil(std::min(p.piece, v), kStepK) > RunSteps(kDataGrad, false);
+    p.earlier = take(p.runs ? sms * kEarlierBytes : 0);
     p.spare = take(want_gx ? static_cast<int64_t>(p.room) * 128 * p.ctas_gx * kTileN * (p.wide_gx ? 2 : 1) * 4 : 0);
   } else {
     p.part = take(2 * p.tiles * p.pad_rows * 8);
@@ -1409,6 +1483,7 @@ inline void ForwardLaunch(float *loss, float *lse, const Problem &q, const Plan 
   a.live = p.pack ? reinterpret_cast<const int32_t *>(ws + p.words) : nullptr;
   a.tokens = static_cast<int32_t>(q.n);
   a.k_blocks = static_cast<int32_t>(Ceil(q.h, kStepK));
+  a.run_steps = RunSteps(kStat, false);
   const int64_t m_tiles = Ceil(q.n, 128 * p.ctas);
   a.group = GroupOf(m_tiles, 16);
   a.instr = tc5::InstrDesc(q.bf16, false, false, 128 * p.ctas, static_cast<int>(p.tile_n));
@@ -1481,6 +1556,7 @@ inline void BackwardLaunch(const GradOut &g, const Problem &q, const Plan &p, ch
   a.q_other = q.smooth != 0.0f ? static_cast<float>(static_cast<double>(q.smooth) / (q.v - 1)) : 0.0f;
   a.bf16 = q.bf16;
   a.status = gpu_rt::StatusWord();
+  a.earlier = p.runs ? reinterpret_cast<float4 *>(ws + p.earlier) : nullptr;
   const CUtensorMap x_along = tc5::MatrixMap(ws + p.x, type, p.pad_rows, q.h, p.ld_x, 128);
   const CUtensorMap x_across = tc5::MatrixMap(ws + p.x, type, p.pad_rows, q.h, p.ld_x, 64);
   const bool tiled = Aligned16(q.x, q.ld_x, 2);
@@ -1495,6 +1571,7 @@ inline void BackwardLaunch(const GradOut &g, const Problem &q, const Plan &p, ch
     a.col0 = static_cast<int32_t>(p0);
     a.n_tiles = static_cast<int32_t>(Ceil(cols, kTileN));
     a.k_blocks = static_cast<int32_t>(Ceil(q.h, kStepK));
+    a.run_steps = RunSteps(kDelta, false);
     a.group = GroupOf(m_tiles, 16);
     a.instr = tc5::InstrDesc(q.bf16, false, false, 128 * p.ctas, kTileN);
     const CUtensorMap w_along = WeightMap(q, p, ws, p0, cols, kTileN / p.ctas, stream, true, &a.b_row0);
@@ -1516,6 +1593,7 @@ inline void BackwardLaunch(const GradOut &g, const Problem &q, const Plan &p, ch
       a.tile_cycles = static_cast<float>(TileCycles(p.shape_gx));
       a.k_blocks = static_cast<int32_t>(Ceil(cols, kStepK));
       a.k_plan = static_cast<int32_t>(Ceil(std::min(p.piece, q.v), kStepK));
+      a.run_steps = RunSteps(kDataGrad, false);
       a.room = p.room;
       a.accumulate = p0 > 0;
       a.group = GroupOf(x_tiles, 8);
@@ -1534,6 +1612,7 @@ inline void BackwardLaunch(const GradOut &g, const Problem &q, const Plan &p, ch
       const int ctas = CtasFor(cols, h_tiles, sms);
       a.m_tiles = static_cast<int32_t>(Ceil(cols, 128 * ctas));
       a.n_tiles = h_tiles;
+      a.run_steps = RunSteps(kWeightGrad, g.gw_type == kFloat32);
       a.b_row0 = 0;
       a.group = GroupOf(a.m_tiles, 8);
       a.instr = tc5::InstrDesc(q.bf16, true, true, 128 * ctas, kTileN);

@@ -1230,3 +1230,76 @@ def test_loss_grad_of_unlike_tokens(lib, n, v, h, smooth, largest):
         lib.linear_softmax_loss_grad(None, alone, x, w, label, lse, gloss, scale, smooth=smooth)
         if np.isfinite(largest):
             within(alone, ww, bw, "gweight alone")
+
+
+# ---- long sums: the tensor cores cut off each time they add, so what is added in one go is bounded --------------------
+
+RUN = 512 * ADD  # a run of 8192 elements is 512 additions, each off by up to one unit in the last place of the sum; where the
+#                  sum is rounded to 16 bits, runs are twice as long
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("n,v,h,gw_dtype,add", [
+    (65536, 256, 64, F32, False), (262144, 256, 64, F32, False), (262144, 256, 64, None, False), (200001, 300, 33, F32, False),
+    (200001, 300, 33, None, True), (150000, 256, 40, None, True), (120000, 256, 64, F32, True), (16500, 40000, 512, F32, False),
+    (16500, 40000, 512, None, False)])
+def test_weight_gradient_of_a_frequent_class(lib, dtype, n, v, h, gw_dtype, add):
+    """Every token names one class and all its terms have one sign: what is lost in each addition adds up."""
+    gw_dtype = gw_dtype or dtype
+    x = (torch.rand(n, h, device="cuda", generator=gen(n)) + 1).to(dtype)
+    w = torch.zeros(v, h, device="cuda", dtype=dtype)
+    label = torch.full((n,), 3, dtype=torch.int32, device="cuda")
+    loss, lse = torch.empty(n, device="cuda"), torch.empty(n, device="cuda")
+    lib.linear_softmax_loss(loss, lse, x, w, label)
+    gw = torch.ones(v, h, dtype=gw_dtype, device="cuda")
+    lib.linear_softmax_loss_grad(None, gw, x, w, label, lse, scale=1.0 / n, saver=int(add))
+    mean = x.double().mean(0)
+    for row, d in ((3, 1.0 / v - 1.0), (4, 1.0 / v)):
+        sums = d * mean
+        # d: the exponential and lse (2^-20), a rounding; the sum: a run, and the runs; scale and result
+        off = (2.0 ** -20 * (1.0 / v if row == 4 else 1.0) / abs(d) + U[dtype] + RUN * (1 if gw_dtype == F32 else 2) + (n / 8192 + 8) * ADD) * sums.abs()
+        if row == 3 and v == 256:
+            off -= U[dtype] * sums.abs()  # 255 / 256 has eight bits
+        want = sums + (1.0 if add else 0.0)
+        bound = off + ADD * want.abs() + U[gw_dtype] * (want.abs() + off) + TINY[gw_dtype]
+        within(gw[row], want, bound, "gweight of class %d" % row)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,v,h", [(8, 1 << 20, 1024), (600, 131072, 4096), (300, 200003, 72), (129, 100000, 520)])
+def test_data_gradient_over_a_long_vocabulary(lib, n, v, h):
+    """Behind the label's term, by far the largest, every class adds one of the other sign."""
+    w = torch.empty(v, h, dtype=F16, device="cuda")
+    for at in range(0, v, 1 << 17):
+        w[at:at + (1 << 17)] = torch.rand(min(1 << 17, v - at), h, device="cuda", generator=gen(at)) + 1
+    w[0] = 100
+    x = torch.zeros(n, h, device="cuda", dtype=F16)
+    label = torch.zeros(n, dtype=torch.int32, device="cuda")
+    loss, lse, gx = torch.empty(n, device="cuda"), torch.empty(n, device="cuda"), torch.empty_like(x)
+    lib.linear_softmax_loss(loss, lse, x, w, label)
+    lib.linear_softmax_loss_grad(gx, None, x, w, label, lse)
+    mean = torch.stack([w[at:at + (1 << 17)].double().sum(0) for at in range(0, v, 1 << 17)]).sum(0) / v
+    want = mean - 100
+    # d: 1 - 1 / v is rounded to 1, and 1 / v is rounded (and 2^-20 for the exponential); sums are up to 102 large
+    off = 102 * (2 * RUN + (v / 8192 + 16) * ADD) + 100.0 / v + mean * (U[F16] + 2.0 ** -20)
+    within(gx, want.expand(n, h), (off + U[F16] * (want.abs() + off)).expand(n, h), "gdata")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,v,h", [(64, 512, 65536), (300, 20000, 16384), (40, 300, 12345)])
+def test_gradient_over_many_features(lib, n, v, h):
+    """Logits whose terms have one sign: those of the gradient are as exact as lse needs them."""
+    x = (torch.rand(n, h, device="cuda", generator=gen(h)) + 1).to(F16)
+    w = torch.full((v, h), 20.0 / 1.5 / h, device="cuda", dtype=F16)
+    label = torch.full((n,), 3, dtype=torch.int32, device="cuda")
+    loss, lse = torch.empty(n, device="cuda"), torch.empty(n, device="cuda")
+    lib.linear_softmax_loss(loss, lse, x, w, label)
+    gw = torch.empty(v, h, device="cuda")
+    lib.linear_softmax_loss_grad(None, gw, x, w, label, lse, scale=1.0 / n)
+    z = (x.double() @ w[0].double()).max().item()
+    # all logits of a token are equal: p = 1 / v, off by what the two logits are (in runs of 8192 features, 512 additions)
+    rho = z * (512 + 64 + h / 8192 + h / 1024 + 16) * ADD + 2.0 ** -19
+    want = x.double().mean(0) / v
+    rows = torch.arange(v, device="cuda") != 3
+    within(gw[rows], want.expand(v - 1, h), (want * (rho + U[F16] + (n + 16) * ADD)).expand(v - 1, h), "gweight")
