@@ -73,7 +73,7 @@ inline void LinearSoftmaxLoss(Tensor<gpu, 1, float> loss, Tensor<gpu, 1, float> 
   const int sms = gpu_rt::CurrentDevice().sm_count;
   const cuda::vloss::Plan plan = cuda::vloss::PlanForward(q, sms);
   char *ws = gpu_rt::Workspace(workspace, workspace_bytes, static_cast<size_t>(plan.bytes), stream, "LinearSoftmaxLoss");
-  cuda::vloss::ForwardLaunch(loss.dptr_, lse.dptr_, q, plan, ws, sms, stream);
+  cuda::vloss::ForwardLaunch<0>(loss.dptr_, lse.dptr_, q, plan, ws, sms, stream);
 }
 
 template <typename Saver, typename DType, typename GType>
@@ -109,7 +109,7 @@ inline void LinearSoftmaxLossGrad(Tensor<gpu, 2, DType> gdata, Tensor<gpu, 2, GT
   g.gw_type = DataType<GType>::kFlag;
   g.gw_add = add;
   g.lse = lse.dptr_, g.gloss = gloss.dptr_, g.scale = scale;
-  cuda::vloss::BackwardLaunch(g, q, plan, ws, sms, stream);
+  cuda::vloss::BackwardLaunch<0>(g, q, plan, ws, sms, stream);
 }
 
 }  // namespace mshadow

@@ -1433,7 +1433,11 @@ inline int GroupOf(int64_t m_tiles, int64_t most) {
   return static_cast<int>(std::min<int64_t>(std::max<int64_t>(m_tiles, 1), most));
 }
 
+// The functions below that launch kernels are templates so that a program that includes the headers and calls no vocabulary
+// operator holds none of their kernels, and needs no architecture that has tcgen05.
+
 /*! \brief the weight rows [p0, p0 + rows) as the products read them: map over W itself, or over an aligned copy */
+template <int kUnused>
 inline CUtensorMap WeightMap(const Problem &q, const Plan &p, char *ws, int64_t p0, int64_t rows, int box_rows,
                              cudaStream_t stream, bool copy_now, int32_t *row0) {
   if (!p.copy_w) {
@@ -1443,7 +1447,7 @@ inline CUtensorMap WeightMap(const Problem &q, const Plan &p, char *ws, int64_t 
   uint16_t *w = reinterpret_cast<uint16_t *>(ws + p.w);
   if (copy_now) {
     const int64_t groups = Ceil(q.h, 8), total = rows * groups;  // below 2^31: a piece holds at most 2^30 elements
-    gpu_rt::LaunchAfterDrain(AlignRowsKernel<0>, dim3(static_cast<unsigned>(std::min<int64_t>(Ceil(total, 256), 4096))), dim3(256),
+    gpu_rt::LaunchAfterDrain(AlignRowsKernel<kUnused>, dim3(static_cast<unsigned>(std::min<int64_t>(Ceil(total, 256), 4096))), dim3(256),
                              0, stream, w, p.ld_w, q.w + p0 * q.ld_w, q.ld_w, total, gpu_rt::FastDiv(static_cast<uint32_t>(groups)),
                              static_cast<int>(q.h));
     MSHADOW_CUDA_POST_KERNEL_CHECK(AlignRowsKernel);
@@ -1452,6 +1456,7 @@ inline CUtensorMap WeightMap(const Problem &q, const Plan &p, char *ws, int64_t 
   return tc5::MatrixMap(w, q.type(), rows, q.h, p.ld_w, box_rows);
 }
 
+template <int kUnused>
 inline void PackLaunch(const Problem &q, const Plan &p, char *ws, PackArgs a, cudaStream_t stream) {
   a.x = q.x, a.ld_x = q.ld_x, a.label = q.label, a.ignore = q.ignore;
   a.n = static_cast<int32_t>(q.n), a.v = static_cast<int32_t>(q.v), a.h = static_cast<int32_t>(q.h);
@@ -1465,19 +1470,20 @@ inline void PackLaunch(const Problem &q, const Plan &p, char *ws, PackArgs a, cu
   if (p.pad_rows > kCountDirectly) {
     a.rows_per_cta = 256;
     a.counts = reinterpret_cast<float2 *>(ws + p.counts);
-    gpu_rt::LaunchAfterDrain(CountRowsKernel<0>, dim3(static_cast<unsigned>(p.pad_rows / 256)), dim3(256), 0, stream, a);
+    gpu_rt::LaunchAfterDrain(CountRowsKernel<kUnused>, dim3(static_cast<unsigned>(p.pad_rows / 256)), dim3(256), 0, stream, a);
     MSHADOW_CUDA_POST_KERNEL_CHECK(CountRowsKernel);
   }
-  gpu_rt::LaunchAfterDrain(PackRowsKernel<0>, dim3(static_cast<unsigned>(p.pad_rows / a.rows_per_cta)), dim3(256), 0, stream, a);
+  gpu_rt::LaunchAfterDrain(PackRowsKernel<kUnused>, dim3(static_cast<unsigned>(p.pad_rows / a.rows_per_cta)), dim3(256), 0, stream, a);
   MSHADOW_CUDA_POST_KERNEL_CHECK(PackRowsKernel);
 }
 
+template <int kUnused>
 inline void ForwardLaunch(float *loss, float *lse, const Problem &q, const Plan &p, char *ws, int sms, cudaStream_t stream) {
   if (p.pack) {
     PackArgs k = {};
     k.row_of = reinterpret_cast<int32_t *>(ws + p.row_of);
     k.loss = loss, k.lse_out = lse;
-    PackLaunch(q, p, ws, k, stream);
+    PackLaunch<kUnused>(q, p, ws, k, stream);
   }
   GemmArgs a = {};
   a.live = p.pack ? reinterpret_cast<const int32_t *>(ws + p.words) : nullptr;
@@ -1500,7 +1506,7 @@ inline void ForwardLaunch(float *loss, float *lse, const Problem &q, const Plan 
   const CUtensorMap mx = Aligned16(q.x, q.ld_x, 2) ? tc5::MatrixMap(q.x, q.type(), q.n, q.h, q.ld_x, 128) : ma;
   for (int64_t p0 = 0; p0 < q.v; p0 += p.piece) {
     const int64_t cols = std::min(p.piece, q.v - p0);
-    const CUtensorMap mb = WeightMap(q, p, ws, p0, cols, static_cast<int>(p.tile_n) / p.ctas, stream, true, &a.b_row0);
+    const CUtensorMap mb = WeightMap<kUnused>(q, p, ws, p0, cols, static_cast<int>(p.tile_n) / p.ctas, stream, true, &a.b_row0);
     a.cols = static_cast<int32_t>(cols);
     a.col0 = static_cast<int32_t>(p0);
     a.tile0 = static_cast<int32_t>(p0 / p.tile_n);
@@ -1531,6 +1537,7 @@ struct GradOut {
   float scale;
 };
 
+template <int kUnused>
 inline void BackwardLaunch(const GradOut &g, const Problem &q, const Plan &p, char *ws, int sms, cudaStream_t stream) {
   PackArgs k = {};
   k.pos_of = reinterpret_cast<int32_t *>(ws + p.pos_of);
@@ -1539,7 +1546,7 @@ inline void BackwardLaunch(const GradOut &g, const Problem &q, const Plan &p, ch
   k.row_scale = reinterpret_cast<float *>(ws + p.row_scale);
   // (bfloat16 has the exponents for a common scale; without the gradient of x there is no use for another)
   if (!q.bf16 && g.gloss != nullptr && g.gx != nullptr) k.row_down = reinterpret_cast<float *>(ws + p.row_down);
-  PackLaunch(q, p, ws, k, stream);
+  PackLaunch<kUnused>(q, p, ws, k, stream);
 
   const int32_t h_tiles = static_cast<int32_t>(p.ld_acc / kTileN);
   const int type = q.type();
@@ -1574,7 +1581,7 @@ inline void BackwardLaunch(const GradOut &g, const Problem &q, const Plan &p, ch
     a.run_steps = RunSteps(kDelta, false);
     a.group = GroupOf(m_tiles, 16);
     a.instr = tc5::InstrDesc(q.bf16, false, false, 128 * p.ctas, kTileN);
-    const CUtensorMap w_along = WeightMap(q, p, ws, p0, cols, kTileN / p.ctas, stream, true, &a.b_row0);
+    const CUtensorMap w_along = WeightMap<kUnused>(q, p, ws, p0, cols, kTileN / p.ctas, stream, true, &a.b_row0);
     if (p.ctas == 2 && WideFor(m_tiles * a.n_tiles, a.n_tiles, a.k_blocks, sms)) {
       a.n_tiles /= 2;
       LaunchGemm<kDelta, 2, true>(x_along, w_along, x_along_in_place, d_along, a, m_tiles * a.n_tiles, sms, stream);
@@ -1582,7 +1589,7 @@ inline void BackwardLaunch(const GradOut &g, const Problem &q, const Plan &p, ch
       Gemm<kDelta>(x_along, w_along, x_along_in_place, d_along, a, m_tiles * a.n_tiles, p.ctas, sms, stream);
     }
     if (g.gx != nullptr) {
-      const CUtensorMap w_across = WeightMap(q, p, ws, p0, cols, 64, stream, false, &a.b_row0);
+      const CUtensorMap w_across = WeightMap<kUnused>(q, p, ws, p0, cols, 64, stream, false, &a.b_row0);
       const CUtensorMap out = tc5::MatrixMap(acc, kFloat32, p.pad_rows, p.ld_acc, p.ld_acc, 128);
       const int64_t tile_n = kTileN * (p.wide_gx ? 2 : 1);
       const CUtensorMap spare =
@@ -1602,7 +1609,7 @@ inline void BackwardLaunch(const GradOut &g, const Problem &q, const Plan &p, ch
       else Gemm<kDataGrad>(d_along, w_across, spare, out, a, x_tiles * a.n_tiles, p.ctas_gx, sms, stream);
     }
     if (g.gw != nullptr && k.row_down != nullptr) {
-      gpu_rt::LaunchAfterDrain(CommonScaleKernel<0>, dim3(static_cast<unsigned>(std::min<int64_t>(Ceil(q.n, 8), 8 * sms))), dim3(256),
+      gpu_rt::LaunchAfterDrain(CommonScaleKernel<kUnused>, dim3(static_cast<unsigned>(std::min<int64_t>(Ceil(q.n, 8), 8 * sms))), dim3(256),
                                0, stream, reinterpret_cast<uint16_t *>(delta), p.piece, a.live,
                                static_cast<const float *>(k.row_down), static_cast<int>(cols));
       MSHADOW_CUDA_POST_KERNEL_CHECK(CommonScaleKernel);
@@ -1650,7 +1657,7 @@ inline void BackwardLaunch(const GradOut &g, const Problem &q, const Plan &p, ch
     f.bf16 = q.bf16, f.vec = Aligned16(g.gx, g.ld_gx, 2);
     f.groups = gpu_rt::FastDiv(static_cast<uint32_t>(Ceil(q.h, 8)));
     const int64_t blocks = std::min<int64_t>(Ceil(Ceil(q.n, 4) * Ceil(q.h, 8), 256), 4 * sms);
-    gpu_rt::LaunchAfterDrain(DataGradFinishKernel<0>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, f);
+    gpu_rt::LaunchAfterDrain(DataGradFinishKernel<kUnused>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, f);
     MSHADOW_CUDA_POST_KERNEL_CHECK(DataGradFinishKernel);
   }
 }

@@ -1303,3 +1303,19 @@ def test_gradient_over_many_features(lib, n, v, h):
     want = x.double().mean(0) / v
     rows = torch.arange(v, device="cuda") != 3
     within(gw[rows], want.expand(v - 1, h), (want * (rho + U[F16] + (n + 16) * ADD)).expand(v - 1, h), "gweight")
+
+
+def test_headers_without_the_operators(tmp_path):
+    """A program that includes the headers and calls none of these operators builds for architectures without tcgen05."""
+    import os
+    import shutil
+    import subprocess
+    nvcc = shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"
+    if not os.path.exists(nvcc):
+        pytest.skip("nvcc not found")
+    src = tmp_path / "user.cu"
+    src.write_text("#include <mshadow/tensor.h>\nint rows(mshadow::Tensor<mshadow::gpu, 2, float> t) { return t.size(0); }\n")
+    inc = os.path.join(os.path.dirname(os.path.abspath(mshadow_b200.__file__)), "include")
+    done = subprocess.run([nvcc, "-std=c++11", "-arch=sm_100", "-I" + inc, "-cubin", str(src), "-o", str(tmp_path / "user.cubin")],
+                          capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
