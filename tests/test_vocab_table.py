@@ -1319,3 +1319,37 @@ def test_headers_without_the_operators(tmp_path):
     done = subprocess.run([nvcc, "-std=c++11", "-arch=sm_100", "-I" + inc, "-cubin", str(src), "-o", str(tmp_path / "user.cubin")],
                           capture_output=True, text=True, timeout=300)
     assert done.returncode == 0, done.stderr[-2000:]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,v,h,gw_dtype", [(20000, 3000, 256, F32), (20000, 3000, 265, None), (700, 70000, 136, F32)])
+def test_long_sums_of_unlike_tokens_repeat(lib, n, v, h, gw_dtype):
+    """Several runs and tokens with scales of their own: the same bits whatever the workspace held, and from a graph."""
+    x, w, label = problem(n, v, h, F16, 23, ignored=0.1)
+    gloss = torch.exp2(-20.0 * torch.rand(n, device="cuda", generator=gen(1)))
+    loss, lse = torch.empty(n, device="cuda"), torch.empty(n, device="cuda")
+    lib.linear_softmax_loss(loss, lse, x, w, label)
+    gx, gw = torch.empty_like(x), torch.empty(v, h, dtype=gw_dtype or F16, device="cuda")
+    ws = torch.empty(lib.linear_softmax_loss_workspace(n, v, h, gradient=True), dtype=torch.uint8, device="cuda")
+
+    def run():
+        lib.linear_softmax_loss_grad(gx, gw, x, w, label, lse, gloss, 0.01, workspace=ws,
+                                     stream=torch.cuda.current_stream().cuda_stream)
+
+    seen = []
+    for fill in (0, 0xff):
+        ws.fill_(fill)
+        run()
+        seen.append((gx.clone(), gw.clone()))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run()
+    ws.fill_(0xff)
+    gx.fill_(9)
+    gw.fill_(9)
+    graph.replay()
+    torch.cuda.synchronize()
+    seen.append((gx, gw))
+    for other in seen[1:]:
+        assert torch.equal(other[0], seen[0][0]) and torch.equal(other[1], seen[0][1])
+    assert torch.isfinite(gx).all() and torch.isfinite(gw).all()
