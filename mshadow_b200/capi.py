@@ -477,7 +477,8 @@ class Library:
         return dst
 
     def linear_softmax_loss_workspace(self, n, v, h, dtype=None, gradient=False):
-        """Bytes of workspace of linear_softmax_loss (gradient=True: of linear_softmax_loss_grad, enough for both)."""
+        """Bytes of workspace of linear_softmax_loss (gradient=True: of linear_softmax_loss_grad, enough for both; the type does
+        not matter)."""
         out, loss = i64(), i64()
         self.call("msb_linear_softmax_loss_workspace", n, v, h, 0, C.byref(loss))
         if not gradient:

@@ -9,8 +9,8 @@
  * binary32 ones, summed in binary32 and rounded once; a scale; and an index outside the table is a
  * token without a row -- padding, or a row another GPU holds -- which looks up zeros and adds nothing
  * (take and AddTakeGrad clip it to the table).  EmbedTakeGrad sorts the indices itself; Saver is sv::saveto
- * (every row of dst is written, zeros where no index names it) or sv::plusto (rows that are not named stay
- * as they are, bit for bit).  dst shares no element with another operand.  Equal calls give equal bits.
+ * (every row of dst is written, zeros where no index names it) or sv::plusto (rows that are not named are not
+ * written).  dst shares no element with another operand.  Equal calls give equal bits.
  *
  * `workspace`: at least EmbedTakeGradWorkspace() bytes of device memory, or NULL for the stream's scratch memory.
  * A call that is captured into a graph must bring its own.

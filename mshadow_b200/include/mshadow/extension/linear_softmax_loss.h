@@ -11,17 +11,24 @@
  *
  * Composed from the framework's other operators this is a matrix product, Softmax, and SoftmaxGrad or
  * SmoothSoftmaxGrad (mshadow/tensor_gpu-inl.h:157-214; the smoothing is theirs) with two more products,
- * and holds tokens x vocabulary logits and probabilities.  Here the products run in the same kernels
- * and what is held is a piece of the vocabulary of bounded size.
+ * and holds tokens x vocabulary logits and probabilities.  Here the products run in the same kernels.
+ * What the gradient holds is a piece of the vocabulary of bounded size; the loss holds 16 bytes for each token
+ * and 256 classes (24 with smoothing).
  *
  * data (n x h) and weight (v x h) are binary16 or bfloat16; loss and lse are binary32; gdata has the type of
- * data; gweight that type or float.  Sums are binary32.  A token whose label equals ignore_label, or lies
+ * data; gweight that type or float.  Sums are binary32, of products that the tensor cores add: they cut off where
+ * a rounding would round, which is bounded by adding long sums in runs (sums of one sign come out up to 6e-5 too
+ * small, 1.2e-4 where the result has 16 bits).  In the gradients each entry of softmax - target is rounded to the operands'
+ * type between the two products, whatever the type of gweight.  A class whose weight is -infinity has probability 0
+ * and a zero row in gweight; gdata is NaN then, as 0 * infinity is.  In binary16 what a token adds to gweight is lost below
+ * 2^-39 of the largest finite |gloss| / (1 - smooth).  float gradients that are added to may lose what they hold below
+ * 2^-126.  A token whose label equals ignore_label, or lies
  * outside [0, v), contributes nothing: its loss and lse are 0, its gdata row is zero, and whatever
  * its data row holds reaches no result.  gdata or gweight may be empty (dptr_ == NULL): not computed.  Outputs share
- * no element with other operands.  Equal calls give equal bits.
+ * no element with other operands, but gdata may lie in the memory of data.  Equal calls give equal bits.
  *
  * `workspace`: at least LinearSoftmaxLossWorkspace() bytes of device memory, or NULL for the stream's scratch memory.
- * A call that is captured into a graph must bring its own.
+ * A call that is captured into a graph must bring its own, and another call on the device precede it.
  */
 #ifndef MSHADOW_EXTENSION_LINEAR_SOFTMAX_LOSS_H_
 #define MSHADOW_EXTENSION_LINEAR_SOFTMAX_LOSS_H_
