@@ -144,7 +144,7 @@ struct GemmArgs {
   int out_vec;           // rows of `out` start on 16-byte boundaries
   int out_tiled;         // written by tiled copies (map_out)
   int run_steps;         // RunSteps
-  float4 *earlier;       // sums of earlier runs (EarlierOf), or null: every contraction is one run
+  float4 *earlier;       // kRuns: sums of earlier runs (EarlierOf)
   int *status;
 };
 
@@ -245,7 +245,7 @@ struct Half {
   int col;           // first column of the half, within the piece
   uint32_t boxes, box;  // shared memory of the group's first outgoing box; which one is filled next
   int group, thread; // 0 / 1; thread of the group: 0 .. 127
-  float4 *earlier;   // this thread's sums of the tile's earlier runs, or null: there are none
+  float4 *earlier;   // kRuns: this thread's sums of the tile's earlier runs, or null: there are none
   __device__ __forceinline__ uint32_t Box() const { return boxes + box * 2 * kBoxOut; }
 };
 
@@ -257,9 +257,9 @@ __device__ __forceinline__ float4 *EarlierOf(float4 *all, int set) {
   return all + (static_cast<int64_t>(blockIdx.x) * 2 + set) * (kHalfN / 4) * kEarlierStep + (threadIdx.x - 128);
 }
 /*! \brief accumulators of the columns from `col` on, plus those of the earlier runs */
-template <int kColumns>
+template <bool kRuns, int kColumns>
 __device__ __forceinline__ void AddEarlier(const Half &t, int col, uint32_t (&r)[kColumns]) {
-  if (t.earlier == nullptr) return;
+  if (!kRuns || t.earlier == nullptr) return;
 #pragma unroll
   for (int q = 0; q < kColumns / 4; ++q) {
     const float4 e = t.earlier[(col / 4 + q) * kEarlierStep];
@@ -276,7 +276,7 @@ __device__ __forceinline__ void KeepHalf(const Half &t, float4 *keep) {
     uint32_t r[32];
     tc5::LoadColumns(t.acc + b * 32, r);
     tc5::WaitColumns(r);
-    AddEarlier(t, b * 32, r);
+    AddEarlier<true>(t, b * 32, r);
 #pragma unroll
     for (int q = 0; q < 8; ++q) {
       keep[(b * 8 + q) * kEarlierStep] = make_float4(__uint_as_float(r[4 * q]), __uint_as_float(r[4 * q + 1]),
@@ -408,7 +408,7 @@ __device__ __forceinline__ void DeltaColumns(const uint32_t (&r)[32], int limit,
   for (int i = 0; i < 16; ++i) out[i] = PackPair(d[2 * i], d[2 * i + 1], a.bf16);
 }
 
-template <int kBoxes>
+template <int kBoxes, bool kRuns>
 __device__ __forceinline__ void DeltaHalf(Half &t, int limit, int label, float lse2, float scale, const CUtensorMap *map,
                                           int row0, const GemmArgs &a) {
 #pragma unroll 1
@@ -418,8 +418,8 @@ __device__ __forceinline__ void DeltaHalf(Half &t, int limit, int label, float l
     tc5::LoadColumns(t.acc + b * 64 + 32, r1);
     tc5::WaitColumns(r0);
     tc5::WaitColumns(r1);
-    AddEarlier(t, b * 64, r0);
-    AddEarlier(t, b * 64 + 32, r1);
+    AddEarlier<kRuns>(t, b * 64, r0);
+    AddEarlier<kRuns>(t, b * 64 + 32, r1);
     DeltaColumns(r0, limit - b * 64, label - b * 64, lse2, scale, a, p0);
     DeltaColumns(r1, limit - b * 64 - 32, label - b * 64 - 32, lse2, scale, a, p1);
     BoxFree<kBoxes>(&t);
@@ -433,14 +433,14 @@ __device__ __forceinline__ void DeltaHalf(Half &t, int limit, int label, float l
 }
 
 /*! \brief the half tile as binary32, times `factor`, stored or added */
-template <int kBoxes, bool kAdd>
+template <int kBoxes, bool kRuns, bool kAdd>
 __device__ __forceinline__ void FloatHalf(Half &t, float factor, const CUtensorMap *map, int x, int y) {
 #pragma unroll 1
   for (int b = 0; b < kHalfN / 32; ++b) {
     uint32_t r[32];
     tc5::LoadColumns(t.acc + b * 32, r);
     tc5::WaitColumns(r);
-    AddEarlier(t, b * 32, r);
+    AddEarlier<kRuns>(t, b * 32, r);
 #pragma unroll
     for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * factor);
     BoxFree<kBoxes>(&t);
@@ -451,7 +451,7 @@ __device__ __forceinline__ void FloatHalf(Half &t, float factor, const CUtensorM
 }
 
 /*! \brief the half tile in the operands' type, times `factor` */
-template <int kBoxes>
+template <int kBoxes, bool kRuns>
 __device__ __forceinline__ void PackedHalf(Half &t, float factor, int bf16, const CUtensorMap *map, int row0) {
 #pragma unroll 1
   for (int b = 0; b < kHalfN / 64; ++b) {
@@ -460,8 +460,8 @@ __device__ __forceinline__ void PackedHalf(Half &t, float factor, int bf16, cons
     tc5::LoadColumns(t.acc + b * 64 + 32, r1);
     tc5::WaitColumns(r0);
     tc5::WaitColumns(r1);
-    AddEarlier(t, b * 64, r0);
-    AddEarlier(t, b * 64 + 32, r1);
+    AddEarlier<kRuns>(t, b * 64, r0);
+    AddEarlier<kRuns>(t, b * 64 + 32, r1);
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       r0[i] = PackPair(__uint_as_float(r0[2 * i]) * factor, __uint_as_float(r0[2 * i + 1]) * factor, bf16);
@@ -582,7 +582,8 @@ __device__ __forceinline__ void WeightRows(const uint32_t (&r)[32], const Half &
  *  of 1024 elements up in registers: over 4096 elements the loss was off by 1.8e-6 of its value in one run, by 4e-7 in
  *  these, which cost 1 % of the time (plain binary32: 6e-7 there, 3e-8 to 4e-8 at 1000 to 2000 features; runs of 512:
  *  2.5e-7 and another 3 %; of 256: 17 %).  The other modes keep the sums of a tile's runs in memory (38 MB for all CTAs,
- *  written and read once per run, some 20 000 cycles); most calls have one run there.  Without runs the gradient of W of a
+ *  written and read once per run, some 20 000 cycles; kRuns, for calls whose contraction is longer than one: kernels apart,
+ *  since the registers of that sum keep the next kernel off the SM, 1 to 3 us of a small call).  Without runs the gradient of W of a
  *  class that 65536 tokens name was off by 4.2e-4 of its value, and by 1.7e-3 at 262144, however well the rounding of
  *  d' averages out, now by 5e-5; 1 % of the time of 2048 x 32000 x 4096, 1.5 % of 32768 x 32000 x 2048 with the gradient of
  *  W as binary32 (runs of 8192 for all: 3.5 % of 8192 x 131072 x 4096).
@@ -591,7 +592,7 @@ __device__ __forceinline__ void WeightRows(const uint32_t (&r)[32], const Half &
  *  and, where A is d', from memory; in return the products wait while a tile is emptied.  For long contractions (not
  *  in kStat, whose runs would be emptied too often).
  */
-template <int kMode, int kCtas, bool kWide>
+template <int kMode, int kCtas, bool kWide, bool kRuns>
 __global__ void __launch_bounds__(kThreads, 1)
 VocabGemmKernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                 const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_out, const GemmArgs a) {
@@ -698,7 +699,7 @@ VocabGemmKernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         const Unit u = UnitOf(w, cut, m_tiles, a.n_tiles, a.group);
         const int k_first = u.slice * k_blocks / u.parts, k_count = (u.slice + 1) * k_blocks / u.parts - k_first;
         if (k_count == 0) continue;  // the last piece of the vocabulary may have fewer steps than there are parts
-        const int runs = (k_count + a.run_steps - 1) / a.run_steps;
+        const int runs = kRuns || kMode == kStat ? (k_count + a.run_steps - 1) / a.run_steps : 1;
         for (int run = 0; ok && run < runs; ++run, turn += S::kSets) {
           const int k_begin = k_first + RunBegin<kMode>(run, runs, k_count, a.run_steps);
           const int k_end = k_first + RunBegin<kMode>(run + 1, runs, k_count, a.run_steps);
@@ -758,7 +759,7 @@ VocabGemmKernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
       const Unit u = UnitOf(w, cut, m_tiles, a.n_tiles, a.group);
       const int k_count = (u.slice + 1) * k_blocks / u.parts - u.slice * k_blocks / u.parts;
       if (kMode == kDataGrad && k_count == 0) continue;
-      const int runs = (k_count + a.run_steps - 1) / a.run_steps;
+      const int runs = kRuns || kMode == kStat ? (k_count + a.run_steps - 1) / a.run_steps : 1;
       const int row0 = u.m * tile_m + static_cast<int>(rank) * 128;
       t.row = row0 + t.thread;
       t.col = u.n * tile_n + t.group * kHalfN;
@@ -790,14 +791,14 @@ VocabGemmKernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
       for (int i = 0; i < runs * S::kSets; ++i) {
         const int run = i / S::kSets, set = i - run * S::kSets;
         t.col = u.n * tile_n + t.group * kHalfN + set * kTileN;
-        t.earlier = run > 0 ? EarlierOf(a.earlier, set) : nullptr;
+        if (kRuns) t.earlier = run > 0 ? EarlierOf(a.earlier, set) : nullptr;
         ready();
-        if (run < runs - 1) {
+        if (kRuns && run < runs - 1) {
           KeepHalf(t, EarlierOf(a.earlier, set));
         } else if (kMode == kDelta) {
           // rows past the live ones: no column of theirs exists, so that d' is zero there whatever the logits of a zero data
           // row are (NaN beside a class with an infinite weight); the product for grad W reads them up to a whole step
-          DeltaHalf<S::kBoxes>(t, t.row < live ? a.cols - t.col : 0, label < 0 ? -1 : label - a.col0 - t.col, a.lse2[t.row],
+          DeltaHalf<S::kBoxes, kRuns>(t, t.row < live ? a.cols - t.col : 0, label < 0 ? -1 : label - a.col0 - t.col, a.lse2[t.row],
                                a.row_scale[t.row], &map_out, row0, a);
         } else if (kMode == kDataGrad) {
           // a whole tile goes to its place in the gradient, a part of one to a tile of its own beside it
@@ -805,21 +806,21 @@ VocabGemmKernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
           const CUtensorMap *to = whole ? &map_out : &map_x;
           const int x = whole ? t.col : t.group * kHalfN + set * kTileN;
           const int y = whole ? row0 : u.spare * tile_m + static_cast<int>(rank) * 128;
-          if (a.accumulate) FloatHalf<S::kBoxes, true>(t, 1.0f, to, x, y);
-          else FloatHalf<S::kBoxes, false>(t, 1.0f, to, x, y);
+          if (a.accumulate) FloatHalf<S::kBoxes, kRuns, true>(t, 1.0f, to, x, y);
+          else FloatHalf<S::kBoxes, kRuns, false>(t, 1.0f, to, x, y);
         } else {
           const float inv = a.inv_scale[0];
           if (a.out_tiled) {
-            if (a.out_type == kFloat32 && a.out_add) FloatHalf<S::kBoxes, true>(t, inv, &map_out, t.col, row0);
-            else if (a.out_type == kFloat32) FloatHalf<S::kBoxes, false>(t, inv, &map_out, t.col, row0);
-            else PackedHalf<S::kBoxes>(t, inv, a.out_type == kBfloat16, &map_out, row0);
+            if (a.out_type == kFloat32 && a.out_add) FloatHalf<S::kBoxes, kRuns, true>(t, inv, &map_out, t.col, row0);
+            else if (a.out_type == kFloat32) FloatHalf<S::kBoxes, kRuns, false>(t, inv, &map_out, t.col, row0);
+            else PackedHalf<S::kBoxes, kRuns>(t, inv, a.out_type == kBfloat16, &map_out, row0);
           } else {
 #pragma unroll 1
             for (int c = 0; c < kHalfN / 32; ++c) {
               uint32_t r[32];
               tc5::LoadColumns(t.acc + c * 32, r);
               tc5::WaitColumns(r);
-              AddEarlier(t, c * 32, r);
+              AddEarlier<kRuns>(t, c * 32, r);
               if (!a.out_vec) WeightRows(r, t, row0, t.col + c * 32, inv, a);
               else if (t.row < a.out_rows) WeightColumns(r, t.row, t.col + c * 32, inv, a);
             }
@@ -1133,7 +1134,7 @@ struct FinishArgs {
   int n_tiles, tile_n, group, k_plan, room, slots, ctas;  // of the kernel that wrote the parts
   float step_cycles, tile_cycles;
   const int32_t *pos_of;
-  const float *inv_scale, *row_down;  // (row_down may be null)
+  const float *inv_scale, *row_down;
   uint16_t *out;
   int64_t ld_out;
   int32_t n, h;
@@ -1145,8 +1146,9 @@ struct FinishArgs {
  * \brief gradient of x: parts of the contraction added in order, rounded once, rows back in token order.  A thread keeps
  *  its eight columns and takes four rows at a time, so that what it computes about tiles is little and
  *  eight 16-byte loads are in flight (a CTA for each row: 54 us for 8192 x 2560; so: 42 us, 3.8 TB/s).
+ *  kOwnScales: rows of d' had scales of their own.
  */
-template <int kUnused>
+template <bool kOwnScales>
 __global__ void __launch_bounds__(256) DataGradFinishKernel(const FinishArgs a) {
   gpu_rt::GridDependencySync();
   constexpr int kRows = 4;
@@ -1182,6 +1184,7 @@ __global__ void __launch_bounds__(256) DataGradFinishKernel(const FinishArgs a) 
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[r][j] = 0.0f;
     }
+#pragma unroll 4  // (two at a time, as the compiler would have it: 16 tokens 19.5 -> 22 us)
     for (int s = 0; s < most; ++s) {
       float4 lo[kRows], hi[kRows];
 #pragma unroll
@@ -1202,9 +1205,10 @@ __global__ void __launch_bounds__(256) DataGradFinishKernel(const FinishArgs a) 
     for (int r = 0; r < kRows; ++r) {
       if (i0 + r >= a.n) break;
       uint16_t *out = a.out + (i0 + r) * a.ld_out;
-      const float down = a.row_down != nullptr && pos[r] >= 0 ? a.row_down[pos[r]] : 1.0f;
+      const float factor = parts[r] > 0 ? inv : 0.0f;  // (inv may be infinite, and the zeros of a row that does not count are zeros)
+      const float down = kOwnScales && parts[r] > 0 ? a.row_down[pos[r]] : 1.0f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[r][j] = pos[r] >= 0 ? v[r][j] * down * inv : 0.0f;  // (inv may be infinite)
+      for (int j = 0; j < 8; ++j) v[r][j] = kOwnScales ? v[r][j] * down * factor : v[r][j] * factor;
       if (a.vec && 8 * g + 8 <= a.h) {
         uint4 w;
         w.x = PackPair(v[r][0], v[r][1], a.bf16);
@@ -1391,10 +1395,10 @@ inline size_t WorkspaceNeed(int64_t n, int64_t v, int64_t h, bool gradient, int 
   return static_cast<size_t>(most);
 }
 
-template <int kMode, int kCtas, bool kWide>
-inline void LaunchGemm(const CUtensorMap &ma, const CUtensorMap &mb, const CUtensorMap &mx, const CUtensorMap &mo, const GemmArgs &args, int64_t units,
+template <int kMode, int kCtas, bool kWide, bool kRuns>
+inline void LaunchRuns(const CUtensorMap &ma, const CUtensorMap &mb, const CUtensorMap &mx, const CUtensorMap &mo, const GemmArgs &args, int64_t units,
                        int sms, cudaStream_t stream) {
-  auto kernel = VocabGemmKernel<kMode, kCtas, kWide>;
+  auto kernel = VocabGemmKernel<kMode, kCtas, kWide, kRuns>;
   const size_t smem = StageShape<kMode, kCtas, kWide>::kSmem;
   gpu_rt::AllowSharedMemory(kernel, smem);
   cudaLaunchConfig_t cfg = {};
@@ -1417,11 +1421,22 @@ inline void LaunchGemm(const CUtensorMap &ma, const CUtensorMap &mb, const CUten
   MSHADOW_CUDA_POST_KERNEL_CHECK(VocabGemmKernel);
 }
 
+/*! \brief `steps`: of the longest contraction, which may be shorter on the device where not all tokens count */
+template <int kMode, int kCtas, bool kWide>
+inline void LaunchGemm(const CUtensorMap &ma, const CUtensorMap &mb, const CUtensorMap &mx, const CUtensorMap &mo, const GemmArgs &args,
+                       int64_t steps, int64_t units, int sms, cudaStream_t stream) {
+  if (kMode != kStat && steps > args.run_steps) {
+    LaunchRuns<kMode, kCtas, kWide, kMode != kStat>(ma, mb, mx, mo, args, units, sms, stream);
+  } else {
+    LaunchRuns<kMode, kCtas, kWide, false>(ma, mb, mx, mo, args, units, sms, stream);
+  }
+}
+
 template <int kMode>
 inline void Gemm(const CUtensorMap &ma, const CUtensorMap &mb, const CUtensorMap &mx, const CUtensorMap &mo, const GemmArgs &args,
-                 int64_t units, int ctas, int sms, cudaStream_t stream) {
-  if (ctas == 2) LaunchGemm<kMode, 2, false>(ma, mb, mx, mo, args, units, sms, stream);
-  else LaunchGemm<kMode, 1, false>(ma, mb, mx, mo, args, units, sms, stream);
+                 int64_t steps, int64_t units, int ctas, int sms, cudaStream_t stream) {
+  if (ctas == 2) LaunchGemm<kMode, 2, false>(ma, mb, mx, mo, args, steps, units, sms, stream);
+  else LaunchGemm<kMode, 1, false>(ma, mb, mx, mo, args, steps, units, sms, stream);
 }
 
 /*!
@@ -1511,7 +1526,7 @@ inline void ForwardLaunch(float *loss, float *lse, const Problem &q, const Plan 
     a.col0 = static_cast<int32_t>(p0);
     a.tile0 = static_cast<int32_t>(p0 / p.tile_n);
     a.n_tiles = static_cast<int32_t>(Ceil(cols, p.tile_n));
-    Gemm<kStat>(ma, mb, mx, mb, a, m_tiles * a.n_tiles, p.ctas, sms, stream);
+    Gemm<kStat>(ma, mb, mx, mb, a, a.k_blocks, m_tiles * a.n_tiles, p.ctas, sms, stream);
   }
   JoinArgs j = {};
   j.live = a.live, j.tokens = a.tokens, j.parts = static_cast<int32_t>(2 * p.tiles), j.v = static_cast<int32_t>(q.v);
@@ -1584,9 +1599,9 @@ inline void BackwardLaunch(const GradOut &g, const Problem &q, const Plan &p, ch
     const CUtensorMap w_along = WeightMap<kUnused>(q, p, ws, p0, cols, kTileN / p.ctas, stream, true, &a.b_row0);
     if (p.ctas == 2 && WideFor(m_tiles * a.n_tiles, a.n_tiles, a.k_blocks, sms)) {
       a.n_tiles /= 2;
-      LaunchGemm<kDelta, 2, true>(x_along, w_along, x_along_in_place, d_along, a, m_tiles * a.n_tiles, sms, stream);
+      LaunchGemm<kDelta, 2, true>(x_along, w_along, x_along_in_place, d_along, a, a.k_blocks, m_tiles * a.n_tiles, sms, stream);
     } else {
-      Gemm<kDelta>(x_along, w_along, x_along_in_place, d_along, a, m_tiles * a.n_tiles, p.ctas, sms, stream);
+      Gemm<kDelta>(x_along, w_along, x_along_in_place, d_along, a, a.k_blocks, m_tiles * a.n_tiles, p.ctas, sms, stream);
     }
     if (g.gx != nullptr) {
       const CUtensorMap w_across = WeightMap<kUnused>(q, p, ws, p0, cols, 64, stream, false, &a.b_row0);
@@ -1605,8 +1620,8 @@ inline void BackwardLaunch(const GradOut &g, const Problem &q, const Plan &p, ch
       a.accumulate = p0 > 0;
       a.group = GroupOf(x_tiles, 8);
       a.instr = tc5::InstrDesc(q.bf16, false, true, 128 * p.ctas_gx, kTileN);
-      if (p.wide_gx) LaunchGemm<kDataGrad, 2, true>(d_along, w_across, spare, out, a, x_tiles * a.n_tiles, sms, stream);
-      else Gemm<kDataGrad>(d_along, w_across, spare, out, a, x_tiles * a.n_tiles, p.ctas_gx, sms, stream);
+      if (p.wide_gx) LaunchGemm<kDataGrad, 2, true>(d_along, w_across, spare, out, a, a.k_blocks, x_tiles * a.n_tiles, sms, stream);
+      else Gemm<kDataGrad>(d_along, w_across, spare, out, a, a.k_blocks, x_tiles * a.n_tiles, p.ctas_gx, sms, stream);
     }
     if (g.gw != nullptr && k.row_down != nullptr) {
       gpu_rt::LaunchAfterDrain(CommonScaleKernel<kUnused>, dim3(static_cast<unsigned>(std::min<int64_t>(Ceil(q.n, 8), 8 * sms))), dim3(256),
@@ -1638,9 +1653,9 @@ inline void BackwardLaunch(const GradOut &g, const Problem &q, const Plan &p, ch
       const int64_t tiles = static_cast<int64_t>(a.m_tiles) * h_tiles;
       if (ctas == 2 && WideFor(tiles, h_tiles, Ceil(q.n, kStepK), sms)) {
         a.n_tiles = h_tiles / 2;
-        LaunchGemm<kWeightGrad, 2, true>(d_across, x_across, x_across_in_place, out, a, tiles / 2, sms, stream);
+        LaunchGemm<kWeightGrad, 2, true>(d_across, x_across, x_across_in_place, out, a, Ceil(q.n, kStepK), tiles / 2, sms, stream);
       } else {
-        Gemm<kWeightGrad>(d_across, x_across, x_across_in_place, out, a, tiles, ctas, sms, stream);
+        Gemm<kWeightGrad>(d_across, x_across, x_across_in_place, out, a, Ceil(q.n, kStepK), tiles, ctas, sms, stream);
       }
     }
   }
@@ -1657,7 +1672,9 @@ inline void BackwardLaunch(const GradOut &g, const Problem &q, const Plan &p, ch
     f.bf16 = q.bf16, f.vec = Aligned16(g.gx, g.ld_gx, 2);
     f.groups = gpu_rt::FastDiv(static_cast<uint32_t>(Ceil(q.h, 8)));
     const int64_t blocks = std::min<int64_t>(Ceil(Ceil(q.n, 4) * Ceil(q.h, 8), 256), 4 * sms);
-    gpu_rt::LaunchAfterDrain(DataGradFinishKernel<kUnused>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, f);
+    const dim3 grid(static_cast<unsigned>(blocks));
+    if (f.row_down != nullptr) gpu_rt::LaunchAfterDrain(DataGradFinishKernel<true>, grid, dim3(256), 0, stream, f);
+    else gpu_rt::LaunchAfterDrain(DataGradFinishKernel<false>, grid, dim3(256), 0, stream, f);
     MSHADOW_CUDA_POST_KERNEL_CHECK(DataGradFinishKernel);
   }
 }
