@@ -582,11 +582,11 @@ __device__ __forceinline__ void WeightRows(const uint32_t (&r)[32], const Half &
  *  of 1024 elements up in registers: over 4096 elements the loss was off by 1.8e-6 of its value in one run, by 4e-7 in
  *  these, which cost 1 % of the time (plain binary32: 6e-7 there, 3e-8 to 4e-8 at 1000 to 2000 features; runs of 512:
  *  2.5e-7 and another 3 %; of 256: 17 %).  The other modes keep the sums of a tile's runs in memory (38 MB for all CTAs,
- *  written and read once per run, some 20 000 cycles; kRuns, for calls whose contraction is longer than one: kernels apart,
- *  since the registers of that sum keep the next kernel off the SM, 1 to 3 us of a small call).  Without runs the gradient of W of a
- *  class that 65536 tokens name was off by 4.2e-4 of its value, and by 1.7e-3 at 262144, however well the rounding of
- *  d' averages out, now by 5e-5; 1 % of the time of 2048 x 32000 x 4096, 1.5 % of 32768 x 32000 x 2048 with the gradient of
- *  W as binary32 (runs of 8192 for all: 3.5 % of 8192 x 131072 x 4096).
+ *  written and read once per run, some 20 000 cycles).  Without runs the gradient of W of a class that 65536 tokens name was
+ *  off by 4.2e-4 of its value, and by 1.7e-3 at 262144, however well the rounding of d' averages out; now by 5e-5, for 1 %
+ *  of the time of 2048 x 32000 x 4096 and 1.5 % of 32768 x 32000 x 2048 with the gradient of W as binary32 (with runs of
+ *  8192 for all sums: 3.5 % of 8192 x 131072 x 4096).  kRuns: for calls with a contraction longer than a run; kernels apart,
+ *  since the registers of those sums keep the next kernel off the SM, 1 to 3 us of a small call.
  *
  *  kWide: both sets belong to one tile.  A step's rows of A then serve 512 columns, a quarter less is read from the L2
  *  and, where A is d', from memory; in return the products wait while a tile is emptied.  For long contractions (not
@@ -798,8 +798,8 @@ VocabGemmKernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         } else if (kMode == kDelta) {
           // rows past the live ones: no column of theirs exists, so that d' is zero there whatever the logits of a zero data
           // row are (NaN beside a class with an infinite weight); the product for grad W reads them up to a whole step
-          DeltaHalf<S::kBoxes, kRuns>(t, t.row < live ? a.cols - t.col : 0, label < 0 ? -1 : label - a.col0 - t.col, a.lse2[t.row],
-                               a.row_scale[t.row], &map_out, row0, a);
+          DeltaHalf<S::kBoxes, kRuns>(t, t.row < live ? a.cols - t.col : 0, label < 0 ? -1 : label - a.col0 - t.col,
+                                      a.lse2[t.row], a.row_scale[t.row], &map_out, row0, a);
         } else if (kMode == kDataGrad) {
           // a whole tile goes to its place in the gradient, a part of one to a tile of its own beside it
           const bool whole = u.parts == 1;
@@ -878,7 +878,7 @@ __device__ __forceinline__ float FiniteSize(float gloss) {
 }
 /*! \brief the power of two that brings `size` to [2^14, 2^15); 0 for one that has none */
 __device__ __forceinline__ int ScaleExponent(float size) {
-  return size > 0.0f && size < INFINITY ? min(100, max(-100, 14 - ilogbf(size))) : 0;
+  return size > 0.0f && size < INFINITY ? 14 - ilogbf(size) : 0;  // -113 .. 163
 }
 
 /*! \brief live rows, and the largest finite |gloss| among them, of every 256 tokens: for lists too long to be counted by each CTA below */
@@ -968,7 +968,7 @@ __global__ void __launch_bounds__(256) PackRowsKernel(const PackArgs a) {
         if (best - common > 6) own = min(best, common + 100);
         a.row_down[pos] = __int_as_float((127 + common - own) << 23);
       }
-      a.row_scale[pos] = factor * __int_as_float((127 + own) << 23);
+      a.row_scale[pos] = ldexpf(factor, own);
       a.lse2[pos] = a.lse[i] * kLog2e;
     }
   }
@@ -981,7 +981,7 @@ __global__ void __launch_bounds__(256) PackRowsKernel(const PackArgs a) {
   if (blockIdx.x == 0 && tid == 0) {
     a.words[0] = total;
     // (with no token that counts the sums are empty, and zero whatever the scale: 1 / 0 tokens, say)
-    reinterpret_cast<float *>(a.words)[1] = total > 0 ? a.scale * a.q_label * __int_as_float((127 - common) << 23) : 0.0f;
+    reinterpret_cast<float *>(a.words)[1] = total > 0 ? ldexpf(a.scale * a.q_label, -common) : 0.0f;
     a.words[2] = a.tiled && total == a.n;
   }
   if (a.tiled && total == a.n) return;

@@ -1353,3 +1353,13 @@ def test_long_sums_of_unlike_tokens_repeat(lib, n, v, h, gw_dtype):
     for other in seen[1:]:
         assert torch.equal(other[0], seen[0][0]) and torch.equal(other[1], seen[0][1])
     assert torch.isfinite(gx).all() and torch.isfinite(gw).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("size", [3e38, 1e34, 1e-30, 2e-38])
+def test_loss_grad_of_huge_and_tiny_gloss(lib, dtype, size):
+    """gloss near the ends of binary32's range, undone by the scale."""
+    x, w, label = problem(50, 300, 40, dtype, 4, ignored=0.1)
+    gloss = torch.full((50,), size, device="cuda") * (0.5 + 0.5 * torch.rand(50, device="cuda", generator=gen(3)))
+    check_grad(lib, x, w, label, gloss=gloss, scale=float(np.float32(0.25 / size)), gw_dtype=F32)
